@@ -304,6 +304,104 @@ p100_status p100_argmax(const float* x, int n, int batch, int* idx, float* val, 
 p100_status p100_peer_reduce_rmsnorm(float* x, const float* w, float eps, int k, void* x_q8_1, void* slots, int world,
                                      int rank, int* epoch, unsigned long long wait_ns, p100_stream_t stream);
 
+/* ------------------------------------------- paged cache: prompts and batches */
+/* A chunk of new tokens of one or more sequences through a K/V cache that is
+ * kept in pages: p100_paged_append puts the tokens' keys and values into the
+ * pages and their queries into a 16-bit tensor, p100_fa_paged attends,
+ * p100_logprobs scores the logits.  The reference has no paged cache and no
+ * prompt path, so these have no reference counterpart.  A single token per
+ * sequence is a chunk of one.
+ *
+ * Sequence s has the new tokens q_start[s] .. q_start[s + 1] - 1 (rows of
+ * qkv, q, o; q_start holds n_seq + 1 entries, never decreasing) and kv_len[s]
+ * tokens in all, the new ones last: new token i of n sits at position
+ * kv_len[s] - n + i.  Token j of the sequence lies in row j % page_size of
+ * page block_table[s * max_pages + j / page_size].  Table entries behind a
+ * sequence's last token are never read, nor is what its last page holds
+ * behind that token, and rows of q and o outside [q_start[0],
+ * q_start[n_seq]) stay as they were.  The three arrays are int32 in device
+ * memory and read when the kernels run, so a captured graph follows them.
+ *
+ * Lengths that decrease, exceed max_q, n_tokens or max_pages pages or are
+ * negative make p100_fa_paged do nothing; a page outside [0, n_pages) is
+ * neither read nor written (the results of its sequence are then undefined).
+ * Both raise P100_ERR_INVALID in p100_device_error(). */
+typedef enum p100_dtype { P100_F32 = 0, P100_F16 = 1, P100_BF16 = 2 } p100_dtype;
+typedef struct p100_paged_desc {
+    int n_seq;          /* sequences, at most P100_PAGED_MAX_SEQ */
+    int n_tokens;       /* rows of qkv, q and o                  */
+    int max_q;          /* new tokens of one sequence at most; 0 = n_tokens */
+    int n_head_q, n_head_kv, head_dim;   /* head_dim 64 or 128 */
+    int dtype;          /* of q, the pages and o: P100_F16 or P100_BF16 */
+    int page_size, n_pages, max_pages;   /* tokens a page, pages, table entries a sequence */
+    float scale;        /* of the scores; 0 means 1/sqrt(head_dim) */
+    float softcap;      /* cap tanh(score / cap); 0 means off      */
+    int causal;         /* bottom-right alignment                  */
+    int o_fp32;         /* o is fp32 (unrounded) instead of dtype  */
+    /* Strides in elements, multiples of 8; 0 = contiguous pages of
+     * [n_head_kv][page_size][head_dim] and rows of [n_head_q][head_dim].
+     * K and V share the pages' strides.  Pages of [page_size][n_head_kv]
+     * [head_dim]: head_stride = head_dim, token_stride = n_head_kv * head_dim. */
+    long long page_stride, head_stride, token_stride;
+    long long q_stride, o_stride;   /* between tokens */
+} p100_paged_desc;
+#define P100_PAGED_MAX_SEQ 1024
+
+/* For each new token, from its fused row qkv [n_head_q q | n_head_kv k |
+ * n_head_kv v] x head_dim of qkv_type (rows qkv_stride elements apart, 0 =
+ * contiguous): the q and k heads x times w / sqrt(mean(x^2) + eps) with the
+ * norm weights q_norm / k_norm [head_dim] (each NULL: no norm), rotated by
+ * rope_cs[position] (p100_rope_table's layout; NULL: no rotation; rope_half
+ * == 0 pairs values 2i and 2i + 1, != 0 values i and i + head_dim / 2), the v
+ * heads as they are; q to q, k and v to their row in the pages.  FP32
+ * arithmetic, one rounding (nearest even) to dtype.  A token whose position
+ * lies outside [0, max_pos) of the table or outside the block table is left
+ * out and raises P100_ERR_INVALID in p100_device_error(). */
+p100_status p100_paged_append(const p100_paged_desc* desc, const void* qkv, int qkv_type, long long qkv_stride,
+                              const float* q_norm, const float* k_norm, float eps, const float* rope_cs, int max_pos,
+                              int rope_half, const int* block_table, const int* q_start, const int* kv_len, void* q,
+                              void* k_pages, void* v_pages, p100_stream_t stream);
+
+/* Workspace bytes p100_fa_paged needs for desc on the current device: a
+ * function of the head dimension and the heads' layout, not of the lengths. */
+size_t p100_fa_paged_workspace_size(const p100_paged_desc* desc);
+/* Makes a workspace ready for its first use (p100_fa_paged leaves it ready).
+ * Calls that may run at the same time need a workspace each. */
+p100_status p100_fa_paged_workspace_init(void* ws, size_t ws_bytes, p100_stream_t stream);
+/* Attention of the new tokens over their sequences' cached tokens, their own
+ * (appended before) among them: query head h reads kv head h / (n_head_q /
+ * n_head_kv); with causal, new token i of n sees keys [0, kv_len - n + i],
+ * without it all kv_len.  Scores, softmax statistics and sums are FP32; the
+ * probabilities are rounded once to dtype for the product with V.  A row that
+ * sees no key gives o = 0 and lse = -inf.  Within [0, kv_len), values that
+ * are not finite reach the rows whose tile holds them even where causal hides
+ * them.  lse [n_tokens][n_head_q] (natural log) may be NULL.
+ * Results do not depend on the order in which blocks run. */
+p100_status p100_fa_paged(const p100_paged_desc* desc, const void* q, const void* k_pages, const void* v_pages,
+                          const int* block_table, const int* q_start, const int* kv_len, void* o, float* lse, void* ws,
+                          size_t ws_bytes, p100_stream_t stream);
+
+/* Scores rows of n logits (dtype P100_F32, P100_F16 or P100_BF16, rows
+ * row_stride elements apart, 0 = n) in one read, every sum in FP32:
+ *   logprob[r] = x[token[r]] - lse, entropy[r] = -sum p ln p,
+ *   rank[r]: how many logits are larger than the token's, or equal with a
+ *     lower index (0: the row's argmax),
+ *   top_index / top_logprob [rows][top_k]: the top_k (0 to 32) largest logits
+ *     in falling order, the lowest index first among equals.
+ * -inf and NaN logits are masked: probability 0, never an alternative (missing
+ * alternatives give index -1, -inf).  token[r] = -1 gives logprob 0 and rank
+ * -1, and so does any other index outside [0, n), which also raises
+ * P100_ERR_INVALID in p100_device_error().  A row with every logit masked has
+ * logprob -inf and entropy 0; one with +inf has NaN log probabilities and
+ * entropy.  token, logprob, entropy and rank may each be NULL; logprob and
+ * rank need token. */
+size_t p100_logprobs_workspace_size(int rows, int n, int dtype, int top_k);
+/* As p100_fa_paged_workspace_init; no bytes are needed when there are many rows. */
+p100_status p100_logprobs_workspace_init(void* ws, size_t ws_bytes, p100_stream_t stream);
+p100_status p100_logprobs(const void* logits, int dtype, int n, int rows, long long row_stride, const int* token,
+                          int top_k, float* logprob, float* entropy, int* rank, int* top_index, float* top_logprob,
+                          void* ws, size_t ws_bytes, p100_stream_t stream);
+
 /* --------------------------------------------------- batch-1 decoder */
 /* A Llama-3-shaped model with synthetic weights, decoded one token per
  * p100_decoder_step.  No reference counterpart (see above).  Every linear

@@ -17,6 +17,7 @@ import ctypes as C
 import pathlib
 import subprocess
 import threading
+import typing
 
 HERE = pathlib.Path(__file__).resolve().parent
 LIB_PATH = HERE / "lib" / "libp100_b200.so"
@@ -34,6 +35,10 @@ Q8_1_BLOCK_BYTES = 36
 QMV_PDL = 1
 QMV_TC = 2   # P100_QMV_TC: batch 2..16 on the tcgen05 kernel wherever it fits
 QMV_MMA = 4  # P100_QMV_MMA: batch 2..16 never on the tcgen05 kernel
+# Element types of the paged cache, fused rows and logits (p100_dtype).
+F32, F16, BF16 = 0, 1, 2
+PAGED_MAX_SEQ = 1024   # P100_PAGED_MAX_SEQ
+LOGPROBS_MAX_TOP = 32
 TP_PEER_MAX = 65536   # P100_TP_PEER_MAX: all-reduces up to this count may run over peer memory
 
 STATUS = {0: "P100_OK", 1: "P100_ERR_INVALID", 2: "P100_ERR_CUDA", 3: "P100_ERR_NCCL",
@@ -67,6 +72,32 @@ class AttnDesc(C.Structure):
                  softcap=0.0, causal=False, kv_splits=0, kv_head_stride=0, kv_batch_stride=0, kv_type=0):
         super().__init__(batch, n_head_q, n_head_kv, seq_q, seq_kv, d_qk, d_v, scale, softcap, int(bool(causal)),
                          kv_splits, kv_head_stride, kv_batch_stride, kv_type)
+
+
+class PagedDesc(C.Structure):
+    """p100_paged_desc: new tokens of a batch of sequences and their paged K/V cache."""
+    _fields_ = [("n_seq", C.c_int), ("n_tokens", C.c_int), ("max_q", C.c_int), ("n_head_q", C.c_int),
+                ("n_head_kv", C.c_int), ("head_dim", C.c_int), ("dtype", C.c_int), ("page_size", C.c_int),
+                ("n_pages", C.c_int), ("max_pages", C.c_int), ("scale", C.c_float), ("softcap", C.c_float),
+                ("causal", C.c_int), ("o_fp32", C.c_int), ("page_stride", C.c_longlong),
+                ("head_stride", C.c_longlong), ("token_stride", C.c_longlong), ("q_stride", C.c_longlong),
+                ("o_stride", C.c_longlong)]
+
+    def __init__(self, n_seq, n_tokens, n_head_q, n_head_kv, page_size, n_pages, max_pages, max_q=0, head_dim=128,
+                 dtype=F16, scale=0.0, softcap=0.0, causal=True, o_fp32=False, page_stride=0, head_stride=0,
+                 token_stride=0, q_stride=0, o_stride=0):
+        super().__init__(n_seq, n_tokens, max_q, n_head_q, n_head_kv, head_dim, dtype, page_size, n_pages, max_pages,
+                         scale, softcap, int(bool(causal)), int(bool(o_fp32)), page_stride, head_stride, token_stride,
+                         q_stride, o_stride)
+
+
+class LogProbs(typing.NamedTuple):
+    """p100_logprobs' outputs; a field that was not asked for is None."""
+    logprob: object       # fp32 [rows]
+    entropy: object       # fp32 [rows]
+    rank: object          # int32 [rows]
+    top_index: object     # int32 [rows, top_k]
+    top_logprob: object   # fp32 [rows, top_k]
 
 
 _lib = None
@@ -128,6 +159,14 @@ def _bind(lib):
         "p100_rope_kv_append": (ip, [vp, ip, ip, ip, vp, ip, vp, vp, vp, C.c_longlong, st]),
         "p100_swiglu_q8_1": (ip, [vp, ip, ip, vp, st]),
         "p100_argmax": (ip, [vp, ip, ip, vp, vp, st]),
+        "p100_paged_append": (ip, [vp, vp, ip, C.c_longlong, vp, vp, C.c_float, vp, ip, ip, vp, vp, vp, vp, vp, vp,
+                                   st]),
+        "p100_fa_paged_workspace_size": (sz, [vp]),
+        "p100_fa_paged_workspace_init": (ip, [vp, sz, st]),
+        "p100_fa_paged": (ip, [vp] * 9 + [vp, sz, st]),
+        "p100_logprobs_workspace_size": (sz, [ip, ip, ip, ip]),
+        "p100_logprobs_workspace_init": (ip, [vp, sz, st]),
+        "p100_logprobs": (ip, [vp, ip, ip, ip, C.c_longlong, vp, ip, vp, vp, vp, vp, vp, vp, sz, st]),
         "p100_decoder_create": (ip, [vp, vp, C.POINTER(vp)]),
         "p100_decoder_init_random": (ip, [vp, C.c_ulonglong]),
         "p100_decoder_fill_kv": (ip, [vp, ip, C.c_ulonglong, C.c_float]),
@@ -328,6 +367,199 @@ def fa_decode(desc, q, k, v, mask=None, o=None, lse=None, ws=None, stream=None):
     check(lib().p100_fa_decode(C.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(mask), _ptr(o), _ptr(lse),
                                _ptr(ws), nbytes, _stream(stream)))
     return o, lse
+
+
+# ------------------------------------------- paged cache: prompts and batches
+def _dtype_of(t, what):
+    torch = _torch()
+    kinds = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    if t.dtype not in kinds:
+        raise InvalidArgument(ERR_INVALID, f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
+    return kinds[t.dtype]
+
+
+def _need(t, what, dtype=None, values=None, dense=True):
+    """Refuses a tensor that a kernel of the current device could not read as it expects to."""
+    torch = _torch()
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise InvalidArgument(ERR_INVALID, f"{what} must be on the current device cuda:{torch.cuda.current_device()}, "
+                                           f"not {t.device}")
+    if dtype is not None and t.dtype != dtype:
+        raise InvalidArgument(ERR_INVALID, f"{what} must be {dtype}, not {t.dtype}")
+    if dense and not t.is_contiguous():
+        raise InvalidArgument(ERR_INVALID, f"{what} must be contiguous")
+    if values is not None and t.numel() < values:
+        raise InvalidArgument(ERR_INVALID, f"{what} needs {values} values, has {t.numel()}")
+
+
+def _alloc(stream, make):
+    """make() with its allocation and fill ordered on the stream of the call."""
+    torch = _torch()
+    if stream is None:
+        return make()
+    with torch.cuda.stream(stream):
+        return make()
+
+
+def _paged_type(desc):
+    torch = _torch()
+    return torch.bfloat16 if desc.dtype == BF16 else torch.float16
+
+
+def _rows_of(t, what, desc, dtype, stride):
+    """A q or o tensor: n_tokens rows of n_head_q * head_dim, `stride` elements apart."""
+    width = desc.n_head_q * desc.head_dim
+    _need(t, what, dtype, dense=False)
+    step = stride or width
+    if t.shape[0] < desc.n_tokens or t.numel() // max(1, t.shape[0]) < width:
+        raise InvalidArgument(ERR_INVALID, f"{what} needs {desc.n_tokens} rows of {width} values")
+    inner = 1
+    for size, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if size != 1 and st != inner:
+            raise InvalidArgument(ERR_INVALID, f"{what} must be contiguous within a row")
+        inner *= size
+    if desc.n_tokens > 1 and t.stride(0) != step:
+        raise InvalidArgument(ERR_INVALID, f"{what} has rows {t.stride(0)} elements apart, the descriptor {step}")
+
+
+def _pages_of(t, what, desc):
+    _need(t, what, _paged_type(desc), dense=False)
+    d = desc.head_dim
+    token = desc.token_stride or d
+    head = desc.head_stride or desc.page_size * d
+    page = desc.page_stride or desc.n_head_kv * desc.page_size * d
+    have = t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
+    need = ((desc.n_pages - 1) * page + (desc.n_head_kv - 1) * head + (desc.page_size - 1) * token + d
+            if desc.n_pages > 0 else 0)
+    if have < need:
+        raise InvalidArgument(ERR_INVALID, f"{what} needs {need} values behind its first, has {have}")
+
+
+def _lengths_of(desc, block_table, q_start, kv_len):
+    torch = _torch()
+    _need(block_table, "block_table", torch.int32, desc.n_seq * desc.max_pages)
+    _need(q_start, "q_start", torch.int32, desc.n_seq + 1)
+    _need(kv_len, "kv_len", torch.int32, desc.n_seq)
+
+
+def paged_append(desc, qkv, block_table, q_start, kv_len, k_pages, v_pages, rope_cs=None, q_norm=None, k_norm=None,
+                 eps=1e-5, rope_half=False, q=None, stream=None):
+    """New tokens into a paged cache (p100_paged_append): per-head norms and rotation of the fused rows qkv
+    [n_tokens, (n_head_q + 2 n_head_kv) head_dim] (float32, float16 or bfloat16), k and v to their pages, the
+    queries returned as q [n_tokens, n_head_q, head_dim] of the cache's type."""
+    torch = _torch()
+    width = (desc.n_head_q + 2 * desc.n_head_kv) * desc.head_dim
+    qkv_type = _dtype_of(qkv, "qkv")
+    _need(qkv, "qkv", dense=False)
+    if qkv.dim() != 2 or qkv.shape[0] < desc.n_tokens or qkv.shape[1] != width or (qkv.stride(1) != 1):
+        raise InvalidArgument(ERR_INVALID, f"qkv must be [{desc.n_tokens}, {width}] with contiguous rows")
+    _lengths_of(desc, block_table, q_start, kv_len)
+    _pages_of(k_pages, "k_pages", desc)
+    _pages_of(v_pages, "v_pages", desc)
+    for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if w is not None:
+            _need(w, what, torch.float32, desc.head_dim)
+    max_pos = 0
+    if rope_cs is not None:
+        _need(rope_cs, "rope_cs", torch.float32)
+        max_pos = rope_cs.numel() // desc.head_dim
+    if q is None:
+        q = _alloc(stream, lambda: torch.empty_strided((desc.n_tokens, desc.n_head_q, desc.head_dim),
+                                                       (desc.q_stride or desc.n_head_q * desc.head_dim,
+                                                        desc.head_dim, 1), dtype=_paged_type(desc),
+                                                       device=qkv.device))
+    else:
+        _rows_of(q, "q", desc, _paged_type(desc), desc.q_stride)
+    stride = qkv.stride(0) if qkv.shape[0] > 1 else 0
+    check(lib().p100_paged_append(C.byref(desc), _ptr(qkv), qkv_type, stride, _ptr(q_norm), _ptr(k_norm), eps,
+                                  _ptr(rope_cs), max_pos, int(bool(rope_half)), _ptr(block_table), _ptr(q_start),
+                                  _ptr(kv_len), _ptr(q), _ptr(k_pages), _ptr(v_pages), _stream(stream)))
+    return q
+
+
+def fa_paged_workspace(desc, stream=None):
+    """A workspace for fa_paged calls of desc's heads on the current device (lengths may change between calls);
+    calls that may run at the same time need one each."""
+    torch = _torch()
+    n = lib().p100_fa_paged_workspace_size(C.byref(desc))
+    if n == 0:
+        raise P100Error(ERR_INVALID, last_error())
+    ws = _alloc(stream, lambda: torch.empty(n, dtype=torch.uint8, device="cuda"))
+    check(lib().p100_fa_paged_workspace_init(_ptr(ws), n, _stream(stream)))
+    return ws
+
+
+def fa_paged(desc, q, k_pages, v_pages, block_table, q_start, kv_len, o=None, lse=None, ws=None, stream=None):
+    """Attention of the new tokens over a paged cache (p100_fa_paged): q [n_tokens, n_head_q, head_dim] of the
+    cache's type -> o of the same shape (float32 with desc.o_fp32), lse fp32 [n_tokens, n_head_q]."""
+    torch = _torch()
+    o_type = torch.float32 if desc.o_fp32 else _paged_type(desc)
+    _rows_of(q, "q", desc, _paged_type(desc), desc.q_stride)
+    _lengths_of(desc, block_table, q_start, kv_len)
+    _pages_of(k_pages, "k_pages", desc)
+    _pages_of(v_pages, "v_pages", desc)
+    if o is None:
+        o = _alloc(stream, lambda: torch.empty_strided((desc.n_tokens, desc.n_head_q, desc.head_dim),
+                                                       (desc.o_stride or desc.n_head_q * desc.head_dim,
+                                                        desc.head_dim, 1), dtype=o_type, device=q.device))
+    else:
+        _rows_of(o, "o", desc, o_type, desc.o_stride)
+    if lse is None:
+        lse = _alloc(stream, lambda: torch.empty(desc.n_tokens, desc.n_head_q, dtype=torch.float32, device=q.device))
+    else:
+        _need(lse, "lse", torch.float32, desc.n_tokens * desc.n_head_q)
+    if ws is None:
+        ws = fa_paged_workspace(desc, stream)
+    else:
+        _need(ws, "ws", torch.uint8)
+    check(lib().p100_fa_paged(C.byref(desc), _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(block_table), _ptr(q_start),
+                              _ptr(kv_len), _ptr(o), _ptr(lse), _ptr(ws), ws.numel(), _stream(stream)))
+    return o, lse
+
+
+def logprobs_workspace(rows, n, top_k=0, dtype=F32, stream=None):
+    """A workspace for logprobs of that many rows, or None where none is needed.  The size for F32 rows serves the
+    16-bit types too."""
+    torch = _torch()
+    size = lib().p100_logprobs_workspace_size(rows, n, dtype, top_k)
+    if size == 0:
+        return None   # none needed, or arguments that p100_logprobs reports with its status
+    ws = _alloc(stream, lambda: torch.empty(size, dtype=torch.uint8, device="cuda"))
+    check(lib().p100_logprobs_workspace_init(_ptr(ws), size, _stream(stream)))
+    return ws
+
+
+def logprobs(logits, tokens=None, top_k=0, ws=None, stream=None):
+    """Log probability, entropy, rank and top alternatives of rows of logits [rows, n] (p100_logprobs); tokens
+    int32 [rows], -1 for none.  Returns LogProbs."""
+    torch = _torch()
+    dtype = _dtype_of(logits, "logits")
+    _need(logits, "logits", dense=False)
+    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise InvalidArgument(ERR_INVALID, "logits must be [rows, n] with contiguous rows")
+    rows, n = logits.shape
+    if not 0 <= top_k <= LOGPROBS_MAX_TOP:
+        raise InvalidArgument(ERR_INVALID, "top_k must be between 0 and 32")
+    if tokens is not None:
+        _need(tokens, "tokens", torch.int32, rows)
+
+    def outputs():
+        f = dict(dtype=torch.float32, device=logits.device)
+        i = dict(dtype=torch.int32, device=logits.device)
+        return LogProbs(torch.empty(rows, **f) if tokens is not None else None, torch.empty(rows, **f),
+                        torch.empty(rows, **i) if tokens is not None else None, torch.empty(rows, top_k, **i),
+                        torch.empty(rows, top_k, **f))
+
+    out = _alloc(stream, outputs)
+    if ws is None:
+        ws = logprobs_workspace(rows, n, top_k, dtype, stream)
+    else:
+        _need(ws, "ws", torch.uint8)
+    stride = logits.stride(0) if rows > 1 else 0
+    check(lib().p100_logprobs(_ptr(logits), dtype, n, rows, stride, _ptr(tokens), top_k, _ptr(out.logprob),
+                              _ptr(out.entropy), _ptr(out.rank), _ptr(out.top_index), _ptr(out.top_logprob), _ptr(ws),
+                              ws.numel() if ws is not None else 0, _stream(stream)))
+    return out
 
 
 # ---------------------------------------------------------------- tensor parallel

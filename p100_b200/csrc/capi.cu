@@ -2,8 +2,10 @@
 // quantised mat-vec and FlashAttention decode paths, plus library plumbing
 // (status text, device checks, the bounded-wait flag).
 //
-// Single CUDA translation unit: every kernel header is included here so the
-// library has one device module and one g_device_error word per device.
+// One of two CUDA translation units (serve.cu holds the paged cache and the
+// scoring of logits): the headers of the decode path are all included here, so
+// its kernels share one g_device_error word per device; p100_device_error
+// reports serve.cu's word too.
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -1071,6 +1073,9 @@ p100_status p100_device_error(int clear) {
         if (p100_status st = cuda_status(cudaMemcpyToSymbol(g_device_error, &zero, sizeof zero), "clear device flag"))
             return st;
     }
+    int served = 0;
+    if (p100_status st = serve_device_error(clear, &served)) return st;
+    if (!value || served == kDevErrTimeout) value = served ? served : value;
     if (value == kDevErrInput)
         return set_error(P100_ERR_INVALID, "a kernel read a device-resident token or position out of range");
     return value ? set_error(P100_ERR_TIMEOUT, "a kernel gave up a bounded wait") : P100_OK;

@@ -20,12 +20,14 @@ p100_status cuda_status(cudaError_t err, const char* what);
 void clear_error();
 // P100_OK when the current device is an sm_100 part (cached per device).
 p100_status require_sm100(int* device_out, int* sm_count_out);
+// Implemented in serve.cu: its kernels' g_device_error on the current device.
+p100_status serve_device_error(int clear, int* value);
 
 // ------------------------------------------------------------ device state
 // Set to kDevErrTimeout by any bounded wait that runs out; read by
-// p100_device_error().  The library is one CUDA translation unit (capi.cu),
-// so this definition exists once per device module.
-__device__ int g_device_error = 0;
+// p100_device_error().  Each of the library's CUDA translation units (capi.cu,
+// serve.cu) has a word of its own.
+static __device__ int g_device_error = 0;
 constexpr int kDevErrTimeout = 1;
 constexpr int kDevErrInput = 2;    // a device-resident index (token, position) out of range
 // One second: far above any legitimate wait in these kernels (microseconds).

@@ -1,0 +1,370 @@
+// fa_paged.cuh — attention of new tokens over a paged cache on mma.sync: the
+// kernel for single tokens (16 query rows of a kv head or fewer) and for page
+// sizes that tensor copies cannot take.
+//
+//   s_ij = scale q_i k_j  (then cap tanh(s / cap)),  j < limit_i
+//   o_i = sum_j e^(s_ij - m_i) v_j / sum_j e^(s_ij - m_i),  lse_i = m_i + ln sum
+//
+// A CTA walks its share of units (paged.cuh): 16 rows x 64 keys.  The four
+// warps of a CTA split every key tile, 16 keys each, with a running maximum,
+// sum and 16 x D accumulator of their own in registers, joined once per item:
+// no exchange per tile.  K and V rows are gathered by 16-byte asynchronous
+// copies (any page size; a row's page is looked up two tiles ahead), swizzled
+// so that ldmatrix reads without bank conflicts; rows behind kv_len are filled
+// with zeros, so what a page holds there never reaches a product.  Statistics
+// and accumulators are FP32; the probabilities are rounded once to the cache's
+// 16-bit type, as the tensor cores take them.
+//
+// HBM bytes bound it: K and V are read once per row tile.  A row tile cut by
+// the shares leaves its partials {m, l, unnormalised o} in the workspace and
+// its last CTA (an atomic ticket, no waiting) joins them in share order.
+#pragma once
+#include "paged.cuh"
+
+namespace p100b {
+namespace fap {
+
+using paged::Desc;
+using paged::Item;
+using paged::Lengths;
+
+constexpr int kThreads = 128;
+constexpr int kRows = 16, kKeys = 64;
+constexpr int kStages = 3;
+constexpr int kOffs = 5;   // tiles whose row offsets are held
+
+struct Params {
+    Desc d;
+    const void *q, *k, *v;
+    void* o;
+    int o_f32;
+    float* lse;        // [n_tokens][n_head_q] or null
+    float* ws_o;       // [CTAs][2][kRows][D]
+    float* ws_ml;      // [CTAs][2][kRows][2], m in units of log2
+    unsigned* tickets; // [CTAs]
+    float scale, softcap;
+};
+
+template <int D>
+constexpr size_t smem_bytes() {
+    return sizeof(Lengths) + size_t(kStages) * 2 * kKeys * D * 2 + kOffs * kKeys * sizeof(long long) + 128;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// cap tanh(x / cap) with tanh y = 1 - 2 / (e^(2y) + 1): two approximate
+// operations, absolute error a few 1e-7 of cap.
+__device__ __forceinline__ float cap_score(float x, float two_over_cap_log2e, float cap) {
+    return fmaf(-2.f * cap, paged::rcp_approx(paged::exp2_approx(x * two_over_cap_log2e) + 1.f), cap);
+}
+
+// Row r (token r / group of the sequence, query head r % group of the kv
+// head) of an item's query or output tensor, in elements.
+__device__ __forceinline__ long long row_offset(const Desc& d, int q0, int head, int r, long long stride, int D) {
+    const int tok = r / d.group, g = r - tok * d.group;
+    return (long long)(q0 + tok) * stride + (long long)(head * d.group + g) * D;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_out2(void* o, int o_f32, long long at, float a, float b) {
+    if (o_f32)
+        *reinterpret_cast<float2*>(static_cast<float*>(o) + at) = make_float2(a, b);
+    else
+        *reinterpret_cast<uint32_t*>(static_cast<T*>(o) + at) = paged::pack2<T>(a, b);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 2) fa_paged_kernel(const Params p) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int kRowBytes = D * 2;
+    constexpr int kTileBytes = kKeys * kRowBytes;
+    constexpr int kChunks = D / 8;            // 16-byte chunks of a row
+    constexpr float kLog2e = 1.4426950408889634f;
+    Lengths& len = *reinterpret_cast<Lengths*>(smem);
+    long long* s_off = reinterpret_cast<long long*>(smem + ((sizeof(Lengths) + 15) & ~size_t(15)));   // [kOffs][kKeys]
+    uint8_t* s_kv = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_off + kOffs * kKeys) + 127) & ~uintptr_t(127));
+    __shared__ int s_last;
+    const Desc& d = p.d;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    paged::read_lengths<kRows, kKeys, kThreads>(d, len);
+    if (!len.ok) return;
+    // at least one unit a share: every CTA between a cut tile's first and last
+    // then holds a part of it
+    const int parts = int(min((long long)gridDim.x, len.total));
+    if (int(blockIdx.x) >= parts) return;
+    paged::Share<kRows, kKeys> share;
+    share.begin(d, len, blockIdx.x, parts);
+    Item it;
+    const float to_log2 = p.scale * kLog2e;
+    const float cap_in = p.softcap != 0.f ? 2.f * to_log2 / p.softcap : 0.f;
+
+    while (share.next(d, len, it)) {
+        const int q0 = len.q0[it.seq], n = len.q0[it.seq + 1] - q0, kv = len.kv[it.seq];
+        const int rows = min(kRows, n * d.group - it.tile * kRows);
+        const int row0 = it.tile * kRows;
+        const int end = paged::key_end<kRows, kKeys>(d, n, kv, it.tile);   // keys any row sees
+        const int* table = d.block_table + (long long)it.seq * d.max_pages;
+        const long long head_off = it.head * d.head_stride;
+
+        // The element offset of key row `key`, or -1 where it is not read.
+        auto find = [&](int key) -> long long {
+            if (key >= end) return -1;
+            const int at = key / d.page_size;
+            const int page = table[at];
+            if (page < 0 || page >= d.n_pages) {
+                paged::flag_input();
+                return -1;
+            }
+            return page * d.page_stride + head_off + (long long)(key - at * d.page_size) * d.token_stride;
+        };
+        // Copies of tile t (counted from the item's first) into its stage.
+        auto issue = [&](int t) {
+            if (t < it.count) {
+                const long long* off = s_off + (t % kOffs) * kKeys;
+                uint8_t* ks = s_kv + size_t(t % kStages) * 2 * kTileBytes;
+                const int c = tid % kChunks;
+#pragma unroll
+                for (int r = tid / kChunks; r < kKeys; r += kThreads / kChunks) {
+                    const long long o = off[r];
+                    const uint32_t dst = smem_addr(ks) + r * kRowBytes + ((c ^ (r & 7)) << 4);
+                    const long long from = (o < 0 ? 0 : o) + c * 8;
+                    cp_async16(dst, static_cast<const T*>(p.k) + from, o >= 0);
+                    cp_async16(dst + kTileBytes, static_cast<const T*>(p.v) + from, o >= 0);
+                }
+            }
+            cp_commit();
+        };
+
+        // Offsets of the first kOffs - 1 tiles, the first copies.
+        for (int i = tid; i < (kOffs - 1) * kKeys; i += kThreads)
+            s_off[i] = i / kKeys < it.count ? find((it.key_tile + i / kKeys) * kKeys + i % kKeys) : -1;
+        __syncthreads();
+        for (int t = 0; t < kStages - 1; ++t) issue(t);
+
+        // Query fragments: rows g and g + 8 of the tile (zero past the rows).
+        const int g = lane >> 2, cq = (lane & 3) * 2;
+        uint32_t qf[D / 16][4];
+        {
+            const T* qa = nullptr;
+            const T* qb = nullptr;
+            if (g < rows) qa = static_cast<const T*>(p.q) + row_offset(d, q0, it.head, row0 + g, d.q_stride, D);
+            if (g + 8 < rows) qb = static_cast<const T*>(p.q) + row_offset(d, q0, it.head, row0 + g + 8, d.q_stride, D);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                qf[k][0] = qa ? *reinterpret_cast<const uint32_t*>(qa + k * 16 + cq) : 0u;
+                qf[k][1] = qb ? *reinterpret_cast<const uint32_t*>(qb + k * 16 + cq) : 0u;
+                qf[k][2] = qa ? *reinterpret_cast<const uint32_t*>(qa + k * 16 + cq + 8) : 0u;
+                qf[k][3] = qb ? *reinterpret_cast<const uint32_t*>(qb + k * 16 + cq + 8) : 0u;
+            }
+        }
+        // Keys [0, limit) of rows g and g + 8.
+        int limit[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = g + 8 * h;
+            limit[h] = r >= rows ? 0 : d.causal ? min(kv, kv - n + (row0 + r) / d.group + 1) : kv;
+        }
+        float acc[D / 8][4];
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+        for (int t = 0; t < it.count; ++t) {
+            cp_wait<kStages - 2>();
+            __syncthreads();   // tile t has landed; everyone is done with tile t - 1
+            long long next_off = -1;
+            const int ahead = t + kOffs - 1;
+            if (tid < kKeys && ahead < it.count) next_off = find((it.key_tile + ahead) * kKeys + tid);
+            issue(t + kStages - 1);
+            const uint32_t ks = smem_addr(s_kv) + (t % kStages) * 2 * kTileBytes;
+            const uint32_t vs = ks + kTileBytes;
+            float s[2][4] = {};
+            {
+                // matrices 0/1: keys 0-7, low and high half of the 16 dims; 2/3: keys 8-15
+                const int key = warp * 16 + (lane & 7) + ((lane >> 4) << 3);
+                const uint32_t row = ks + key * kRowBytes;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    uint32_t b[4];
+                    ldsm4(row + (((2 * k + ((lane >> 3) & 1)) ^ (key & 7)) << 4), b);
+                    mma16<T>(s[0], qf[k], b[0], b[1]);
+                    mma16<T>(s[1], qf[k], b[2], b[3]);
+                }
+            }
+            const int key0 = (it.key_tile + t) * kKeys + warp * 16 + cq;   // this lane's first column
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x = p.softcap != 0.f ? cap_score(s[j][e], cap_in, p.softcap) * kLog2e : s[j][e] * to_log2;
+                    s[j][e] = key0 + j * 8 + (e & 1) < limit[e >> 1] ? x : -INFINITY;
+                }
+            uint32_t pf[4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float mx = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                const float mn = fmaxf(m[h], mx);
+                const float base = mn == -INFINITY ? 0.f : mn;
+                const float a = paged::exp2_approx(m[h] - base);
+                m[h] = mn;
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        s[j][2 * h + e] = paged::exp2_approx(s[j][2 * h + e] - base);
+                        sum += s[j][2 * h + e];
+                    }
+                l[h] = l[h] * a + sum;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    acc[i][2 * h] *= a;
+                    acc[i][2 * h + 1] *= a;
+                }
+                pf[h] = paged::pack2<T>(s[0][2 * h], s[0][2 * h + 1]);
+                pf[2 + h] = paged::pack2<T>(s[1][2 * h], s[1][2 * h + 1]);
+            }
+            {
+                // matrices 0/1: dims 0-7 of keys 0-7 and 8-15; 2/3: dims 8-15
+                const int key = warp * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
+                const uint32_t row = vs + key * kRowBytes;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    uint32_t b[4];
+                    ldsm4_t(row + (((2 * i + (lane >> 4)) ^ (key & 7)) << 4), b);
+                    mma16<T>(acc[2 * i], pf, b[0], b[1]);
+                    mma16<T>(acc[2 * i + 1], pf, b[2], b[3]);
+                }
+            }
+            if (tid < kKeys) s_off[(ahead % kOffs) * kKeys + tid] = next_off;
+        }
+
+        // Join the warps: statistics, then the accumulators added in warp order.
+        cp_wait<0>();
+        __syncthreads();
+        float* s_m = reinterpret_cast<float*>(s_kv);          // [4][16]
+        float* s_l = s_m + 4 * kRows;                         // [4][16]
+        float* s_o = s_l + 4 * kRows;                         // [4][16][D + 4]
+        constexpr int kLd = D + 4;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            if ((lane & 3) == 0) {
+                s_m[warp * kRows + g + 8 * h] = m[h];
+                s_l[warp * kRows + g + 8 * h] = l[h];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                *reinterpret_cast<float2*>(s_o + (warp * kRows + g + 8 * h) * kLd + i * 8 + cq) =
+                    make_float2(acc[i][2 * h], acc[i][2 * h + 1]);
+        __syncthreads();
+        const bool whole = it.count == it.units;
+        const int slot = blockIdx.x * 2 + (it.key_tile == 0);   // 0: a tile begun by another CTA, 1: begun here
+        for (int e = tid; e < rows * (D / 2); e += kThreads) {
+            const int r = e / (D / 2), c = (e - r * (D / 2)) * 2;
+            float mx = s_m[r];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) mx = fmaxf(mx, s_m[w * kRows + r]);
+            const float base = mx == -INFINITY ? 0.f : mx;
+            float a = 0.f, b = 0.f, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = paged::exp2_approx(s_m[w * kRows + r] - base);
+                const float2 o = *reinterpret_cast<const float2*>(s_o + (w * kRows + r) * kLd + c);
+                a = fmaf(f, o.x, a);
+                b = fmaf(f, o.y, b);
+                sum = fmaf(f, s_l[w * kRows + r], sum);
+            }
+            if (whole) {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                const int tok = (row0 + r) / d.group;
+                store_out2<T>(p.o, p.o_f32, row_offset(d, q0, it.head, row0 + r, d.o_stride, D) + c, a * inv, b * inv);
+                if (p.lse && c == 0)
+                    p.lse[(long long)(q0 + tok) * d.n_head_q + it.head * d.group + (row0 + r - tok * d.group)] =
+                        sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
+            } else {
+                *reinterpret_cast<float2*>(p.ws_o + ((long long)slot * kRows + r) * D + c) = make_float2(a, b);
+                if (c == 0)
+                    *reinterpret_cast<float2*>(p.ws_ml + ((long long)slot * kRows + r) * 2) = make_float2(mx, sum);
+            }
+        }
+        if (!whole) {
+            const int c0 = paged::share_of(it.tile_first, len.total, parts);
+            const int c1 = paged::share_of(it.tile_first + it.units - 1, len.total, parts);
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) s_last = atomicAdd(p.tickets + c0, 1u) == unsigned(c1 - c0);
+            __syncthreads();
+            if (s_last) {
+                __threadfence();
+                if (tid == 0) p.tickets[c0] = 0;   // ready for the next call
+                for (int e = tid; e < rows * (D / 2); e += kThreads) {
+                    const int r = e / (D / 2), c = (e - r * (D / 2)) * 2;
+                    float mx = -INFINITY;
+                    for (int q = c0; q <= c1; ++q)
+                        mx = fmaxf(mx, __ldcg(p.ws_ml + ((long long)(2 * q + (q == c0)) * kRows + r) * 2));
+                    const float base = mx == -INFINITY ? 0.f : mx;
+                    float a = 0.f, b = 0.f, sum = 0.f;
+#pragma unroll 4
+                    for (int q = c0; q <= c1; ++q) {
+                        const long long at = (long long)(2 * q + (q == c0)) * kRows + r;
+                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + at * 2));
+                        const float2 o = __ldcg(reinterpret_cast<const float2*>(p.ws_o + at * D + c));
+                        const float f = paged::exp2_approx(ml.x - base);
+                        a = fmaf(f, o.x, a);
+                        b = fmaf(f, o.y, b);
+                        sum = fmaf(f, ml.y, sum);
+                    }
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                    const int tok = (row0 + r) / d.group;
+                    store_out2<T>(p.o, p.o_f32, row_offset(d, q0, it.head, row0 + r, d.o_stride, D) + c, a * inv, b * inv);
+                    if (p.lse && c == 0)
+                        p.lse[(long long)(q0 + tok) * d.n_head_q + it.head * d.group + (row0 + r - tok * d.group)] =
+                            sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
+                }
+            }
+        }
+        __syncthreads();   // shared memory is free for the next item
+    }
+}
+
+}  // namespace fap
+}  // namespace p100b

@@ -1,0 +1,244 @@
+// paged.cuh — what the paged-cache kernels share: the 16-bit types, the
+// descriptor as the kernels see it, the check of the device-resident lengths
+// and the division of an attention call's work into equal shares.
+//
+// A paged cache holds pages of page_size token rows per kv head; sequence s
+// finds token j in row j % page_size of page block_table[s][j / page_size].
+// The n = q_start[s+1] - q_start[s] new tokens of a sequence are its last
+// ones: new token i sits at position kv_len[s] - n + i.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace p100b {
+namespace paged {
+
+constexpr int kMaxSeq = 1024;   // sequences of one call: their lengths live in shared memory
+
+struct Desc {
+    int n_seq, n_tokens, max_q;
+    int n_head_q, n_head_kv, group;
+    int page_size, n_pages, max_pages;
+    int causal;
+    long long page_stride, head_stride, token_stride;   // of the pages, in elements
+    long long q_stride, o_stride;                       // between tokens, in elements
+    const int* block_table;   // [n_seq][max_pages]
+    const int* q_start;       // [n_seq + 1]
+    const int* kv_len;        // [n_seq]
+};
+
+// ------------------------------------------------------------ 16-bit types
+template <typename T>
+__device__ __forceinline__ float to_float(T v);
+template <>
+__device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Two floats rounded to nearest even, lo in the low half.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void flag_input() { atomicExch(&g_device_error, kDevErrInput); }
+
+// ------------------------------------------------------------ shares
+// An attention call is a list of units, one unit = one tile of KEYS keys of
+// one tile of ROWS query rows of one (sequence, kv head).  The rows of a kv
+// head are the (token, query head of the group) pairs in token order, so a
+// tile serves every query head that reads its keys.  Units are ordered by
+// sequence, kv head, row tile, key tile; CTA c of P takes the units
+// [c U / P, (c + 1) U / P): every CTA gets the same amount whatever the
+// lengths, and a row tile is cut only where a share ends.  A row tile that
+// sees no key still counts one unit, which writes its zeros.
+struct Lengths {
+    long long total;                 // units of the call
+    int ok;                          // the lengths are usable
+    int q0[kMaxSeq + 1];
+    int kv[kMaxSeq];
+    unsigned per_head[kMaxSeq];      // units of one kv head
+    unsigned long long first[kMaxSeq];   // units before the sequence
+};
+
+template <int ROWS, int KEYS>
+__device__ __forceinline__ int key_end(const Desc& d, int n, int kv, int tile) {
+    const int last = min((tile + 1) * ROWS, n * d.group) - 1;
+    const int end = d.causal ? kv - n + last / d.group + 1 : kv;
+    return max(0, min(end, kv));
+}
+template <int ROWS, int KEYS>
+__device__ __forceinline__ int tile_units(const Desc& d, int n, int kv, int tile) {
+    return max(1, (key_end<ROWS, KEYS>(d, n, kv, tile) + KEYS - 1) / KEYS);
+}
+
+// Reads and checks the lengths and counts the units; every thread of the CTA
+// calls it.  Lengths that are out of order or out of range raise the device
+// flag and make the call do nothing.
+template <int ROWS, int KEYS, int THREADS>
+__device__ void read_lengths(const Desc& d, Lengths& s) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) s.ok = 1;
+    for (int i = tid; i <= d.n_seq; i += THREADS) s.q0[i] = d.q_start[i];
+    for (int i = tid; i < d.n_seq; i += THREADS) s.kv[i] = d.kv_len[i];
+    __syncthreads();
+    for (int i = tid; i < d.n_seq; i += THREADS) {
+        const int n = s.q0[i + 1] - s.q0[i];
+        if (s.q0[i] < 0 || n < 0 || n > d.max_q || s.q0[i + 1] > d.n_tokens || s.kv[i] < 0 ||
+            (long long)s.kv[i] > (long long)d.max_pages * d.page_size)
+            s.ok = 0;
+    }
+    __syncthreads();
+    if (!s.ok) {
+        if (tid == 0) flag_input();
+        return;
+    }
+    // Sequences of few row tiles a thread each, longer ones a warp each.
+    for (int i = tid; i < d.n_seq; i += THREADS) {
+        const int n = s.q0[i + 1] - s.q0[i];
+        const int tiles = int(((long long)n * d.group + ROWS - 1) / ROWS);
+        unsigned sum = 0;
+        if (tiles <= 4)
+            for (int t = 0; t < tiles; ++t) sum += tile_units<ROWS, KEYS>(d, n, s.kv[i], t);
+        s.per_head[i] = sum;
+    }
+    __syncthreads();
+    for (int i = warp; i < d.n_seq; i += THREADS / 32) {
+        const int n = s.q0[i + 1] - s.q0[i];
+        const int tiles = int(((long long)n * d.group + ROWS - 1) / ROWS);
+        if (tiles <= 4) continue;
+        unsigned sum = 0;
+        for (int t = lane; t < tiles; t += 32) sum += tile_units<ROWS, KEYS>(d, n, s.kv[i], t);
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        if (lane == 0) s.per_head[i] = sum;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        unsigned long long at = 0;
+        for (int i = 0; i < d.n_seq; i += 32) {
+            unsigned long long v = i + lane < d.n_seq ? (unsigned long long)s.per_head[i + lane] * d.n_head_kv : 0;
+            const unsigned long long own = v;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const unsigned long long u = __shfl_up_sync(0xffffffffu, v, off);
+                if (lane >= off) v += u;
+            }
+            if (i + lane < d.n_seq) s.first[i + lane] = at + v - own;
+            at += __shfl_sync(0xffffffffu, v, 31);
+        }
+        if (lane == 0) s.total = (long long)at;
+    }
+    __syncthreads();
+}
+
+struct Item {
+    int seq, head, tile;     // row tile of the sequence's head
+    int key_tile, count;     // its key tiles [key_tile, key_tile + count) are this CTA's
+    int units;               // key tiles of the whole row tile
+    long long tile_first;    // its first unit
+};
+
+// One CTA's share as a list of items; the calls are warp-uniform.
+template <int ROWS, int KEYS>
+struct Share {
+    long long at, end;
+    int seq, head, tile, key_tile, tiles, n, kv;
+    bool fresh;
+
+    __device__ __forceinline__ void enter_seq(const Desc& d, const Lengths& s, int i) {
+        seq = i;
+        n = s.q0[i + 1] - s.q0[i];
+        kv = s.kv[i];
+        tiles = int(((long long)n * d.group + ROWS - 1) / ROWS);
+    }
+
+    // cta's share of `parts` equal ones.
+    __device__ __forceinline__ void begin(const Desc& d, const Lengths& s, int cta, int parts) {
+        at = s.total * cta / parts;
+        end = s.total * (cta + 1) / parts;
+        if (at >= end) return;
+        int lo = 0, hi = d.n_seq - 1;   // the last sequence whose first unit is at or before `at`, with units
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if ((long long)s.first[mid] <= at) lo = mid; else hi = mid - 1;
+        }
+        enter_seq(d, s, lo);
+        const unsigned long long in_seq = (unsigned long long)at - s.first[lo];
+        head = int(in_seq / s.per_head[lo]);
+        unsigned rest = unsigned(in_seq - (unsigned long long)head * s.per_head[lo]);
+        const int lane = threadIdx.x & 31;
+        for (int t0 = 0;; t0 += 32) {   // the row tile that holds unit `rest` of the head
+            const unsigned own = t0 + lane < tiles ? tile_units<ROWS, KEYS>(d, n, kv, t0 + lane) : 0;
+            unsigned v = own;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const unsigned u = __shfl_up_sync(0xffffffffu, v, off);
+                if (lane >= off) v += u;
+            }
+            const unsigned ahead = __ballot_sync(0xffffffffu, v <= rest);
+            if (ahead != 0xffffffffu) {
+                const int l = __popc(ahead);
+                tile = t0 + l;
+                key_tile = int(rest - __shfl_sync(0xffffffffu, v - own, l));
+                break;
+            }
+            rest -= __shfl_sync(0xffffffffu, v, 31);
+        }
+    }
+
+    __device__ __forceinline__ bool next(const Desc& d, const Lengths& s, Item& it) {
+        if (at >= end) return false;
+        while (tile == tiles) {
+            tile = 0;
+            if (tiles == 0 || ++head == d.n_head_kv) {
+                head = 0;
+                enter_seq(d, s, seq + 1);
+            }
+        }
+        it.seq = seq;
+        it.head = head;
+        it.tile = tile;
+        it.units = tile_units<ROWS, KEYS>(d, n, kv, tile);
+        it.key_tile = key_tile;
+        it.count = int(min((long long)(it.units - key_tile), end - at));
+        it.tile_first = at - key_tile;
+        at += it.count;
+        key_tile = 0;
+        ++tile;
+        return true;
+    }
+};
+
+// The CTA whose share of `parts` holds unit u: the largest c with
+// total * c / parts <= u.
+__device__ __forceinline__ int share_of(long long u, long long total, int parts) {
+    return int(((u + 1) * parts - 1) / total);
+}
+
+}  // namespace paged
+}  // namespace p100b

@@ -1,0 +1,349 @@
+// serve.cu — the extern "C" entry points of include/p100/b200.h for prompts
+// and batches: the append of new tokens to a paged cache, attention over it,
+// and the scoring of logits.  A translation unit of its own, with its own
+// g_device_error word, which p100_device_error reads through
+// serve_device_error.
+#include <climits>
+#include <cmath>
+#include <cstring>
+#include <algorithm>
+
+#include <cudaTypedefs.h>
+
+#include "common.cuh"
+#include "fa_paged.cuh"
+#include "logprobs.cuh"
+#include "paged_append.cuh"
+
+namespace p100b {
+
+p100_status serve_device_error(int clear, int* value) {
+    if (p100_status st = cuda_status(cudaMemcpyFromSymbol(value, g_device_error, sizeof *value), "read device flag"))
+        return st;
+    if (clear && *value) {
+        const int zero = 0;
+        return cuda_status(cudaMemcpyToSymbol(g_device_error, &zero, sizeof zero), "clear device flag");
+    }
+    return P100_OK;
+}
+
+namespace {
+
+size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// Dynamic shared memory beyond 48 KB, once per kernel and device.
+template <typename K>
+p100_status allow_smem(K kern, size_t bytes, int (&configured)[64], const char* what) {
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return cuda_status(e, what);
+    if (configured[dev]) return P100_OK;
+    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)))
+        return cuda_status(e, what);
+    configured[dev] = 1;
+    return P100_OK;
+}
+
+// ------------------------------------------------------------ paged cache
+// The descriptor with its defaults filled in, or the reason it is refused.
+const char* paged_reason(const p100_paged_desc& in, paged::Desc& d) {
+    if (in.n_seq < 0 || in.n_tokens < 0 || in.max_q < 0 || in.n_pages < 0 || in.max_pages < 0)
+        return "counts must not be negative";
+    if (in.n_seq > P100_PAGED_MAX_SEQ) return "n_seq exceeds P100_PAGED_MAX_SEQ";
+    if (in.n_head_q <= 0 || in.n_head_kv <= 0 || in.page_size <= 0) return "all dimensions must be positive";
+    if (in.n_head_q % in.n_head_kv) return "n_head_q must be divisible by n_head_kv";
+    if (in.head_dim != 64 && in.head_dim != 128) return "head_dim must be 64 or 128";
+    if (in.dtype != P100_F16 && in.dtype != P100_BF16) return "dtype must be P100_F16 or P100_BF16";
+    if (!std::isfinite(in.scale)) return "scale must be finite";
+    if (!std::isfinite(in.softcap) || in.softcap < 0.0f) return "softcap must be finite and non-negative";
+    if ((long long)in.n_tokens * in.n_head_q > INT_MAX) return "n_tokens * n_head_q exceeds 2^31 - 1";
+    if ((long long)in.max_pages * in.page_size > INT_MAX) return "max_pages * page_size exceeds 2^31 - 1";
+    const long long D = in.head_dim;
+    d.n_seq = in.n_seq;
+    d.n_tokens = in.n_tokens;
+    d.max_q = in.max_q ? std::min(in.max_q, in.n_tokens) : in.n_tokens;
+    d.n_head_q = in.n_head_q;
+    d.n_head_kv = in.n_head_kv;
+    d.group = in.n_head_q / in.n_head_kv;
+    d.page_size = in.page_size;
+    d.n_pages = in.n_pages;
+    d.max_pages = in.max_pages;
+    d.causal = in.causal != 0;
+    d.token_stride = in.token_stride ? in.token_stride : D;
+    d.head_stride = in.head_stride ? in.head_stride : in.page_size * D;
+    d.page_stride = in.page_stride ? in.page_stride : in.n_head_kv * in.page_size * D;
+    d.q_stride = in.q_stride ? in.q_stride : in.n_head_q * D;
+    d.o_stride = in.o_stride ? in.o_stride : in.n_head_q * D;
+    for (long long s : {d.token_stride, d.head_stride, d.page_stride}) {
+        if (s < D) return "page strides must be at least head_dim";
+        if (s % 8) return "strides must be multiples of 8 elements";
+    }
+    for (long long s : {d.q_stride, d.o_stride}) {
+        if (s < in.n_head_q * D) return "q and o strides must be at least n_head_q * head_dim";
+        if (s % 8) return "strides must be multiples of 8 elements";
+    }
+    return nullptr;
+}
+
+// CTAs of the mma.sync kernel: two on every SM.
+constexpr int kMmaCtas = 2;
+
+struct FaPagedWs {
+    size_t o, ml, tickets, total;
+};
+FaPagedWs fa_paged_ws(const p100_paged_desc& in, int sms) {
+    const size_t ctas = size_t(sms) * kMmaCtas;
+    FaPagedWs w;
+    w.tickets = round256(ctas * sizeof(unsigned));   // first, so that init clears little
+    w.o = round256(ctas * 2 * fap::kRows * in.head_dim * sizeof(float));
+    w.ml = round256(ctas * 2 * fap::kRows * 2 * sizeof(float));
+    w.total = w.tickets + w.o + w.ml;
+    return w;
+}
+size_t fa_paged_ticket_bytes(int sms) { return round256(size_t(sms) * kMmaCtas * sizeof(unsigned)); }
+
+template <typename T, int D>
+p100_status launch_fa_paged_mma(const fap::Params& prm, int sms, cudaStream_t stream) {
+    static thread_local int configured[64] = {};
+    auto kern = fap::fa_paged_kernel<T, D>;
+    if (p100_status st = allow_smem(kern, fap::smem_bytes<D>(), configured, "cudaFuncSetAttribute(fa_paged)")) return st;
+    kern<<<sms * kMmaCtas, fap::kThreads, fap::smem_bytes<D>(), stream>>>(prm);
+    return cuda_status(cudaGetLastError(), "fa_paged_kernel launch");
+}
+
+template <typename S, typename T>
+p100_status launch_append(const paged::AppendParams& prm, int head_dim, unsigned blocks, cudaStream_t stream) {
+    if (head_dim == 64)
+        paged::paged_append_kernel<S, T, 64><<<blocks, paged::kAppendThreads, 0, stream>>>(prm);
+    else
+        paged::paged_append_kernel<S, T, 128><<<blocks, paged::kAppendThreads, 0, stream>>>(prm);
+    return cuda_status(cudaGetLastError(), "paged_append_kernel launch");
+}
+template <typename S>
+p100_status launch_append_to(const paged::AppendParams& prm, int dtype, int head_dim, unsigned blocks, cudaStream_t s) {
+    return dtype == P100_F16 ? launch_append<S, __half>(prm, head_dim, blocks, s)
+                             : launch_append<S, __nv_bfloat16>(prm, head_dim, blocks, s);
+}
+
+// ------------------------------------------------------------ logits
+size_t dtype_bytes(int t) { return t == P100_F32 ? 4 : 2; }
+const char* logprobs_reason(int rows, int n, int dtype, int top_k) {
+    if (rows < 0 || n <= 0) return "rows must not be negative and n must be positive";
+    if (dtype != P100_F32 && dtype != P100_F16 && dtype != P100_BF16) return "unknown logit type";
+    if (top_k < 0 || top_k > lp::kMaxTop) return "top_k must be between 0 and 32";
+    return nullptr;
+}
+// Parts of a row: enough CTAs for three on every SM, each with a vector or
+// more for every thread.
+int logprobs_parts(int rows, int n, int dtype, int sms) {
+    const long long vec = 16 / (long long)dtype_bytes(dtype);
+    const long long most = std::min<long long>(lp::kMaxParts, std::max(1LL, n / (vec * lp::kThreads)));
+    return int(std::max(1LL, std::min(most, 3LL * sms / std::max(1, rows))));
+}
+struct LogprobsWs {
+    size_t tickets, sums, keys, total;
+};
+// Rows are split while there are at most 3 sms / 2 of them; the tickets' place
+// does not depend on the call, so one workspace serves calls of other shapes.
+LogprobsWs logprobs_ws(int rows, int parts, int top_k, int sms) {
+    LogprobsWs w = {};
+    if (parts > 1 && rows > 0) {
+        const size_t cells = size_t(rows) * parts;
+        w.tickets = round256(size_t(sms) * 2 * sizeof(unsigned));
+        w.sums = round256(cells * sizeof(float4));
+        w.keys = round256(cells * top_k * sizeof(unsigned long long));
+        w.total = w.tickets + w.sums + w.keys;
+    }
+    return w;
+}
+
+}  // namespace
+}  // namespace p100b
+
+using namespace p100b;
+
+extern "C" {
+
+p100_status p100_paged_append(const p100_paged_desc* desc, const void* qkv, int qkv_type, long long qkv_stride,
+                              const float* q_norm, const float* k_norm, float eps, const float* rope_cs, int max_pos,
+                              int rope_half, const int* block_table, const int* q_start, const int* kv_len, void* q,
+                              void* k_pages, void* v_pages, p100_stream_t stream) {
+    clear_error();
+    if (!desc) return set_error(P100_ERR_INVALID, "null descriptor");
+    paged::AppendParams prm = {};
+    if (const char* why = paged_reason(*desc, prm.d)) return set_error(P100_ERR_INVALID, "%s", why);
+    if (qkv_type != P100_F32 && qkv_type != P100_F16 && qkv_type != P100_BF16)
+        return set_error(P100_ERR_INVALID, "unknown qkv type %d", qkv_type);
+    const long long heads = (long long)desc->n_head_q + 2LL * desc->n_head_kv, width = heads * desc->head_dim;
+    if (qkv_stride == 0) qkv_stride = width;
+    if (qkv_stride < width) return set_error(P100_ERR_INVALID, "qkv_stride must be at least a fused row");
+    if (qkv_stride * (qkv_type == P100_F32 ? 4 : 2) % 16)
+        return set_error(P100_ERR_INVALID, "qkv rows must be 16-byte aligned");
+    if ((q_norm || k_norm) && !(std::isfinite(eps) && eps >= 0.0f))
+        return set_error(P100_ERR_INVALID, "eps must be finite and non-negative");
+    if (rope_cs && max_pos <= 0) return set_error(P100_ERR_INVALID, "max_pos must be positive");
+    if (p100_status st = require_sm100(nullptr, nullptr)) return st;
+    if (desc->n_tokens == 0 || desc->n_seq == 0) return P100_OK;
+    if (!qkv || !block_table || !q_start || !kv_len || !q || !k_pages || !v_pages)
+        return set_error(P100_ERR_INVALID, "null buffer");
+    if (!aligned(qkv, 16) || !aligned(q, 16) || !aligned(k_pages, 16) || !aligned(v_pages, 16))
+        return set_error(P100_ERR_INVALID, "qkv, q and the pages must be 16-byte aligned");
+    if (!aligned(rope_cs, 8)) return set_error(P100_ERR_INVALID, "rope_cs must be 8-byte aligned");
+    prm.d.block_table = block_table;
+    prm.d.q_start = q_start;
+    prm.d.kv_len = kv_len;
+    prm.qkv = qkv;
+    prm.qkv_stride = qkv_stride;
+    prm.q_norm = q_norm;
+    prm.k_norm = k_norm;
+    prm.eps = eps;
+    prm.rope = reinterpret_cast<const float2*>(rope_cs);
+    prm.max_pos = max_pos;
+    prm.half = rope_half != 0;
+    prm.q = q;
+    prm.k = k_pages;
+    prm.v = v_pages;
+    const long long groups = (heads + paged::kAppendHeads - 1) / paged::kAppendHeads;
+    const long long blocks = (desc->n_tokens * groups + paged::kAppendThreads / 32 - 1) / (paged::kAppendThreads / 32);
+    if (blocks > INT_MAX) return set_error(P100_ERR_INVALID, "too many heads and tokens for one call");
+    switch (qkv_type) {
+        case P100_F32: return launch_append_to<float>(prm, desc->dtype, desc->head_dim, unsigned(blocks), stream);
+        case P100_F16: return launch_append_to<__half>(prm, desc->dtype, desc->head_dim, unsigned(blocks), stream);
+        default: return launch_append_to<__nv_bfloat16>(prm, desc->dtype, desc->head_dim, unsigned(blocks), stream);
+    }
+}
+
+size_t p100_fa_paged_workspace_size(const p100_paged_desc* desc) {
+    clear_error();
+    paged::Desc d = {};
+    int sms = 0;
+    if (!desc) {
+        set_error(P100_ERR_INVALID, "null descriptor");
+        return 0;
+    }
+    if (const char* why = paged_reason(*desc, d)) {
+        set_error(P100_ERR_INVALID, "%s", why);
+        return 0;
+    }
+    if (require_sm100(nullptr, &sms)) return 0;
+    return fa_paged_ws(*desc, sms).total;
+}
+
+p100_status p100_fa_paged_workspace_init(void* ws, size_t ws_bytes, p100_stream_t stream) {
+    clear_error();
+    int sms = 0;
+    if (p100_status st = require_sm100(nullptr, &sms)) return st;
+    if (!ws || !ws_bytes) return P100_OK;
+    return cuda_status(cudaMemsetAsync(ws, 0, std::min(ws_bytes, fa_paged_ticket_bytes(sms)), stream),
+                       "cudaMemsetAsync(workspace)");
+}
+
+p100_status p100_fa_paged(const p100_paged_desc* desc, const void* q, const void* k_pages, const void* v_pages,
+                          const int* block_table, const int* q_start, const int* kv_len, void* o, float* lse, void* ws,
+                          size_t ws_bytes, p100_stream_t stream) {
+    clear_error();
+    if (!desc) return set_error(P100_ERR_INVALID, "null descriptor");
+    fap::Params prm = {};
+    if (const char* why = paged_reason(*desc, prm.d)) return set_error(P100_ERR_INVALID, "%s", why);
+    int sms = 0;
+    if (p100_status st = require_sm100(nullptr, &sms)) return st;
+    if (desc->n_tokens == 0 || desc->n_seq == 0) return P100_OK;
+    if (!q || !k_pages || !v_pages || !block_table || !q_start || !kv_len || !o)
+        return set_error(P100_ERR_INVALID, "null buffer");
+    if (!aligned(q, 16) || !aligned(o, 16) || !aligned(k_pages, 16) || !aligned(v_pages, 16))
+        return set_error(P100_ERR_INVALID, "q, o and the pages must be 16-byte aligned");
+    const FaPagedWs w = fa_paged_ws(*desc, sms);
+    if (ws_bytes < w.total || !ws)
+        return set_error(P100_ERR_INVALID, "workspace of %zu bytes needed, %zu given", w.total, ws ? ws_bytes : size_t(0));
+    if (!aligned(ws, 256)) return set_error(P100_ERR_INVALID, "workspace must be 256-byte aligned");
+    prm.d.block_table = block_table;
+    prm.d.q_start = q_start;
+    prm.d.kv_len = kv_len;
+    prm.q = q;
+    prm.k = k_pages;
+    prm.v = v_pages;
+    prm.o = o;
+    prm.o_f32 = desc->o_fp32 != 0;
+    prm.lse = lse;
+    uint8_t* at = static_cast<uint8_t*>(ws);
+    prm.tickets = reinterpret_cast<unsigned*>(at);
+    prm.ws_o = reinterpret_cast<float*>(at + w.tickets);
+    prm.ws_ml = reinterpret_cast<float*>(at + w.tickets + w.o);
+    prm.scale = desc->scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(desc->head_dim)) : desc->scale;
+    prm.softcap = desc->softcap;
+    if (desc->dtype == P100_F16)
+        return desc->head_dim == 64 ? launch_fa_paged_mma<__half, 64>(prm, sms, stream)
+                                    : launch_fa_paged_mma<__half, 128>(prm, sms, stream);
+    return desc->head_dim == 64 ? launch_fa_paged_mma<__nv_bfloat16, 64>(prm, sms, stream)
+                                : launch_fa_paged_mma<__nv_bfloat16, 128>(prm, sms, stream);
+}
+
+size_t p100_logprobs_workspace_size(int rows, int n, int dtype, int top_k) {
+    clear_error();
+    int sms = 0;
+    if (const char* why = logprobs_reason(rows, n, dtype, top_k)) {
+        set_error(P100_ERR_INVALID, "%s", why);
+        return 0;
+    }
+    if (require_sm100(nullptr, &sms)) return 0;
+    return logprobs_ws(rows, logprobs_parts(rows, n, dtype, sms), top_k, sms).total;
+}
+
+p100_status p100_logprobs_workspace_init(void* ws, size_t ws_bytes, p100_stream_t stream) {
+    clear_error();
+    if (p100_status st = require_sm100(nullptr, nullptr)) return st;
+    if (!ws || !ws_bytes) return P100_OK;
+    return cuda_status(cudaMemsetAsync(ws, 0, ws_bytes, stream), "cudaMemsetAsync(workspace)");
+}
+
+p100_status p100_logprobs(const void* logits, int dtype, int n, int rows, long long row_stride, const int* token,
+                          int top_k, float* logprob, float* entropy, int* rank, int* top_index, float* top_logprob,
+                          void* ws, size_t ws_bytes, p100_stream_t stream) {
+    clear_error();
+    if (const char* why = logprobs_reason(rows, n, dtype, top_k)) return set_error(P100_ERR_INVALID, "%s", why);
+    if (row_stride == 0) row_stride = n;
+    if (row_stride < n) return set_error(P100_ERR_INVALID, "row_stride must be at least n");
+    if ((logprob || rank) && !token) return set_error(P100_ERR_INVALID, "logprob and rank need tokens");
+    if (top_k > 0 && (!top_index || !top_logprob))
+        return set_error(P100_ERR_INVALID, "top_k needs top_index and top_logprob");
+    int sms = 0;
+    if (p100_status st = require_sm100(nullptr, &sms)) return st;
+    if (rows == 0) return P100_OK;
+    if (!logits) return set_error(P100_ERR_INVALID, "null buffer");
+    if (!aligned(logits, dtype_bytes(dtype))) return set_error(P100_ERR_INVALID, "logits must be aligned to their type");
+    lp::Params prm = {};
+    prm.x = logits;
+    prm.stride = row_stride;
+    prm.n = n;
+    prm.rows = rows;
+    prm.parts = logprobs_parts(rows, n, dtype, sms);
+    const int vec = int(16 / dtype_bytes(dtype));
+    prm.part_len = int(((long long)n + (long long)prm.parts * vec - 1) / ((long long)prm.parts * vec)) * vec;
+    const LogprobsWs w = logprobs_ws(rows, prm.parts, top_k, sms);
+    if (w.total > ws_bytes || (w.total && !ws))
+        return set_error(P100_ERR_INVALID, "workspace of %zu bytes needed, %zu given", w.total, ws ? ws_bytes : size_t(0));
+    if (w.total && !aligned(ws, 256)) return set_error(P100_ERR_INVALID, "workspace must be 256-byte aligned");
+    prm.top = top_k;
+    prm.token = token;
+    prm.logprob = logprob;
+    prm.entropy = entropy;
+    prm.rank = rank;
+    prm.top_index = top_index;
+    prm.top_logprob = top_logprob;
+    if (w.total) {
+        uint8_t* at = static_cast<uint8_t*>(ws);
+        prm.tickets = reinterpret_cast<unsigned*>(at);
+        prm.ws_sums = reinterpret_cast<float4*>(at + w.tickets);
+        prm.ws_keys = reinterpret_cast<unsigned long long*>(at + w.tickets + w.sums);
+    }
+    if ((long long)rows * prm.parts > INT_MAX) return set_error(P100_ERR_INVALID, "too many rows for one call");
+    const unsigned grid = unsigned(rows) * unsigned(prm.parts);
+    switch (dtype) {
+        case P100_F32: lp::logprobs_kernel<float><<<grid, lp::kThreads, 0, stream>>>(prm); break;
+        case P100_F16: lp::logprobs_kernel<__half><<<grid, lp::kThreads, 0, stream>>>(prm); break;
+        default: lp::logprobs_kernel<__nv_bfloat16><<<grid, lp::kThreads, 0, stream>>>(prm); break;
+    }
+    return cuda_status(cudaGetLastError(), "logprobs_kernel launch");
+}
+
+}  // extern "C"
