@@ -12,6 +12,7 @@
 
 #include "common.cuh"
 #include "fa_paged.cuh"
+#include "fa_paged_tc.cuh"
 #include "logprobs.cuh"
 #include "paged_append.cuh"
 
@@ -88,19 +89,76 @@ const char* paged_reason(const p100_paged_desc& in, paged::Desc& d) {
 // CTAs of the mma.sync kernel: two on every SM.
 constexpr int kMmaCtas = 2;
 
+// The tensor-core kernel takes calls in which a sequence may have more rows
+// (new tokens x query heads per kv head) than the mma.sync kernel's row tile,
+// if the pages can be copied by boxes of whole rows.
+bool fa_paged_on_tc(const paged::Desc& d) {
+    return (long long)d.max_q * d.group > fap::kRows && d.page_size % 8 == 0 && d.n_pages > 0;
+}
+
+// Partials of both kernels share one place: their calls follow one another.
 struct FaPagedWs {
-    size_t o, ml, tickets, total;
+    size_t tickets, o, ml, total;
 };
+size_t fa_paged_ticket_bytes(int sms) { return round256(size_t(sms) * kMmaCtas * sizeof(unsigned)); }
 FaPagedWs fa_paged_ws(const p100_paged_desc& in, int sms) {
-    const size_t ctas = size_t(sms) * kMmaCtas;
+    const size_t rows = size_t(sms) * 2 * std::max(kMmaCtas * fap::kRows, fatc::kRows);
     FaPagedWs w;
-    w.tickets = round256(ctas * sizeof(unsigned));   // first, so that init clears little
-    w.o = round256(ctas * 2 * fap::kRows * in.head_dim * sizeof(float));
-    w.ml = round256(ctas * 2 * fap::kRows * 2 * sizeof(float));
+    w.tickets = fa_paged_ticket_bytes(sms);   // first, so that init clears little
+    w.o = round256(rows * in.head_dim * sizeof(float));
+    w.ml = round256(rows * 2 * sizeof(float));
     w.total = w.tickets + w.o + w.ml;
     return w;
 }
-size_t fa_paged_ticket_bytes(int sms) { return round256(size_t(sms) * kMmaCtas * sizeof(unsigned)); }
+
+// The pages as a 4-d tensor (head_dim, token of the page, kv head, page) in
+// boxes of 64 values x `box` tokens with the 128-byte swizzle.
+p100_status page_map(CUtensorMap* map, const void* base, const p100_paged_desc& in, const paged::Desc& d, int box) {
+    static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess) {
+            (void)cudaGetLastError();
+            f = nullptr;
+        }
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    }();
+    if (!encode) return set_error(P100_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[4] = {cuuint64_t(in.head_dim), cuuint64_t(d.page_size), cuuint64_t(d.n_head_kv),
+                                cuuint64_t(d.n_pages)};
+    const cuuint64_t strides[3] = {cuuint64_t(d.token_stride) * 2, cuuint64_t(d.head_stride) * 2,
+                                   cuuint64_t(d.page_stride) * 2};
+    const cuuint32_t boxes[4] = {64, cuuint32_t(box), 1, 1};
+    const cuuint32_t elem[4] = {1, 1, 1, 1};
+    const CUresult r =
+        encode(map, in.dtype == P100_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+               const_cast<void*>(base), dims, strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return set_error(P100_ERR_INVALID, "page tensor map rejected (error %d): strides or extents", int(r));
+    return P100_OK;
+}
+
+template <typename T, int D, bool CAP>
+p100_status launch_fa_paged_tc(const fatc::Params& prm, const CUtensorMap& tmk, const CUtensorMap& tmv, int sms,
+                               cudaStream_t stream) {
+    static thread_local int configured[64] = {};
+    auto kern = fatc::fa_paged_tc_kernel<T, D, CAP>;
+    if (p100_status st = allow_smem(kern, fatc::smem_bytes<D>(), configured, "cudaFuncSetAttribute(fa_paged_tc)")) return st;
+    kern<<<sms, fatc::kThreads, fatc::smem_bytes<D>(), stream>>>(prm, tmk, tmv);
+    return cuda_status(cudaGetLastError(), "fa_paged_tc_kernel launch");
+}
+template <typename T>
+p100_status launch_fa_paged_tc_d(const fatc::Params& prm, int head_dim, const CUtensorMap& tmk, const CUtensorMap& tmv,
+                                 int sms, cudaStream_t s) {
+    const bool cap = prm.softcap != 0.0f;
+    if (head_dim == 64)
+        return cap ? launch_fa_paged_tc<T, 64, true>(prm, tmk, tmv, sms, s)
+                   : launch_fa_paged_tc<T, 64, false>(prm, tmk, tmv, sms, s);
+    return cap ? launch_fa_paged_tc<T, 128, true>(prm, tmk, tmv, sms, s)
+               : launch_fa_paged_tc<T, 128, false>(prm, tmk, tmv, sms, s);
+}
 
 template <typename T, int D>
 p100_status launch_fa_paged_mma(const fap::Params& prm, int sms, cudaStream_t stream) {
@@ -271,6 +329,25 @@ p100_status p100_fa_paged(const p100_paged_desc* desc, const void* q, const void
     prm.ws_ml = reinterpret_cast<float*>(at + w.tickets + w.o);
     prm.scale = desc->scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(desc->head_dim)) : desc->scale;
     prm.softcap = desc->softcap;
+    if (fa_paged_on_tc(prm.d)) {
+        fatc::Params t = {};
+        t.d = prm.d;
+        t.q = prm.q;
+        t.o = prm.o;
+        t.o_f32 = prm.o_f32;
+        t.lse = prm.lse;
+        t.ws_o = prm.ws_o;
+        t.ws_ml = prm.ws_ml;
+        t.tickets = prm.tickets;
+        t.scale = prm.scale;
+        t.softcap = prm.softcap;
+        t.box = std::min(fatc::kKeys, prm.d.page_size & -prm.d.page_size);
+        CUtensorMap tmk, tmv;
+        if (p100_status st = page_map(&tmk, k_pages, *desc, prm.d, t.box)) return st;
+        if (p100_status st = page_map(&tmv, v_pages, *desc, prm.d, t.box)) return st;
+        return desc->dtype == P100_F16 ? launch_fa_paged_tc_d<__half>(t, desc->head_dim, tmk, tmv, sms, stream)
+                                       : launch_fa_paged_tc_d<__nv_bfloat16>(t, desc->head_dim, tmk, tmv, sms, stream);
+    }
     if (desc->dtype == P100_F16)
         return desc->head_dim == 64 ? launch_fa_paged_mma<__half, 64>(prm, sms, stream)
                                     : launch_fa_paged_mma<__half, 128>(prm, sms, stream);
