@@ -19,6 +19,8 @@
 // the shares leaves its partials {m, l, unnormalised o} in the workspace and
 // its last CTA (an atomic ticket, no waiting) joins them in share order.
 #pragma once
+#include <climits>
+
 #include "paged.cuh"
 
 namespace p100b {
@@ -30,6 +32,7 @@ using paged::Lengths;
 
 constexpr int kThreads = 128;
 constexpr int kRows = 16, kKeys = 64;
+constexpr int kOver = 1;   // what a row tile costs beyond its keys, in units
 constexpr int kStages = 3;
 constexpr int kOffs = 5;   // tiles whose row offsets are held
 
@@ -116,23 +119,23 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_kernel(const Params p) {
     const Desc& d = p.d;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    paged::read_lengths<kRows, kKeys, kThreads>(d, len);
+    paged::read_lengths<kRows, kKeys, kOver, kThreads>(d, len, LLONG_MAX);
     if (!len.ok) return;
     // at least one unit a share: every CTA between a cut tile's first and last
     // then holds a part of it
     const int parts = int(min((long long)gridDim.x, len.total));
     if (int(blockIdx.x) >= parts) return;
-    paged::Share<kRows, kKeys> share;
+    paged::Share<kRows, kKeys, kOver> share;
     share.begin(d, len, blockIdx.x, parts);
     Item it;
     const float to_log2 = p.scale * kLog2e;
     const float cap_in = p.softcap != 0.f ? 2.f * to_log2 / p.softcap : 0.f;
 
     while (share.next(d, len, it)) {
-        const int q0 = len.q0[it.seq], n = len.q0[it.seq + 1] - q0, kv = len.kv[it.seq];
+        const int q0 = len.q0[it.seq], n = it.n, kv = it.kv;
         const int rows = min(kRows, n * d.group - it.tile * kRows);
         const int row0 = it.tile * kRows;
-        const int end = paged::key_end<kRows, kKeys>(d, n, kv, it.tile);   // keys any row sees
+        const int end = paged::key_end<kRows>(d, n, kv, it.tile);   // keys any row sees
         const int* table = d.block_table + (long long)it.seq * d.max_pages;
         const long long head_off = it.head * d.head_stride;
 

@@ -46,9 +46,18 @@ using paged::Item;
 using paged::Lengths;
 
 constexpr int kRows = 256, kKeys = 128;
-constexpr int kThreads = 320;
+constexpr int kOver = 2;                  // what a row tile costs beyond its keys, in units
+constexpr int kWholeFrom = 4;             // row tiles per CTA from which they are dealt out whole
+constexpr int kThreads = 384;             // two softmax warpgroups; one of the two issuing warps and two idle ones
 constexpr int kMmaWarp = 8, kLoadWarp = 9;
+// Registers a thread after the split; 256 x 208 + 128 x 88 is what the block
+// is launched with (384 x 168).
+constexpr int kSoftmaxRegs = 208, kIssueRegs = 88;
+static_assert(256 * kSoftmaxRegs + 128 * kIssueRegs <= kThreads * 168, "register split");
 constexpr int kSub = 128 * 128;           // bytes of 128 rows x 64 values
+// Pairs of probabilities that exp2_poly computes, of every kPolyOf: it and the
+// special-function unit then take about the same time.
+constexpr int kPoly = 1, kPolyOf = 4;
 constexpr float kRise = 8.0f;             // log2 of the rise that forces a rescale
 
 template <int D>
@@ -69,12 +78,23 @@ struct Params {
     int box;            // rows of a TMA box
 };
 
+// An item as the load warp hands it to the others, kJobs of them in a ring.
+struct Job {
+    int count;           // key tiles; 0: no more items
+    int key_tile, row0;  // first key tile; first row of the row tile in its kv head
+    int q0, n, kv, end, head;
+    int whole, c0, c1;   // no other CTA has a part, or the CTAs that do
+};
+constexpr int kJobs = 4;
+
 struct Barriers {
-    uint64_t full[6], empty[6], q_full[2], s_full[2], p_full[2], joined[2], drain;
+    uint64_t full[6], empty[6], q_full[2], s_full[2], p_full[2], joined[2], job_full[kJobs], job_empty[kJobs], drain;
     uint32_t tmem;
     int abort;
     int last[2];
+    Job jobs[kJobs];
 };
+using Units = paged::Share<kRows, kKeys, kOver>;
 
 template <int D>
 constexpr size_t smem_bytes() {
@@ -89,7 +109,8 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo, uin
     return uint64_t((saddr >> 4) & 0x3fffu) | uint64_t((lbo >> 4) & 0x3fffu) << 16 |
            uint64_t((sbo >> 4) & 0x3fffu) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
 }
-// kind::f16 with FP32 accumulation, M = 128.
+// kind::f16 with FP32 accumulation, M = 128; bit 13 negates A.
+constexpr uint32_t kNegateA = 1u << 13;
 template <typename T>
 __device__ __forceinline__ constexpr uint32_t idesc_f16(int n, bool b_n_major) {
     const uint32_t t = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
@@ -128,14 +149,14 @@ __device__ __forceinline__ void ld32(uint32_t a, float* r) {
         : "r"(a)
         : "memory");
 }
-__device__ __forceinline__ void st32(uint32_t a, const float* r) {
+// 16 columns.
+__device__ __forceinline__ void ld16(uint32_t a, float* r) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(a),
-        "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]),
-        "f"(r[10]), "f"(r[11]), "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15]), "f"(r[16]), "f"(r[17]), "f"(r[18]),
-        "f"(r[19]), "f"(r[20]), "f"(r[21]), "f"(r[22]), "f"(r[23]), "f"(r[24]), "f"(r[25]), "f"(r[26]), "f"(r[27]),
-        "f"(r[28]), "f"(r[29]), "f"(r[30]), "f"(r[31])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+        : "r"(a)
         : "memory");
 }
 __device__ __forceinline__ void st16(uint32_t a, const uint32_t* r) {
@@ -145,6 +166,12 @@ __device__ __forceinline__ void st16(uint32_t a, const uint32_t* r) {
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+
+__device__ __forceinline__ void st8(uint32_t a, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(a), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 
 // Waits for a barrier phase, for at most kWaitLimitNs or until the CTA aborts.
@@ -167,12 +194,59 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* a
     return __all_sync(0xffffffffu, wait_bar(bar, parity, abort));
 }
 
+// ------------------------------------------------------------ pairs of floats
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// 2^x of two finite x <= 8 on the FMA pipe: x = n + f with |f| <= 1/2 (adding
+// 1.5 * 2^23 rounds to an integer), a polynomial of degree 4 for 2^f whose
+// coefficients were fitted to the least relative error (2.7e-6, mean 4e-8:
+// far below the rounding to 16 bits that follows, and without bias in the
+// sum), and n added to the exponent.
+__device__ __forceinline__ void exp2_poly(uint64_t x2, float& a, float& b) {
+    float x, y;
+    unpair(x2, x, y);
+    x2 = pair(fmaxf(x, -125.f), fmaxf(y, -125.f));
+    const uint64_t t = add2(x2, pair(12582912.f, 12582912.f));
+    const uint64_t f = fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), x2);
+    uint64_t r = fma2(f, pair(0.009570050984621048f, 0.009570050984621048f), pair(0.05591786280274391f, 0.05591786280274391f));
+    r = fma2(f, r, pair(0.2402474582195282f, 0.2402474582195282f));
+    r = fma2(f, r, pair(0.6931217908859253f, 0.6931217908859253f));
+    r = fma2(f, r, pair(0.9999992847442627f, 0.9999992847442627f));
+    float tx, ty;
+    unpair(t, tx, ty);
+    unpair(r, a, b);
+    a = __int_as_float(__float_as_int(a) + (__float_as_int(tx) << 23));
+    b = __int_as_float(__float_as_int(b) + (__float_as_int(ty) << 23));
+}
+
 // ------------------------------------------------------------ roles
-// K and V tiles of the CTA's items into the ring, in the order the products
-// take them.
+// Hands out the CTA's items and brings their K and V tiles into the ring, in
+// the order the products take them.
 template <int D>
 __device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tmk, const CUtensorMap* tmv, Lengths& len,
-                                          Barriers& bars, uint8_t* ring, paged::Share<kRows, kKeys> share) {
+                                          Barriers& bars, uint8_t* ring, Units share) {
     constexpr int NS = slots<D>();
     const Desc& d = p.d;
     const int lane = threadIdx.x & 31;
@@ -182,10 +256,33 @@ __device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tm
     const uint32_t at = uint32_t(half) * kSub + uint32_t(i) * p.box * 128;
     unsigned used = 0;                               // slots filled so far
     bool ok = true;
-    Item it;
-    while (ok && share.next(d, len, it)) {
-        const int q0 = len.q0[it.seq];
-        const int end = paged::key_end<kRows, kKeys>(d, len.q0[it.seq + 1] - q0, len.kv[it.seq], it.tile);
+    for (unsigned j = 0; ok; ++j) {
+        Item it;
+        const bool more = share.next(d, len, it);
+        if (j >= kJobs) ok = warp_wait(&bars.job_empty[j % kJobs], (j / kJobs - 1) & 1, &bars.abort);
+        if (!ok) break;
+        int end = 0;
+        if (more) end = paged::key_end<kRows>(d, it.n, it.kv, it.tile);
+        if (lane == 0) {
+            Job& job = bars.jobs[j % kJobs];
+            job.count = more ? it.count : 0;
+            if (more) {
+                job.key_tile = it.key_tile;
+                job.row0 = it.tile * kRows;
+                job.q0 = len.q0[it.seq];
+                job.n = it.n;
+                job.kv = it.kv;
+                job.end = end;
+                job.head = it.head;
+                job.whole = it.count == it.units;
+                if (!job.whole) {
+                    job.c0 = paged::share_of(it.tile_first, len.total, share.parts);
+                    job.c1 = paged::share_of(it.tile_first + it.units - 1, len.total, share.parts);
+                }
+            }
+            mbar_arrive(&bars.job_full[j % kJobs]);
+        }
+        if (!more) break;
         const int* table = d.block_table + (long long)it.seq * d.max_pages;
         auto find = [&](int t, int& page, int& off) {
             const int key = (it.key_tile + t) * kKeys + i * p.box;
@@ -233,21 +330,23 @@ __device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tm
         for (unsigned u = used > NS ? used - NS : 0; u < used; ++u) mbar_wait(&bars.full[u % NS], (u / NS) & 1);
 }
 
+// One lane issues the products; false when a wait was given up.
 template <typename T, int D>
-__device__ __forceinline__ bool mma_role(const Params& p, Lengths& len, Barriers& bars, uint32_t q_smem, uint32_t ring,
-                                         uint32_t tmem, paged::Share<kRows, kKeys> share) {
+__device__ __forceinline__ bool mma_role(const Desc& d, float scale, Barriers& bars, uint32_t q_smem, uint32_t ring,
+                                         uint32_t tmem) {
     constexpr int NS = slots<D>();
-    constexpr uint32_t kIdescS = idesc_f16<T>(kKeys, false), kIdescO = idesc_f16<T>(D, true);
+    // a negative scale turns the scores' sign here, so that the softmax has a positive one
+    const uint32_t idesc_s = idesc_f16<T>(kKeys, false) | (scale < 0.f ? kNegateA : 0u);
+    constexpr uint32_t kIdescO = idesc_f16<T>(D, true);
     const int lane = threadIdx.x & 31;
     unsigned used = 0;                 // K and V tiles taken so far
     unsigned items[2] = {0, 0}, tiles[2] = {0, 0};
-    Item it;
     auto qk = [&](int w, int slot) {   // S_w = Q_w K^T
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
             const uint32_t off = uint32_t(k >> 2) * kSub + uint32_t(k & 3) * 32;
             mma_ss(tmem + w * 128, sw128_desc(q_smem + w * tile_bytes<D>() + off, 16, 1024),
-                   sw128_desc(ring + slot * tile_bytes<D>() + off, 16, 1024), kIdescS, k > 0);
+                   sw128_desc(ring + slot * tile_bytes<D>() + off, 16, 1024), idesc_s, k > 0);
         }
     };
     auto pv = [&](int w, int slot, bool add) {   // O_w += P_w V
@@ -256,24 +355,28 @@ __device__ __forceinline__ bool mma_role(const Params& p, Lengths& len, Barriers
             mma_ts(tmem + 256 + w * D, tmem + w * 128 + k * 8,
                    sw128_desc(ring + slot * tile_bytes<D>() + uint32_t(k) * 2048, kSub, 1024), kIdescO, add || k > 0);
     };
-    while (share.next(p.d, len, it)) {
-        const int n = len.q0[it.seq + 1] - len.q0[it.seq];
-        const int groups = n * p.d.group - it.tile * kRows > 128 ? 2 : 1;
-        for (int w = 0; w < groups; ++w)
-            if (!warp_wait(&bars.q_full[w], items[w]++ & 1, &bars.abort)) return false;
+    for (unsigned j = 0;; ++j) {
+        if (!warp_wait(&bars.job_full[j % kJobs], (j / kJobs) & 1, &bars.abort)) return false;
+        const Job& job = bars.jobs[j % kJobs];
+        const int count = job.count;
+        if (count == 0) return true;
+        const int groups = job.n * d.group - job.row0 > 128 ? 2 : 1;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.job_empty[j % kJobs]);
         if (!warp_wait(&bars.full[used % NS], (used / NS) & 1, &bars.abort)) return false;
-        fence_after();
-        if (lane == 0) {
-            for (int w = 0; w < groups; ++w) {
+        for (int w = 0; w < groups; ++w) {
+            if (!warp_wait(&bars.q_full[w], items[w]++ & 1, &bars.abort)) return false;
+            fence_after();
+            if (lane == 0) {
                 qk(w, used % NS);
                 mma_commit(&bars.s_full[w]);
+                if (w + 1 == groups) mma_commit(&bars.empty[used % NS]);
             }
-            mma_commit(&bars.empty[used % NS]);
         }
         ++used;
-        for (int t = 0; t < it.count; ++t) {
+        for (int t = 0; t < count; ++t) {
             const unsigned v = used, k = used + 1;
-            const bool more = t + 1 < it.count;
+            const bool more = t + 1 < count;
             if (!warp_wait(&bars.full[v % NS], (v / NS) & 1, &bars.abort)) return false;
             for (int w = 0; w < groups; ++w) {
                 if (!warp_wait(&bars.p_full[w], tiles[w]++ & 1, &bars.abort)) return false;
@@ -292,70 +395,101 @@ __device__ __forceinline__ bool mma_role(const Params& p, Lengths& len, Barriers
             used += more ? 2 : 1;
         }
     }
-    return true;
+}
+
+// The row of a thread in an item.
+struct Row {
+    int tok, g, limit;   // token of the sequence, query head of the group, keys it sees
+    bool live;
+    __device__ __forceinline__ Row(const Desc& d, const Job& job, int w, int row) {
+        const int rows = job.n * d.group - job.row0 - w * 128;
+        const int r = job.row0 + w * 128 + row;
+        tok = r / d.group;
+        g = r - tok * d.group;
+        live = row < rows;
+        limit = !live ? 0 : d.causal ? max(0, min(job.kv, job.kv - job.n + tok + 1)) : job.kv;
+    }
+    __device__ __forceinline__ long long at(const Desc& d, const Job& job, long long stride, int D) const {
+        return (long long)(job.q0 + tok) * stride + (long long)(job.head * d.group + g) * D;
+    }
+};
+
+// The thread's query row on its way into shared memory (zeros for none).
+template <typename T, int D>
+__device__ __forceinline__ void load_query(const Params& p, const Job& job, int w, int row, uint32_t q_smem) {
+    const Row r(p.d, job, w, row);
+    const T* src = static_cast<const T*>(p.q) + (r.live ? r.at(p.d, job, p.d.q_stride, D) : 0);
+    const uint32_t dst = q_smem + w * tile_bytes<D>() + row * 128;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) fap::cp_async16(dst + (i >> 3) * kSub + (((i & 7) ^ (row & 7)) << 4), src + i * 8, r.live);
 }
 
 template <typename T, int D, bool CAP>
-__device__ __forceinline__ void softmax_role(const Params& p, Lengths& len, Barriers& bars, uint8_t* q_smem, uint8_t* ring,
-                                             uint32_t tmem, int parts, paged::Share<kRows, kKeys> share) {
+__device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, uint32_t q_smem, uint8_t* ring, uint32_t tmem) {
     constexpr int NS = slots<D>();
     constexpr float kLog2e = 1.4426950408889634f;
     const Desc& d = p.d;
     const int w = threadIdx.x >> 7, row = threadIdx.x & 127;
     const uint32_t lanes = uint32_t(row & ~31) << 16;
     const uint32_t t_s = tmem + w * 128 + lanes, t_o = tmem + 256 + w * D + lanes;
-    // scores in units of log2 e; a negative scale turns the queries' sign
+    // the scores' unit: log2 e / scale, or log2 once capped
     const float c = CAP ? 1.0f : fabsf(p.scale) * kLog2e;
     const float cap_in = CAP ? 2.f * fabsf(p.scale) * kLog2e / p.softcap : 0.f, cap = p.softcap * kLog2e;
-    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
     unsigned done = 0, used = 0;   // phases of s_full passed; key tiles of the CTA before this item
-    Item it;
-    while (share.next(d, len, it)) {
-        const int q0 = len.q0[it.seq], n = len.q0[it.seq + 1] - q0, kv = len.kv[it.seq];
-        const int first_row = it.tile * kRows + w * 128;
-        const int rows = min(128, n * d.group - first_row);
-        const unsigned tile0 = used;
-        used += it.count;
-        if (rows <= 0) continue;
-        const int r = first_row + row;
-        const int tok = r / d.group, g = r - tok * d.group;
-        const bool live = row < rows;
-        const int limit = !live ? 0 : d.causal ? max(0, min(kv, kv - n + tok + 1)) : kv;
-        const int end = paged::key_end<kRows, kKeys>(d, n, kv, it.tile);
-        {
-            const T* src = static_cast<const T*>(p.q) + (long long)(q0 + tok) * d.q_stride + (long long)(it.head * d.group + g) * D;
-            uint8_t* dst = q_smem + w * tile_bytes<D>() + row * 128;
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                uint4 v = live ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
-                v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-                *reinterpret_cast<uint4*>(dst + (i >> 3) * kSub + (((i & 7) ^ (row & 7)) << 4)) = v;
-            }
-            fence_async();
-            fence_before();
-            mbar_arrive(&bars.q_full[w]);
+    bool loaded = false;           // the item's query row is on its way
+    for (unsigned j = 0;; ++j) {
+        if (!warp_wait(&bars.job_full[j % kJobs], (j / kJobs) & 1, &bars.abort)) return;
+        const Job& job = bars.jobs[j % kJobs];
+        const int count = job.count;
+        if (count == 0) return;
+        if (job.n * d.group - job.row0 - w * 128 <= 0) {   // no rows for this warpgroup
+            used += count;
+            __syncwarp();
+            if ((row & 31) == 0) mbar_arrive(&bars.job_empty[j % kJobs]);
+            loaded = false;
+            continue;
         }
+        if (!loaded) load_query<T, D>(p, job, w, row, q_smem);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_async();
+        fence_before();
+        mbar_arrive(&bars.q_full[w]);
+        loaded = false;
+        const int limit = Row(d, job, w, row).limit;
         float m = -INFINITY, l = 0.f;
-        for (int t = 0; t < it.count; ++t) {
+        int key0 = job.key_tile * kKeys;
+        for (int t = 0; t < count; ++t, key0 += kKeys) {
             if (!warp_wait(&bars.s_full[w], done++ & 1, &bars.abort)) return;
             fence_after();
             float s[128];
 #pragma unroll
             for (int i = 0; i < 4; ++i) ld32(t_s + i * 32, s + i * 32);
             wait_ld();
-            const int key0 = (it.key_tile + t) * kKeys;
+            if (t + 1 == count) {   // the last scores are there, so the queries' place is free for the next item's
+                if (!warp_wait(&bars.job_full[(j + 1) % kJobs], ((j + 1) / kJobs) & 1, &bars.abort)) return;
+                const Job& next = bars.jobs[(j + 1) % kJobs];
+                if (next.count && next.n * d.group - next.row0 - w * 128 > 0) {
+                    load_query<T, D>(p, next, w, row, q_smem);
+                    loaded = true;
+                }
+            }
             if (CAP) {
 #pragma unroll
                 for (int i = 0; i < 128; ++i) s[i] = fap::cap_score(s[i], cap_in, cap);
             }
-            if (__any_sync(0xffffffffu, limit < key0 + kKeys)) {
+            const bool masked = __any_sync(0xffffffffu, limit < key0 + kKeys);
+            if (masked) {
                 const int lim = limit - key0;
 #pragma unroll
                 for (int i = 0; i < 128; ++i) s[i] = i < lim ? s[i] : -INFINITY;
             }
             float mx4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int i = 4; i < 128; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], s[i]);
+            for (int i = 4; i < 128; i += 8) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    mx4[e] = i + 4 + e < 128 ? fmaxf(fmaxf(mx4[e], s[i + e]), s[i + 4 + e]) : fmaxf(mx4[e], s[i + e]);
+            }
             const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
             if (t == 0) {
                 m = mx;
@@ -365,37 +499,65 @@ __device__ __forceinline__ void softmax_role(const Params& p, Lengths& len, Barr
                     const float a = rise ? paged::exp2_approx((m - mx) * c) : 1.f;
                     if (rise) m = mx;
                     l *= a;
-#pragma unroll
-                    for (int i = 0; i < D / 32; ++i) {
-                        float o[32];
-                        ld32(t_o + i * 32, o);
+#pragma unroll 1
+                    for (int i = 0; i < D / 16; ++i) {   // few registers: the scores stay in theirs
+                        float o[16];
+                        ld16(t_o + i * 16, o);
                         wait_ld();
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] *= a;
-                        st32(t_o + i * 32, o);
+                        for (int e = 0; e < 16; ++e) o[e] *= a;
+                        st16(t_o + i * 16, reinterpret_cast<const uint32_t*>(o));
                     }
                 }
             }
             const float base = m == -INFINITY ? 0.f : m * c;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint64_t c2 = pair(c, c), b2 = pair(-base, -base);
+            uint64_t sum[2] = {0, 0};
+            if (masked) {   // exp2 of -inf must be 0: the special-function unit alone
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t pk[16];
+                for (int i = 0; i < 8; ++i) {
+                    uint32_t pk[8];
 #pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    const float a = paged::exp2_approx(fmaf(s[i * 32 + j], c, -base));
-                    const float b = paged::exp2_approx(fmaf(s[i * 32 + j + 1], c, -base));
-                    sum[(j >> 1) & 1] += a;
-                    sum[2 + ((j >> 1) & 1)] += b;
-                    pk[j >> 1] = paged::pack2<T>(a, b);
+                    for (int e = 0; e < 16; e += 2) {
+                        float a, b;
+                        unpair(fma2(pair(s[i * 16 + e], s[i * 16 + e + 1]), c2, b2), a, b);
+                        a = paged::exp2_approx(a);
+                        b = paged::exp2_approx(b);
+                        sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair(a, b));
+                        pk[e >> 1] = paged::pack2<T>(a, b);
+                    }
+                    st8(t_s + i * 8, pk);
                 }
-                st16(t_s + i * 16, pk);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    uint32_t pk[8];
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        float a, b;
+                        const uint64_t x = fma2(pair(s[i * 16 + e], s[i * 16 + e + 1]), c2, b2);
+                        if (!CAP && (e >> 1) % kPolyOf < kPoly) {
+                            exp2_poly(x, a, b);
+                        } else {
+                            unpair(x, a, b);
+                            a = paged::exp2_approx(a);
+                            b = paged::exp2_approx(b);
+                        }
+                        sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair(a, b));
+                        pk[e >> 1] = paged::pack2<T>(a, b);
+                    }
+                    st8(t_s + i * 8, pk);
+                }
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            if (w == 0 && key0 + kKeys > end) {   // rows of V that no key of the tile's rows reaches
-                const unsigned u = 2 * (tile0 + t) + 1;
+            {
+                float a, b;
+                unpair(add2(sum[0], sum[1]), a, b);
+                l += a + b;
+            }
+            if (w == 0 && key0 + kKeys > job.end) {   // rows of V that no key of the item's rows reaches
+                const unsigned u = 2 * (used + t) + 1;
                 if (!warp_wait(&bars.full[u % NS], (u / NS) & 1, &bars.abort)) return;
-                if (key0 + row >= end) {
+                if (key0 + row >= job.end) {
                     uint8_t* v = ring + (u % NS) * tile_bytes<D>() + row * 128;
 #pragma unroll
                     for (int i = 0; i < D / 8; ++i)
@@ -407,32 +569,34 @@ __device__ __forceinline__ void softmax_role(const Params& p, Lengths& len, Barr
             fence_before();
             mbar_arrive(&bars.p_full[w]);
         }
+        used += count;
         if (!warp_wait(&bars.s_full[w], done++ & 1, &bars.abort)) return;   // the accumulator is complete
         fence_after();
+        const Row r(d, job, w, row);
         const float base = m == -INFINITY ? -INFINITY : m * c;
-        const long long o_at = (long long)(q0 + tok) * d.o_stride + (long long)(it.head * d.group + g) * D;
+        const long long o_at = r.at(d, job, d.o_stride, D);
         auto write = [&](int i, float (&o)[32], float inv) {   // columns 32 i .. 32 i + 31 of the row
-            if (!live) return;
+            if (!r.live) return;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] *= inv;
+            for (int e = 0; e < 32; ++e) o[e] *= inv;
             if (p.o_f32) {
                 float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.o) + o_at + i * 32);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             } else {
                 uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.o) + o_at + i * 32);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    dst[j] = make_uint4(paged::pack2<T>(o[8 * j], o[8 * j + 1]), paged::pack2<T>(o[8 * j + 2], o[8 * j + 3]),
-                                        paged::pack2<T>(o[8 * j + 4], o[8 * j + 5]), paged::pack2<T>(o[8 * j + 6], o[8 * j + 7]));
+                for (int e = 0; e < 4; ++e)
+                    dst[e] = make_uint4(paged::pack2<T>(o[8 * e], o[8 * e + 1]), paged::pack2<T>(o[8 * e + 2], o[8 * e + 3]),
+                                        paged::pack2<T>(o[8 * e + 4], o[8 * e + 5]), paged::pack2<T>(o[8 * e + 6], o[8 * e + 7]));
             }
         };
         auto write_lse = [&](float top, float total) {
-            if (live && p.lse)
-                p.lse[(long long)(q0 + tok) * d.n_head_q + it.head * d.group + g] =
+            if (r.live && p.lse)
+                p.lse[(long long)(job.q0 + r.tok) * d.n_head_q + job.head * d.group + r.g] =
                     total == 0.f ? -INFINITY : (top + log2f(total)) / kLog2e;
         };
-        if (it.count == it.units) {
+        if (job.whole) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
@@ -443,7 +607,8 @@ __device__ __forceinline__ void softmax_role(const Params& p, Lengths& len, Barr
             }
             write_lse(base, l);
         } else {
-            const long long slot = (long long)(blockIdx.x * 2 + (it.key_tile == 0)) * 2 + w;
+            const int c0 = job.c0, c1 = job.c1;
+            const long long slot = (long long)(blockIdx.x * 2 + (job.key_tile == 0)) * 2 + w;
             float4* dst = reinterpret_cast<float4*>(p.ws_o) + slot * (D / 4) * 128 + row;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
@@ -451,12 +616,10 @@ __device__ __forceinline__ void softmax_role(const Params& p, Lengths& len, Barr
                 ld32(t_o + i * 32, o);
                 wait_ld();
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    __stcg(dst + (i * 8 + j) * 128, make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
+                for (int e = 0; e < 8; ++e)
+                    __stcg(dst + (i * 8 + e) * 128, make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
             }
             __stcg(reinterpret_cast<float2*>(p.ws_ml) + slot * 128 + row, make_float2(base, l));
-            const int c0 = paged::share_of(it.tile_first, len.total, parts);
-            const int c1 = paged::share_of(it.tile_first + it.units - 1, len.total, parts);
             // one thread of the warpgroup takes the ticket when all have written
             __threadfence();
             mbar_arrive(&bars.joined[w]);
@@ -471,9 +634,11 @@ __device__ __forceinline__ void softmax_role(const Params& p, Lengths& len, Barr
                 const float4* po = reinterpret_cast<const float4*>(p.ws_o) + (long long)w * (D / 4) * 128 + row;
                 auto part = [&](int q) { return ((long long)q * 2 + (q == c0)) * 2; };
                 float top = -INFINITY;
+#pragma unroll 4
                 for (int q = c0; q <= c1; ++q) top = fmaxf(top, __ldcg(ml + part(q) * 128).x);
                 const float safe = top == -INFINITY ? 0.f : top;
                 float total = 0.f;
+#pragma unroll 4
                 for (int q = c0; q <= c1; ++q) {
                     const float2 v = __ldcg(ml + part(q) * 128);
                     total = fmaf(paged::exp2_approx(v.x - safe), v.y, total);
@@ -483,18 +648,19 @@ __device__ __forceinline__ void softmax_role(const Params& p, Lengths& len, Barr
                 for (int i = 0; i < D / 32; ++i) {
                     float o[32];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] = 0.f;
+                    for (int e = 0; e < 32; ++e) o[e] = 0.f;
+#pragma unroll 3
                     for (int q = c0; q <= c1; ++q) {
                         const float f = paged::exp2_approx(__ldcg(ml + part(q) * 128).x - safe);
                         float4 v[8];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) v[j] = __ldcg(po + (part(q) * (D / 4) + i * 8 + j) * 128);
+                        for (int e = 0; e < 8; ++e) v[e] = __ldcg(po + (part(q) * (D / 4) + i * 8 + e) * 128);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            o[4 * j] = fmaf(f, v[j].x, o[4 * j]);
-                            o[4 * j + 1] = fmaf(f, v[j].y, o[4 * j + 1]);
-                            o[4 * j + 2] = fmaf(f, v[j].z, o[4 * j + 2]);
-                            o[4 * j + 3] = fmaf(f, v[j].w, o[4 * j + 3]);
+                        for (int e = 0; e < 8; ++e) {
+                            o[4 * e] = fmaf(f, v[e].x, o[4 * e]);
+                            o[4 * e + 1] = fmaf(f, v[e].y, o[4 * e + 1]);
+                            o[4 * e + 2] = fmaf(f, v[e].z, o[4 * e + 2]);
+                            o[4 * e + 3] = fmaf(f, v[e].w, o[4 * e + 3]);
                         }
                     }
                     write(i, o, inv);
@@ -502,6 +668,8 @@ __device__ __forceinline__ void softmax_role(const Params& p, Lengths& len, Barr
                 write_lse(top, total);
             }
         }
+        __syncwarp();
+        if ((row & 31) == 0) mbar_arrive(&bars.job_empty[j % kJobs]);
     }
 }
 
@@ -521,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         prefetch_tensormap(&tmk);
         prefetch_tensormap(&tmv);
     }
-    paged::read_lengths<kRows, kKeys, kThreads>(p.d, len);
+    paged::read_lengths<kRows, kKeys, kOver, kThreads>(p.d, len, (long long)kWholeFrom * gridDim.x);
     const int parts = len.ok ? int(min((long long)gridDim.x, len.total)) : 0;
     if (int(blockIdx.x) >= parts) return;
     if (threadIdx.x == 0) {
@@ -534,6 +702,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&bars.s_full[w], 1);
             mbar_init(&bars.p_full[w], 128);
             mbar_init(&bars.joined[w], 128);
+        }
+        for (int i = 0; i < kJobs; ++i) {
+            mbar_init(&bars.job_full[i], 1);
+            mbar_init(&bars.job_empty[i], 9);   // the softmax warps and the issuing one
         }
         mbar_init(&bars.drain, 1);
         bars.abort = 0;
@@ -549,20 +721,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem);
-    paged::Share<kRows, kKeys> share;
-    share.begin(p.d, len, blockIdx.x, parts);
-
-    if (warp == kLoadWarp)
-        load_role<D>(p, &tmk, &tmv, len, bars, ring, share);
-    else if (warp == kMmaWarp) {
-        if (!mma_role<T, D>(p, len, bars, smem_addr(q_smem), smem_addr(ring), tmem, share)) {
-            // leave only when the products in flight are done
-            if ((threadIdx.x & 31) == 0) mma_commit(&bars.drain);
-            __syncwarp();
-            mbar_wait(&bars.drain, 0);
+    if (warp < kMmaWarp) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        softmax_role<T, D, CAP>(p, bars, smem_addr(q_smem), ring, tmem);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+        if (warp == kLoadWarp) {
+            Units share;
+            share.begin(p.d, len, blockIdx.x, parts);
+            load_role<D>(p, &tmk, &tmv, len, bars, ring, share);
+        } else if (warp == kMmaWarp) {
+            if (!mma_role<T, D>(p.d, p.scale, bars, smem_addr(q_smem), smem_addr(ring), tmem)) {
+                // leave only when the products in flight are done
+                if ((threadIdx.x & 31) == 0) mma_commit(&bars.drain);
+                __syncwarp();
+                mbar_wait(&bars.drain, 0);
+            }
         }
-    } else
-        softmax_role<T, D, CAP>(p, len, bars, q_smem, ring, tmem, parts, share);
+    }
 
     fence_before();
     __syncthreads();

@@ -69,24 +69,35 @@ __device__ __forceinline__ float rcp_approx(float x) {
 __device__ __forceinline__ void flag_input() { atomicExch(&g_device_error, kDevErrInput); }
 
 // ------------------------------------------------------------ shares
-// An attention call is a list of units, one unit = one tile of KEYS keys of
-// one tile of ROWS query rows of one (sequence, kv head).  The rows of a kv
-// head are the (token, query head of the group) pairs in token order, so a
-// tile serves every query head that reads its keys.  Units are ordered by
-// sequence, kv head, row tile, key tile; CTA c of P takes the units
-// [c U / P, (c + 1) U / P): every CTA gets the same amount whatever the
-// lengths, and a row tile is cut only where a share ends.  A row tile that
-// sees no key still counts one unit, which writes its zeros.
+// An attention call is a list of row tiles, each with the key tiles that its
+// rows see: unit = KEYS keys of ROWS query rows of one (sequence, kv head).
+// The rows of a kv head are the (token, query head of the group) pairs in
+// token order, so a tile serves every query head that reads its keys.  A row
+// tile that sees no key still has one unit, which writes its zeros.
+//
+// Cut: units are ordered by sequence, kv head, row tile, key tile, each row
+// tile with OVER more units behind it for what a row tile costs beyond its
+// keys, and CTA c of P takes [c U / P, (c + 1) U / P): equal work whatever the
+// lengths, a row tile cut only where a share ends.  Whole: with many row tiles
+// per CTA they are dealt out uncut, the ones with the most keys of a sequence
+// first and back and forth over the CTAs, so that neighbours in time read the
+// same keys and nothing is joined.
 struct Lengths {
-    long long total;                 // units of the call
+    long long total;                 // units (cut) or row tiles (whole) of the call
     int ok;                          // the lengths are usable
+    int whole;
     int q0[kMaxSeq + 1];
     int kv[kMaxSeq];
-    unsigned per_head[kMaxSeq];      // units of one kv head
-    unsigned long long first[kMaxSeq];   // units before the sequence
+    unsigned per_head[kMaxSeq];      // units or row tiles of one kv head
+    unsigned long long first[kMaxSeq];   // units or row tiles before the sequence
 };
 
-template <int ROWS, int KEYS>
+template <int ROWS>
+__device__ __forceinline__ int row_tiles(const Desc& d, int n) {
+    return int(((long long)n * d.group + ROWS - 1) / ROWS);
+}
+// Keys [0, key_end) are seen by some row of the tile.
+template <int ROWS>
 __device__ __forceinline__ int key_end(const Desc& d, int n, int kv, int tile) {
     const int last = min((tile + 1) * ROWS, n * d.group) - 1;
     const int end = d.causal ? kv - n + last / d.group + 1 : kv;
@@ -94,16 +105,17 @@ __device__ __forceinline__ int key_end(const Desc& d, int n, int kv, int tile) {
 }
 template <int ROWS, int KEYS>
 __device__ __forceinline__ int tile_units(const Desc& d, int n, int kv, int tile) {
-    return max(1, (key_end<ROWS, KEYS>(d, n, kv, tile) + KEYS - 1) / KEYS);
+    return max(1, (key_end<ROWS>(d, n, kv, tile) + KEYS - 1) / KEYS);
 }
 
 // Reads and checks the lengths and counts the units; every thread of the CTA
 // calls it.  Lengths that are out of order or out of range raise the device
-// flag and make the call do nothing.
-template <int ROWS, int KEYS, int THREADS>
-__device__ void read_lengths(const Desc& d, Lengths& s) {
+// flag and make the call do nothing.  Row tiles are dealt out whole from
+// whole_from of them on.
+template <int ROWS, int KEYS, int OVER, int THREADS>
+__device__ void read_lengths(const Desc& d, Lengths& s, long long whole_from) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (tid == 0) s.ok = 1;
+    if (tid == 0) s.ok = 1, s.total = 0;
     for (int i = tid; i <= d.n_seq; i += THREADS) s.q0[i] = d.q_start[i];
     for (int i = tid; i < d.n_seq; i += THREADS) s.kv[i] = d.kv_len[i];
     __syncthreads();
@@ -112,30 +124,39 @@ __device__ void read_lengths(const Desc& d, Lengths& s) {
         if (s.q0[i] < 0 || n < 0 || n > d.max_q || s.q0[i + 1] > d.n_tokens || s.kv[i] < 0 ||
             (long long)s.kv[i] > (long long)d.max_pages * d.page_size)
             s.ok = 0;
+        else
+            s.per_head[i] = row_tiles<ROWS>(d, n);
     }
     __syncthreads();
     if (!s.ok) {
         if (tid == 0) flag_input();
         return;
     }
-    // Sequences of few row tiles a thread each, longer ones a warp each.
-    for (int i = tid; i < d.n_seq; i += THREADS) {
-        const int n = s.q0[i + 1] - s.q0[i];
-        const int tiles = int(((long long)n * d.group + ROWS - 1) / ROWS);
-        unsigned sum = 0;
-        if (tiles <= 4)
-            for (int t = 0; t < tiles; ++t) sum += tile_units<ROWS, KEYS>(d, n, s.kv[i], t);
-        s.per_head[i] = sum;
-    }
+    long long tiles = 0;
+    for (int i = tid; i < d.n_seq; i += THREADS) tiles += s.per_head[i];
+    tiles *= d.n_head_kv;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, off);
+    if (lane == 0 && tiles) atomicAdd(reinterpret_cast<unsigned long long*>(&s.total), (unsigned long long)tiles);
     __syncthreads();
-    for (int i = warp; i < d.n_seq; i += THREADS / 32) {
-        const int n = s.q0[i + 1] - s.q0[i];
-        const int tiles = int(((long long)n * d.group + ROWS - 1) / ROWS);
-        if (tiles <= 4) continue;
-        unsigned sum = 0;
-        for (int t = lane; t < tiles; t += 32) sum += tile_units<ROWS, KEYS>(d, n, s.kv[i], t);
-        sum = __reduce_add_sync(0xffffffffu, sum);
-        if (lane == 0) s.per_head[i] = sum;
+    const bool whole = s.total >= whole_from;
+    if (!whole) {
+        // sequences of few row tiles a thread each, longer ones a warp each
+        for (int i = tid; i < d.n_seq; i += THREADS) {
+            const int n = s.q0[i + 1] - s.q0[i], tiles = int(s.per_head[i]);
+            if (tiles > 4) continue;
+            unsigned sum = 0;
+            for (int t = 0; t < tiles; ++t) sum += tile_units<ROWS, KEYS>(d, n, s.kv[i], t) + OVER;
+            s.per_head[i] = sum;
+        }
+        for (int i = warp; i < d.n_seq; i += THREADS / 32) {
+            const int n = s.q0[i + 1] - s.q0[i], tiles = row_tiles<ROWS>(d, n);
+            if (tiles <= 4) continue;
+            unsigned sum = 0;
+            for (int t = lane; t < tiles; t += 32) sum += tile_units<ROWS, KEYS>(d, n, s.kv[i], t) + OVER;
+            sum = __reduce_add_sync(0xffffffffu, sum);
+            if (lane == 0) s.per_head[i] = sum;
+        }
     }
     __syncthreads();
     if (warp == 0) {
@@ -151,49 +172,63 @@ __device__ void read_lengths(const Desc& d, Lengths& s) {
             if (i + lane < d.n_seq) s.first[i + lane] = at + v - own;
             at += __shfl_sync(0xffffffffu, v, 31);
         }
-        if (lane == 0) s.total = (long long)at;
+        if (lane == 0) s.total = (long long)at, s.whole = whole;
     }
     __syncthreads();
 }
 
 struct Item {
     int seq, head, tile;     // row tile of the sequence's head
-    int key_tile, count;     // its key tiles [key_tile, key_tile + count) are this CTA's
+    int n, kv;               // the sequence's new tokens and length
+    int key_tile, count;     // key tiles [key_tile, key_tile + count) of the row tile are this CTA's
     int units;               // key tiles of the whole row tile
-    long long tile_first;    // its first unit
+    long long tile_first;    // its first unit (cut)
 };
 
+// The CTA whose share of `parts` holds unit u: the largest c with
+// total * c / parts <= u.
+__device__ __forceinline__ int share_of(long long u, long long total, int parts) {
+    return int(((u + 1) * parts - 1) / total);
+}
+
 // One CTA's share as a list of items; the calls are warp-uniform.
-template <int ROWS, int KEYS>
+template <int ROWS, int KEYS, int OVER>
 struct Share {
-    long long at, end;
-    int seq, head, tile, key_tile, tiles, n, kv;
-    bool fresh;
+    long long at, end;       // units left (cut); the next row tile (whole)
+    int seq, head, tile, key_tile, tiles, n, kv, cta, parts, round;
 
     __device__ __forceinline__ void enter_seq(const Desc& d, const Lengths& s, int i) {
         seq = i;
         n = s.q0[i + 1] - s.q0[i];
         kv = s.kv[i];
-        tiles = int(((long long)n * d.group + ROWS - 1) / ROWS);
+        tiles = row_tiles<ROWS>(d, n);
+    }
+    // The last sequence whose first unit is at or before u.
+    __device__ __forceinline__ int seq_of(const Desc& d, const Lengths& s, long long u) const {
+        int lo = 0, hi = d.n_seq - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if ((long long)s.first[mid] <= u) lo = mid; else hi = mid - 1;
+        }
+        return lo;
     }
 
-    // cta's share of `parts` equal ones.
-    __device__ __forceinline__ void begin(const Desc& d, const Lengths& s, int cta, int parts) {
+    // cta's share of `parts`, at most one for each unit.
+    __device__ __forceinline__ void begin(const Desc& d, const Lengths& s, int c, int p) {
+        cta = c;
+        parts = p;
+        round = 0;
+        if (s.whole) return;
         at = s.total * cta / parts;
         end = s.total * (cta + 1) / parts;
         if (at >= end) return;
-        int lo = 0, hi = d.n_seq - 1;   // the last sequence whose first unit is at or before `at`, with units
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if ((long long)s.first[mid] <= at) lo = mid; else hi = mid - 1;
-        }
-        enter_seq(d, s, lo);
-        const unsigned long long in_seq = (unsigned long long)at - s.first[lo];
-        head = int(in_seq / s.per_head[lo]);
-        unsigned rest = unsigned(in_seq - (unsigned long long)head * s.per_head[lo]);
+        enter_seq(d, s, seq_of(d, s, at));
+        const unsigned long long in_seq = (unsigned long long)at - s.first[seq];
+        head = int(in_seq / s.per_head[seq]);
+        unsigned rest = unsigned(in_seq - (unsigned long long)head * s.per_head[seq]);
         const int lane = threadIdx.x & 31;
         for (int t0 = 0;; t0 += 32) {   // the row tile that holds unit `rest` of the head
-            const unsigned own = t0 + lane < tiles ? tile_units<ROWS, KEYS>(d, n, kv, t0 + lane) : 0;
+            const unsigned own = t0 + lane < tiles ? tile_units<ROWS, KEYS>(d, n, kv, t0 + lane) + OVER : 0;
             unsigned v = own;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
@@ -212,33 +247,45 @@ struct Share {
     }
 
     __device__ __forceinline__ bool next(const Desc& d, const Lengths& s, Item& it) {
-        if (at >= end) return false;
-        while (tile == tiles) {
-            tile = 0;
-            if (tiles == 0 || ++head == d.n_head_kv) {
-                head = 0;
-                enter_seq(d, s, seq + 1);
+        if (s.whole) {
+            const long long i = (long long)round * parts + (round & 1 ? parts - 1 - cta : cta);
+            ++round;
+            if (i >= s.total) return false;
+            enter_seq(d, s, seq_of(d, s, i));
+            const unsigned in_seq = unsigned((unsigned long long)i - s.first[seq]);
+            it.tile = tiles - 1 - int(in_seq / d.n_head_kv);
+            it.head = int(in_seq % d.n_head_kv);
+            it.key_tile = 0;
+            it.units = it.count = tile_units<ROWS, KEYS>(d, n, kv, it.tile);
+            it.tile_first = 0;
+        } else {
+            for (;;) {
+                if (at >= end) return false;
+                while (tile == tiles) {
+                    tile = 0;
+                    if (tiles == 0 || ++head == d.n_head_kv) {
+                        head = 0;
+                        enter_seq(d, s, seq + 1);
+                    }
+                }
+                it.tile = tile;
+                it.head = head;
+                it.units = tile_units<ROWS, KEYS>(d, n, kv, tile);
+                it.key_tile = key_tile;
+                it.tile_first = at - key_tile;
+                it.count = int(min((long long)(it.units - key_tile), end - at));
+                at += it.units - key_tile + OVER;
+                key_tile = 0;
+                ++tile;
+                if (it.count > 0) break;   // else the share began behind the tile's last key tile
             }
         }
         it.seq = seq;
-        it.head = head;
-        it.tile = tile;
-        it.units = tile_units<ROWS, KEYS>(d, n, kv, tile);
-        it.key_tile = key_tile;
-        it.count = int(min((long long)(it.units - key_tile), end - at));
-        it.tile_first = at - key_tile;
-        at += it.count;
-        key_tile = 0;
-        ++tile;
+        it.n = n;
+        it.kv = kv;
         return true;
     }
 };
-
-// The CTA whose share of `parts` holds unit u: the largest c with
-// total * c / parts <= u.
-__device__ __forceinline__ int share_of(long long u, long long total, int parts) {
-    return int(((u + 1) * parts - 1) / total);
-}
 
 }  // namespace paged
 }  // namespace p100b

@@ -164,6 +164,9 @@ CASES = [
     ([77], [513], 14, 2, 128, "f16", 9, "head"),            # pages of 9 tokens end inside every tile
     ([40, 200], [1000, 200], 8, 8, 128, "bf16", 8, "token"),
     ([700, 1, 1, 130], [900, 5, 2049, 4000], 16, 2, 64, "f16", 48, "head"),
+    ([17 + i for i in range(20)], [60 + 11 * i for i in range(20)], 40, 40, 64, "f16", 16, "head"),   # 800 row tiles
+    ([3000], [3500], 16, 16, 64, "bf16", 64, "token"),      # 192 row tiles of one sequence, several a CTA
+    ([600, 555], [600, 1200], 144, 48, 64, "f16", 32, "head"),   # 672 row tiles, three query heads of a group
 ]
 
 
@@ -188,6 +191,8 @@ def test_softcap_scale_and_fp32_output(cuda, q_lens, kv_lens, page, dtype):
     o, lse = attend(b, q, o_fp32=True, **kw)
     assert o.dtype == cuda.float32
     check(cuda, b, o, lse, attend64(b, q, **kw))
+    for kw in (dict(scale=-0.15), dict(scale=-0.15, softcap=20.0)):
+        check(cuda, b, *attend(b, q, **kw), attend64(b, q, **kw))
 
 
 @pytest.mark.parametrize("rows", [1, 130])
