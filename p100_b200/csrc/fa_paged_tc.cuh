@@ -46,22 +46,19 @@ using paged::Item;
 using paged::Lengths;
 
 constexpr int kRows = 256, kKeys = 128;
-constexpr int kOver = 2;                  // what a row tile costs beyond its keys, in units
+constexpr int kOver = 4;                  // what a row tile costs beyond its keys, in units
 constexpr int kWholeFrom = 4;             // row tiles per CTA from which they are dealt out whole
 constexpr int kThreads = 384;             // two softmax warpgroups; one of the two issuing warps and two idle ones
 constexpr int kMmaWarp = 8, kLoadWarp = 9;
-// Registers a thread after the split; 256 x 208 + 128 x 88 is what the block
+// Registers a thread after the split; 256 x 192 + 128 x 120 is what the block
 // is launched with (384 x 168).
-constexpr int kSoftmaxRegs = 208, kIssueRegs = 88;
+constexpr int kSoftmaxRegs = 192, kIssueRegs = 120;
 static_assert(256 * kSoftmaxRegs + 128 * kIssueRegs <= kThreads * 168, "register split");
 constexpr int kSub = 128 * 128;           // bytes of 128 rows x 64 values
-// Pairs of probabilities that exp2_poly computes, of every kPolyOf: it and the
-// special-function unit then take about the same time.
-constexpr int kPoly = 1, kPolyOf = 4;
 constexpr float kRise = 8.0f;             // log2 of the rise that forces a rescale
 
 template <int D>
-__host__ __device__ constexpr int slots() { return D == 128 ? 4 : 6; }
+__host__ __device__ constexpr int slots() { return D == 128 ? 4 : 8; }
 template <int D>
 __host__ __device__ constexpr int tile_bytes() { return kSub * (D / 64); }
 
@@ -88,7 +85,7 @@ struct Job {
 constexpr int kJobs = 4;
 
 struct Barriers {
-    uint64_t full[6], empty[6], q_full[2], s_full[2], p_full[2], joined[2], job_full[kJobs], job_empty[kJobs], drain;
+    uint64_t full[8], empty[8], q_full[2], s_full[2], p_full[2][2], joined[2], job_full[kJobs], job_empty[kJobs], drain;
     uint32_t tmem;
     int abort;
     int last[2];
@@ -116,21 +113,30 @@ __device__ __forceinline__ constexpr uint32_t idesc_f16(int n, bool b_n_major) {
     const uint32_t t = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     return (1u << 4) | (t << 7) | (t << 10) | (uint32_t(b_n_major) << 16) | (uint32_t(n >> 3) << 17) | ((128u >> 4) << 24);
 }
+// The products and commits are called by a whole warp and issued by the lane
+// that elect.sync picks (the same every time): with warp-uniform operands the
+// descriptors stay in uniform registers.  Issued under a branch on the lane
+// instead, every product waited for its operands' way there, 100 cycles each.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+        "{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
         : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+        "{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
         : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+    asm volatile(
+        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar))
+        : "memory");
 }
+// A value that every lane of the warp has, as one the compiler knows to be uniform.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -174,24 +180,24 @@ __device__ __forceinline__ void st8(uint32_t a, const uint32_t* r) {
                  : "memory");
 }
 
-// Waits for a barrier phase, for at most kWaitLimitNs or until the CTA aborts.
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, int* abort) {
-    if (mbar_try_wait(bar, parity)) return true;
+// Waits for a barrier phase, for at most kWaitLimitNs or until the CTA aborts;
+// a whole warp calls it and every lane gets the same answer.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* abort) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     const unsigned long long start = globaltimer_ns();
     for (;;) {
+#pragma unroll 1
         for (int i = 0; i < 32; ++i)
-            if (mbar_try_wait(bar, parity)) return true;
-        if (*reinterpret_cast<volatile int*>(abort)) return false;
-        if (globaltimer_ns() - start > kWaitLimitNs) {
-            atomicExch(&g_device_error, kDevErrTimeout);
-            atomicExch(abort, 1);
+            if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(abort) != 0)) return false;
+        if (__any_sync(0xffffffffu, globaltimer_ns() - start > kWaitLimitNs)) {
+            if ((threadIdx.x & 31) == 0) {
+                atomicExch(&g_device_error, kDevErrTimeout);
+                atomicExch(abort, 1);
+            }
             return false;
         }
     }
-}
-// The same for a whole warp: every lane gets the same answer.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* abort) {
-    return __all_sync(0xffffffffu, wait_bar(bar, parity, abort));
 }
 
 // ------------------------------------------------------------ pairs of floats
@@ -217,28 +223,6 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
-}
-
-// 2^x of two finite x <= 8 on the FMA pipe: x = n + f with |f| <= 1/2 (adding
-// 1.5 * 2^23 rounds to an integer), a polynomial of degree 4 for 2^f whose
-// coefficients were fitted to the least relative error (2.7e-6, mean 4e-8:
-// far below the rounding to 16 bits that follows, and without bias in the
-// sum), and n added to the exponent.
-__device__ __forceinline__ void exp2_poly(uint64_t x2, float& a, float& b) {
-    float x, y;
-    unpair(x2, x, y);
-    x2 = pair(fmaxf(x, -125.f), fmaxf(y, -125.f));
-    const uint64_t t = add2(x2, pair(12582912.f, 12582912.f));
-    const uint64_t f = fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), x2);
-    uint64_t r = fma2(f, pair(0.009570050984621048f, 0.009570050984621048f), pair(0.05591786280274391f, 0.05591786280274391f));
-    r = fma2(f, r, pair(0.2402474582195282f, 0.2402474582195282f));
-    r = fma2(f, r, pair(0.6931217908859253f, 0.6931217908859253f));
-    r = fma2(f, r, pair(0.9999992847442627f, 0.9999992847442627f));
-    float tx, ty;
-    unpair(t, tx, ty);
-    unpair(r, a, b);
-    a = __int_as_float(__float_as_int(a) + (__float_as_int(tx) << 23));
-    b = __int_as_float(__float_as_int(b) + (__float_as_int(ty) << 23));
 }
 
 // ------------------------------------------------------------ roles
@@ -330,7 +314,7 @@ __device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tm
         for (unsigned u = used > NS ? used - NS : 0; u < used; ++u) mbar_wait(&bars.full[u % NS], (u / NS) & 1);
 }
 
-// One lane issues the products; false when a wait was given up.
+// Issues the products; false when a wait was given up.
 template <typename T, int D>
 __device__ __forceinline__ bool mma_role(const Desc& d, float scale, Barriers& bars, uint32_t q_smem, uint32_t ring,
                                          uint32_t tmem) {
@@ -349,29 +333,27 @@ __device__ __forceinline__ bool mma_role(const Desc& d, float scale, Barriers& b
                    sw128_desc(ring + slot * tile_bytes<D>() + off, 16, 1024), idesc_s, k > 0);
         }
     };
-    auto pv = [&](int w, int slot, bool add) {   // O_w += P_w V
+    auto pv = [&](int w, int half, int slot, bool add) {   // O_w += P_w V over half of the keys
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
+        for (int k = half * (kKeys / 32); k < (half + 1) * (kKeys / 32); ++k)
             mma_ts(tmem + 256 + w * D, tmem + w * 128 + k * 8,
                    sw128_desc(ring + slot * tile_bytes<D>() + uint32_t(k) * 2048, kSub, 1024), kIdescO, add || k > 0);
     };
     for (unsigned j = 0;; ++j) {
         if (!warp_wait(&bars.job_full[j % kJobs], (j / kJobs) & 1, &bars.abort)) return false;
         const Job& job = bars.jobs[j % kJobs];
-        const int count = job.count;
+        const int count = int(uniform(job.count));
         if (count == 0) return true;
-        const int groups = job.n * d.group - job.row0 > 128 ? 2 : 1;
+        const int groups = int(uniform(job.n * d.group - job.row0 > 128 ? 2 : 1));
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.job_empty[j % kJobs]);
         if (!warp_wait(&bars.full[used % NS], (used / NS) & 1, &bars.abort)) return false;
         for (int w = 0; w < groups; ++w) {
             if (!warp_wait(&bars.q_full[w], items[w]++ & 1, &bars.abort)) return false;
             fence_after();
-            if (lane == 0) {
-                qk(w, used % NS);
-                mma_commit(&bars.s_full[w]);
-                if (w + 1 == groups) mma_commit(&bars.empty[used % NS]);
-            }
+            qk(w, used % NS);
+            mma_commit(&bars.s_full[w]);
+            if (w + 1 == groups) mma_commit(&bars.empty[used % NS]);
         }
         ++used;
         for (int t = 0; t < count; ++t) {
@@ -379,18 +361,19 @@ __device__ __forceinline__ bool mma_role(const Desc& d, float scale, Barriers& b
             const bool more = t + 1 < count;
             if (!warp_wait(&bars.full[v % NS], (v / NS) & 1, &bars.abort)) return false;
             for (int w = 0; w < groups; ++w) {
-                if (!warp_wait(&bars.p_full[w], tiles[w]++ & 1, &bars.abort)) return false;
-                if (more && w == 0 && !warp_wait(&bars.full[k % NS], (k / NS) & 1, &bars.abort)) return false;
+                if (!warp_wait(&bars.p_full[w][0], tiles[w] & 1, &bars.abort)) return false;
                 fence_after();
-                if (lane == 0) {
-                    pv(w, v % NS, t > 0);
-                    if (w + 1 == groups) mma_commit(&bars.empty[v % NS]);
-                    if (more) {
-                        qk(w, k % NS);
-                        if (w + 1 == groups) mma_commit(&bars.empty[k % NS]);
-                    }
-                    mma_commit(&bars.s_full[w]);
+                pv(w, 0, v % NS, t > 0);
+                if (more && w == 0 && !warp_wait(&bars.full[k % NS], (k / NS) & 1, &bars.abort)) return false;
+                if (!warp_wait(&bars.p_full[w][1], tiles[w]++ & 1, &bars.abort)) return false;
+                fence_after();
+                pv(w, 1, v % NS, true);
+                if (w + 1 == groups) mma_commit(&bars.empty[v % NS]);
+                if (more) {
+                    qk(w, k % NS);
+                    if (w + 1 == groups) mma_commit(&bars.empty[k % NS]);
                 }
+                mma_commit(&bars.s_full[w]);
             }
             used += more ? 2 : 1;
         }
@@ -477,8 +460,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
 #pragma unroll
                 for (int i = 0; i < 128; ++i) s[i] = fap::cap_score(s[i], cap_in, cap);
             }
-            const bool masked = __any_sync(0xffffffffu, limit < key0 + kKeys);
-            if (masked) {
+            if (__any_sync(0xffffffffu, limit < key0 + kKeys)) {
                 const int lim = limit - key0;
 #pragma unroll
                 for (int i = 0; i < 128; ++i) s[i] = i < lim ? s[i] : -INFINITY;
@@ -510,12 +492,24 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
                     }
                 }
             }
+            if (w == 0 && key0 + kKeys > job.end) {   // rows of V that no key of the item's rows reaches
+                const unsigned u = 2 * (used + t) + 1;
+                if (!warp_wait(&bars.full[u % NS], (u / NS) & 1, &bars.abort)) return;
+                if (key0 + row >= job.end) {
+                    uint8_t* v = ring + (u % NS) * tile_bytes<D>() + row * 128;
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i)
+                        *reinterpret_cast<uint4*>(v + (i >> 3) * kSub + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_async();
+            }
             const float base = m == -INFINITY ? 0.f : m * c;
             const uint64_t c2 = pair(c, c), b2 = pair(-base, -base);
             uint64_t sum[2] = {0, 0};
-            if (masked) {   // exp2 of -inf must be 0: the special-function unit alone
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+            for (int half = 0; half < 2; ++half) {   // the products with the first half start while the second is computed
+#pragma unroll
+                for (int i = 4 * half; i < 4 * half + 4; ++i) {
                     uint32_t pk[8];
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
@@ -528,46 +522,15 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
                     }
                     st8(t_s + i * 8, pk);
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    uint32_t pk[8];
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        float a, b;
-                        const uint64_t x = fma2(pair(s[i * 16 + e], s[i * 16 + e + 1]), c2, b2);
-                        if (!CAP && (e >> 1) % kPolyOf < kPoly) {
-                            exp2_poly(x, a, b);
-                        } else {
-                            unpair(x, a, b);
-                            a = paged::exp2_approx(a);
-                            b = paged::exp2_approx(b);
-                        }
-                        sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair(a, b));
-                        pk[e >> 1] = paged::pack2<T>(a, b);
-                    }
-                    st8(t_s + i * 8, pk);
-                }
+                wait_st();
+                fence_before();
+                mbar_arrive(&bars.p_full[w][half]);
             }
             {
                 float a, b;
                 unpair(add2(sum[0], sum[1]), a, b);
                 l += a + b;
             }
-            if (w == 0 && key0 + kKeys > job.end) {   // rows of V that no key of the item's rows reaches
-                const unsigned u = 2 * (used + t) + 1;
-                if (!warp_wait(&bars.full[u % NS], (u / NS) & 1, &bars.abort)) return;
-                if (key0 + row >= job.end) {
-                    uint8_t* v = ring + (u % NS) * tile_bytes<D>() + row * 128;
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i)
-                        *reinterpret_cast<uint4*>(v + (i >> 3) * kSub + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-                }
-                fence_async();
-            }
-            wait_st();
-            fence_before();
-            mbar_arrive(&bars.p_full[w]);
         }
         used += count;
         if (!warp_wait(&bars.s_full[w], done++ & 1, &bars.abort)) return;   // the accumulator is complete
@@ -693,14 +656,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int parts = len.ok ? int(min((long long)gridDim.x, len.total)) : 0;
     if (int(blockIdx.x) >= parts) return;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 6; ++i) {
+        for (int i = 0; i < 8; ++i) {
             mbar_init(&bars.full[i], 1);
             mbar_init(&bars.empty[i], 1);
         }
         for (int w = 0; w < 2; ++w) {
             mbar_init(&bars.q_full[w], 128);
             mbar_init(&bars.s_full[w], 1);
-            mbar_init(&bars.p_full[w], 128);
+            mbar_init(&bars.p_full[w][0], 128);
+            mbar_init(&bars.p_full[w][1], 128);
             mbar_init(&bars.joined[w], 128);
         }
         for (int i = 0; i < kJobs; ++i) {
@@ -731,9 +695,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             share.begin(p.d, len, blockIdx.x, parts);
             load_role<D>(p, &tmk, &tmv, len, bars, ring, share);
         } else if (warp == kMmaWarp) {
-            if (!mma_role<T, D>(p.d, p.scale, bars, smem_addr(q_smem), smem_addr(ring), tmem)) {
+            if (!mma_role<T, D>(p.d, p.scale, bars, uniform(smem_addr(q_smem)), uniform(smem_addr(ring)),
+                                uniform(tmem))) {
                 // leave only when the products in flight are done
-                if ((threadIdx.x & 31) == 0) mma_commit(&bars.drain);
+                mma_commit(&bars.drain);
                 __syncwarp();
                 mbar_wait(&bars.drain, 0);
             }
