@@ -17,7 +17,9 @@
 //
 // HBM bytes bound it: K and V are read once per row tile.  A row tile cut by
 // the shares leaves its partials {m, l, unnormalised o} in the workspace and
-// its last CTA (an atomic ticket, no waiting) joins them in share order.
+// its last CTA (an atomic ticket, no waiting) joins them in share order; more
+// than kDirect parts are joined in groups first, each by its last CTA, so that
+// no CTA reads more than about the square root of their number.
 #pragma once
 #include <climits>
 
@@ -35,6 +37,9 @@ constexpr int kRows = 16, kKeys = 64;
 constexpr int kOver = 1;   // what a row tile costs beyond its keys, in units
 constexpr int kStages = 3;
 constexpr int kOffs = 5;   // tiles whose row offsets are held
+constexpr int kDirect = 16;   // parts that one CTA joins
+constexpr int kMaxJoin = 32;  // at most so many in one join (kDirect, or the square root of the CTAs)
+constexpr int kMinUnits = 2;  // of a share, where there is less work than CTAs
 
 struct Params {
     Desc d;
@@ -44,13 +49,14 @@ struct Params {
     float* lse;        // [n_tokens][n_head_q] or null
     float* ws_o;       // [CTAs][2][kRows][D]
     float* ws_ml;      // [CTAs][2][kRows][2], m in units of log2
-    unsigned* tickets; // [CTAs]
+    unsigned* tickets; // [2][CTAs]
     float scale, softcap;
 };
 
+// Without the lengths, which lie behind.
 template <int D>
 constexpr size_t smem_bytes() {
-    return sizeof(Lengths) + size_t(kStages) * 2 * kKeys * D * 2 + kOffs * kKeys * sizeof(long long) + 128;
+    return size_t(kStages) * 2 * kKeys * D * 2 + kOffs * kKeys * sizeof(long long);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -97,12 +103,75 @@ __device__ __forceinline__ long long row_offset(const Desc& d, int q0, int head,
     return (long long)(q0 + tok) * stride + (long long)(head * d.group + g) * D;
 }
 
-template <typename T>
-__device__ __forceinline__ void store_out2(void* o, int o_f32, long long at, float a, float b) {
-    if (o_f32)
-        *reinterpret_cast<float2*>(static_cast<float*>(o) + at) = make_float2(a, b);
-    else
-        *reinterpret_cast<uint32_t*>(static_cast<T*>(o) + at) = paged::pack2<T>(a, b);
+// Where a finished row goes.
+struct Out {
+    int q0, head, row0, rows;
+    template <typename T, int D>
+    __device__ __forceinline__ void write4(const Params& p, int r, int c, float4 o, float sum) const {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const long long at = row_offset(p.d, q0, head, row0 + r, p.d.o_stride, D) + c;
+        if (p.o_f32)
+            *reinterpret_cast<float4*>(static_cast<float*>(p.o) + at) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        else
+            *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + at) =
+                make_uint2(paged::pack2<T>(o.x * inv, o.y * inv), paged::pack2<T>(o.z * inv, o.w * inv));
+    }
+    __device__ __forceinline__ void write_lse(const Params& p, int r, float m, float sum) const {
+        if (!p.lse) return;
+        const int tok = (row0 + r) / p.d.group;
+        p.lse[(long long)(q0 + tok) * p.d.n_head_q + head * p.d.group + (row0 + r - tok * p.d.group)] =
+            sum == 0.f ? -INFINITY : (m + log2f(sum)) / 1.4426950408889634f;
+    }
+};
+
+// Joins the partials of parts first, first + step, ... (n of them) of the row
+// tile whose part 0 belongs to CTA c0, in that order: into the output, or back
+// into the first one's place.  Every thread of the CTA calls it; scratch:
+// (2 n + 2) x kRows floats.
+template <typename T, int D>
+__device__ void join_parts(const Params& p, const Out& out, int c0, int first, int step, int n, bool final, float* scratch) {
+    const int tid = threadIdx.x;
+    float* s_w = scratch;                    // [n][kRows] m, then the weight
+    float* s_l = s_w + n * kRows;            // [n][kRows]
+    float* s_top = s_l + n * kRows;          // [kRows]
+    float* s_sum = s_top + kRows;            // [kRows]
+    auto slot = [&](int i) { return 2LL * (c0 + i) + (i == 0); };
+    for (int i = tid; i < n * kRows; i += kThreads) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + slot(first + i / kRows * step) * kRows + i % kRows);
+        s_w[i] = ml.x;
+        s_l[i] = ml.y;
+    }
+    __syncthreads();
+    if (tid < kRows) {
+        float top = -INFINITY, sum = 0.f;
+        for (int i = 0; i < n; ++i) top = fmaxf(top, s_w[i * kRows + tid]);
+        const float base = top == -INFINITY ? 0.f : top;
+        for (int i = 0; i < n; ++i) {
+            const float w = paged::exp2_approx(s_w[i * kRows + tid] - base);
+            s_w[i * kRows + tid] = w;
+            sum = fmaf(w, s_l[i * kRows + tid], sum);
+        }
+        s_top[tid] = top;
+        s_sum[tid] = sum;
+        if (final && tid < out.rows) out.write_lse(p, tid, top, sum);
+        if (!final) reinterpret_cast<float2*>(p.ws_ml)[slot(first) * kRows + tid] = make_float2(top, sum);
+    }
+    __syncthreads();
+    for (int e = tid; e < out.rows * (D / 4); e += kThreads) {
+        const int r = e / (D / 4), c = (e - r * (D / 4)) * 4;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            const float4 o = __ldcg(reinterpret_cast<const float4*>(p.ws_o + (slot(first + i * step) * kRows + r) * D + c));
+            const float w = s_w[i * kRows + r];
+            a.x = fmaf(w, o.x, a.x);
+            a.y = fmaf(w, o.y, a.y);
+            a.z = fmaf(w, o.z, a.z);
+            a.w = fmaf(w, o.w, a.w);
+        }
+        if (final) out.write4<T, D>(p, r, c, a, s_sum[r]);
+        else *reinterpret_cast<float4*>(p.ws_o + (slot(first) * kRows + r) * D + c) = a;
+    }
 }
 
 template <typename T, int D>
@@ -112,18 +181,18 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_kernel(const Params p) {
     constexpr int kTileBytes = kKeys * kRowBytes;
     constexpr int kChunks = D / 8;            // 16-byte chunks of a row
     constexpr float kLog2e = 1.4426950408889634f;
-    Lengths& len = *reinterpret_cast<Lengths*>(smem);
-    long long* s_off = reinterpret_cast<long long*>(smem + ((sizeof(Lengths) + 15) & ~size_t(15)));   // [kOffs][kKeys]
-    uint8_t* s_kv = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_off + kOffs * kKeys) + 127) & ~uintptr_t(127));
+    uint8_t* s_kv = smem;
+    long long* s_off = reinterpret_cast<long long*>(s_kv + size_t(kStages) * 2 * kTileBytes);   // [kOffs][kKeys]
+    const Lengths len(s_off + kOffs * kKeys, p.d.n_seq);
     __shared__ int s_last;
     const Desc& d = p.d;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     paged::read_lengths<kRows, kKeys, kOver, kThreads>(d, len, LLONG_MAX);
-    if (!len.ok) return;
-    // at least one unit a share: every CTA between a cut tile's first and last
-    // then holds a part of it
-    const int parts = int(min((long long)gridDim.x, len.total));
+    if (!len.head->ok) return;
+    // every share has a unit, so every CTA between a cut tile's first and last
+    // holds a part of it
+    const int parts = int(min((long long)gridDim.x, (len.head->total + kMinUnits - 1) / kMinUnits));
     if (int(blockIdx.x) >= parts) return;
     paged::Share<kRows, kKeys, kOver> share;
     share.begin(d, len, blockIdx.x, parts);
@@ -300,68 +369,64 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_kernel(const Params p) {
                     make_float2(acc[i][2 * h], acc[i][2 * h + 1]);
         __syncthreads();
         const bool whole = it.count == it.units;
+        const Out out = {q0, it.head, row0, rows};
         const int slot = blockIdx.x * 2 + (it.key_tile == 0);   // 0: a tile begun by another CTA, 1: begun here
-        for (int e = tid; e < rows * (D / 2); e += kThreads) {
-            const int r = e / (D / 2), c = (e - r * (D / 2)) * 2;
+        for (int e = tid; e < rows * (D / 4); e += kThreads) {
+            const int r = e / (D / 4), c = (e - r * (D / 4)) * 4;
             float mx = s_m[r];
 #pragma unroll
             for (int w = 1; w < 4; ++w) mx = fmaxf(mx, s_m[w * kRows + r]);
             const float base = mx == -INFINITY ? 0.f : mx;
-            float a = 0.f, b = 0.f, sum = 0.f;
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            float sum = 0.f;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 const float f = paged::exp2_approx(s_m[w * kRows + r] - base);
-                const float2 o = *reinterpret_cast<const float2*>(s_o + (w * kRows + r) * kLd + c);
-                a = fmaf(f, o.x, a);
-                b = fmaf(f, o.y, b);
+                const float4 o = *reinterpret_cast<const float4*>(s_o + (w * kRows + r) * kLd + c);
+                a.x = fmaf(f, o.x, a.x);
+                a.y = fmaf(f, o.y, a.y);
+                a.z = fmaf(f, o.z, a.z);
+                a.w = fmaf(f, o.w, a.w);
                 sum = fmaf(f, s_l[w * kRows + r], sum);
             }
             if (whole) {
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                const int tok = (row0 + r) / d.group;
-                store_out2<T>(p.o, p.o_f32, row_offset(d, q0, it.head, row0 + r, d.o_stride, D) + c, a * inv, b * inv);
-                if (p.lse && c == 0)
-                    p.lse[(long long)(q0 + tok) * d.n_head_q + it.head * d.group + (row0 + r - tok * d.group)] =
-                        sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
+                out.write4<T, D>(p, r, c, a, sum);
+                if (c == 0) out.write_lse(p, r, mx, sum);
             } else {
-                *reinterpret_cast<float2*>(p.ws_o + ((long long)slot * kRows + r) * D + c) = make_float2(a, b);
+                *reinterpret_cast<float4*>(p.ws_o + ((long long)slot * kRows + r) * D + c) = a;
                 if (c == 0)
                     *reinterpret_cast<float2*>(p.ws_ml + ((long long)slot * kRows + r) * 2) = make_float2(mx, sum);
             }
         }
         if (!whole) {
-            const int c0 = paged::share_of(it.tile_first, len.total, parts);
-            const int c1 = paged::share_of(it.tile_first + it.units - 1, len.total, parts);
+            const int c0 = paged::share_of(it.tile_first, len.head->total, parts);
+            const int np = paged::share_of(it.tile_first + it.units - 1, len.head->total, parts) - c0 + 1;
+            int per = np;   // parts of a group
+            if (np > kDirect) {
+                per = int(ceilf(sqrtf(float(np))));
+                per = min(per, kMaxJoin);
+            }
+            const int groups = (np + per - 1) / per;
+            const int group = (int(blockIdx.x) - c0) / per, first = group * per;
+            const int n = min(per, np - first);
             __threadfence();
             __syncthreads();
-            if (tid == 0) s_last = atomicAdd(p.tickets + c0, 1u) == unsigned(c1 - c0);
+            if (tid == 0) s_last = atomicAdd(p.tickets + c0 + first, 1u) == unsigned(n - 1);
             __syncthreads();
             if (s_last) {
                 __threadfence();
-                if (tid == 0) p.tickets[c0] = 0;   // ready for the next call
-                for (int e = tid; e < rows * (D / 2); e += kThreads) {
-                    const int r = e / (D / 2), c = (e - r * (D / 2)) * 2;
-                    float mx = -INFINITY;
-                    for (int q = c0; q <= c1; ++q)
-                        mx = fmaxf(mx, __ldcg(p.ws_ml + ((long long)(2 * q + (q == c0)) * kRows + r) * 2));
-                    const float base = mx == -INFINITY ? 0.f : mx;
-                    float a = 0.f, b = 0.f, sum = 0.f;
-#pragma unroll 4
-                    for (int q = c0; q <= c1; ++q) {
-                        const long long at = (long long)(2 * q + (q == c0)) * kRows + r;
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + at * 2));
-                        const float2 o = __ldcg(reinterpret_cast<const float2*>(p.ws_o + at * D + c));
-                        const float f = paged::exp2_approx(ml.x - base);
-                        a = fmaf(f, o.x, a);
-                        b = fmaf(f, o.y, b);
-                        sum = fmaf(f, ml.y, sum);
+                if (tid == 0) p.tickets[c0 + first] = 0;   // ready for the next call
+                join_parts<T, D>(p, out, c0, first, 1, n, groups == 1, reinterpret_cast<float*>(s_kv));
+                if (groups > 1) {
+                    __threadfence();
+                    __syncthreads();
+                    if (tid == 0) s_last = atomicAdd(p.tickets + gridDim.x + c0, 1u) == unsigned(groups - 1);
+                    __syncthreads();
+                    if (s_last) {
+                        __threadfence();
+                        if (tid == 0) p.tickets[gridDim.x + c0] = 0;
+                        join_parts<T, D>(p, out, c0, 0, per, groups, true, reinterpret_cast<float*>(s_kv));
                     }
-                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                    const int tok = (row0 + r) / d.group;
-                    store_out2<T>(p.o, p.o_f32, row_offset(d, q0, it.head, row0 + r, d.o_stride, D) + c, a * inv, b * inv);
-                    if (p.lse && c == 0)
-                        p.lse[(long long)(q0 + tok) * d.n_head_q + it.head * d.group + (row0 + r - tok * d.group)] =
-                            sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
                 }
             }
         }

@@ -93,9 +93,10 @@ struct Barriers {
 };
 using Units = paged::Share<kRows, kKeys, kOver>;
 
+// Without the lengths.
 template <int D>
 constexpr size_t smem_bytes() {
-    return 1024 + 2 * tile_bytes<D>() + slots<D>() * tile_bytes<D>() + sizeof(Lengths) + sizeof(Barriers) + 64;
+    return 1024 + 2 * tile_bytes<D>() + slots<D>() * tile_bytes<D>() + sizeof(Barriers) + 64;
 }
 
 // ------------------------------------------------------------ tcgen05
@@ -229,7 +230,7 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 // Hands out the CTA's items and brings their K and V tiles into the ring, in
 // the order the products take them.
 template <int D>
-__device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tmk, const CUtensorMap* tmv, Lengths& len,
+__device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tmk, const CUtensorMap* tmv, const Lengths& len,
                                           Barriers& bars, uint8_t* ring, Units share) {
     constexpr int NS = slots<D>();
     const Desc& d = p.d;
@@ -260,8 +261,8 @@ __device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tm
                 job.head = it.head;
                 job.whole = it.count == it.units;
                 if (!job.whole) {
-                    job.c0 = paged::share_of(it.tile_first, len.total, share.parts);
-                    job.c1 = paged::share_of(it.tile_first + it.units - 1, len.total, share.parts);
+                    job.c0 = paged::share_of(it.tile_first, len.head->total, share.parts);
+                    job.c1 = paged::share_of(it.tile_first + it.units - 1, len.head->total, share.parts);
                 }
             }
             mbar_arrive(&bars.job_full[j % kJobs]);
@@ -643,9 +644,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* q_smem = smem;
     uint8_t* ring = q_smem + 2 * tile_bytes<D>();
-    Lengths& len = *reinterpret_cast<Lengths*>(ring + slots<D>() * tile_bytes<D>());
-    Barriers& bars = *reinterpret_cast<Barriers*>(
-        (reinterpret_cast<uintptr_t>(&len) + sizeof(Lengths) + 15) & ~uintptr_t(15));
+    Barriers& bars = *reinterpret_cast<Barriers*>(ring + slots<D>() * tile_bytes<D>());
+    const Lengths len(reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(&bars + 1) + 15) & ~uintptr_t(15)), p.d.n_seq);
     const int warp = threadIdx.x >> 5;
 
     if (threadIdx.x == kLoadWarp * 32) {
@@ -653,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         prefetch_tensormap(&tmv);
     }
     paged::read_lengths<kRows, kKeys, kOver, kThreads>(p.d, len, (long long)kWholeFrom * gridDim.x);
-    const int parts = len.ok ? int(min((long long)gridDim.x, len.total)) : 0;
+    const int parts = len.head->ok ? int(min((long long)gridDim.x, len.head->total)) : 0;
     if (int(blockIdx.x) >= parts) return;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 8; ++i) {

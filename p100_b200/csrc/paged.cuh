@@ -82,14 +82,28 @@ __device__ __forceinline__ void flag_input() { atomicExch(&g_device_error, kDevE
 // per CTA they are dealt out uncut, the ones with the most keys of a sequence
 // first and back and forth over the CTAs, so that neighbours in time read the
 // same keys and nothing is joined.
-struct Lengths {
-    long long total;                 // units (cut) or row tiles (whole) of the call
-    int ok;                          // the lengths are usable
-    int whole;
-    int q0[kMaxSeq + 1];
-    int kv[kMaxSeq];
-    unsigned per_head[kMaxSeq];      // units or row tiles of one kv head
-    unsigned long long first[kMaxSeq];   // units or row tiles before the sequence
+struct Lengths {                     // in shared memory, the arrays sized by n_seq
+    struct Head {
+        long long total;             // units (cut) or row tiles (whole) of the call
+        int ok;                      // the lengths are usable
+        int whole;
+    };
+    Head* head;
+    unsigned long long* first;       // [n_seq] units or row tiles before the sequence
+    int* q0;                         // [n_seq + 1]
+    int* kv;                         // [n_seq]
+    unsigned* per_head;              // [n_seq] units or row tiles of one kv head
+
+    __device__ Lengths(void* at, int n_seq) {   // 16-byte aligned
+        head = static_cast<Head*>(at);
+        first = reinterpret_cast<unsigned long long*>(head + 1);
+        q0 = reinterpret_cast<int*>(first + n_seq);
+        kv = q0 + n_seq + 1;
+        per_head = reinterpret_cast<unsigned*>(kv + n_seq);
+    }
+    __host__ __device__ static size_t bytes(int n_seq) {
+        return (sizeof(Head) + size_t(n_seq) * (8 + 3 * 4) + 4 + 127) / 128 * 128;
+    }
 };
 
 template <int ROWS>
@@ -113,9 +127,9 @@ __device__ __forceinline__ int tile_units(const Desc& d, int n, int kv, int tile
 // flag and make the call do nothing.  Row tiles are dealt out whole from
 // whole_from of them on.
 template <int ROWS, int KEYS, int OVER, int THREADS>
-__device__ void read_lengths(const Desc& d, Lengths& s, long long whole_from) {
+__device__ void read_lengths(const Desc& d, const Lengths& s, long long whole_from) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (tid == 0) s.ok = 1, s.total = 0;
+    if (tid == 0) s.head->ok = 1, s.head->total = 0;
     for (int i = tid; i <= d.n_seq; i += THREADS) s.q0[i] = d.q_start[i];
     for (int i = tid; i < d.n_seq; i += THREADS) s.kv[i] = d.kv_len[i];
     __syncthreads();
@@ -123,12 +137,12 @@ __device__ void read_lengths(const Desc& d, Lengths& s, long long whole_from) {
         const int n = s.q0[i + 1] - s.q0[i];
         if (s.q0[i] < 0 || n < 0 || n > d.max_q || s.q0[i + 1] > d.n_tokens || s.kv[i] < 0 ||
             (long long)s.kv[i] > (long long)d.max_pages * d.page_size)
-            s.ok = 0;
+            s.head->ok = 0;
         else
             s.per_head[i] = row_tiles<ROWS>(d, n);
     }
     __syncthreads();
-    if (!s.ok) {
+    if (!s.head->ok) {
         if (tid == 0) flag_input();
         return;
     }
@@ -137,9 +151,9 @@ __device__ void read_lengths(const Desc& d, Lengths& s, long long whole_from) {
     tiles *= d.n_head_kv;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, off);
-    if (lane == 0 && tiles) atomicAdd(reinterpret_cast<unsigned long long*>(&s.total), (unsigned long long)tiles);
+    if (lane == 0 && tiles) atomicAdd(reinterpret_cast<unsigned long long*>(&s.head->total), (unsigned long long)tiles);
     __syncthreads();
-    const bool whole = s.total >= whole_from;
+    const bool whole = s.head->total >= whole_from;
     if (!whole) {
         // sequences of few row tiles a thread each, longer ones a warp each
         for (int i = tid; i < d.n_seq; i += THREADS) {
@@ -172,7 +186,7 @@ __device__ void read_lengths(const Desc& d, Lengths& s, long long whole_from) {
             if (i + lane < d.n_seq) s.first[i + lane] = at + v - own;
             at += __shfl_sync(0xffffffffu, v, 31);
         }
-        if (lane == 0) s.total = (long long)at, s.whole = whole;
+        if (lane == 0) s.head->total = (long long)at, s.head->whole = whole;
     }
     __syncthreads();
 }
@@ -218,9 +232,9 @@ struct Share {
         cta = c;
         parts = p;
         round = 0;
-        if (s.whole) return;
-        at = s.total * cta / parts;
-        end = s.total * (cta + 1) / parts;
+        if (s.head->whole) return;
+        at = s.head->total * cta / parts;
+        end = s.head->total * (cta + 1) / parts;
         if (at >= end) return;
         enter_seq(d, s, seq_of(d, s, at));
         const unsigned long long in_seq = (unsigned long long)at - s.first[seq];
@@ -247,10 +261,10 @@ struct Share {
     }
 
     __device__ __forceinline__ bool next(const Desc& d, const Lengths& s, Item& it) {
-        if (s.whole) {
+        if (s.head->whole) {
             const long long i = (long long)round * parts + (round & 1 ? parts - 1 - cta : cta);
             ++round;
-            if (i >= s.total) return false;
+            if (i >= s.head->total) return false;
             enter_seq(d, s, seq_of(d, s, i));
             const unsigned in_seq = unsigned((unsigned long long)i - s.first[seq]);
             it.tile = tiles - 1 - int(in_seq / d.n_head_kv);

@@ -88,6 +88,7 @@ const char* paged_reason(const p100_paged_desc& in, paged::Desc& d) {
 
 // CTAs of the mma.sync kernel: two on every SM.
 constexpr int kMmaCtas = 2;
+static_assert(paged::kMaxSeq == P100_PAGED_MAX_SEQ, "lengths in shared memory");
 
 // The tensor-core kernel takes calls in which a sequence may have more rows
 // (new tokens x query heads per kv head) than the mma.sync kernel's row tile,
@@ -100,7 +101,7 @@ bool fa_paged_on_tc(const paged::Desc& d) {
 struct FaPagedWs {
     size_t tickets, o, ml, total;
 };
-size_t fa_paged_ticket_bytes(int sms) { return round256(size_t(sms) * kMmaCtas * sizeof(unsigned)); }
+size_t fa_paged_ticket_bytes(int sms) { return round256(size_t(sms) * kMmaCtas * 2 * sizeof(unsigned)); }
 FaPagedWs fa_paged_ws(const p100_paged_desc& in, int sms) {
     const size_t rows = size_t(sms) * 2 * std::max(kMmaCtas * fap::kRows, fatc::kRows);
     FaPagedWs w;
@@ -145,8 +146,11 @@ p100_status launch_fa_paged_tc(const fatc::Params& prm, const CUtensorMap& tmk, 
                                cudaStream_t stream) {
     static thread_local int configured[64] = {};
     auto kern = fatc::fa_paged_tc_kernel<T, D, CAP>;
-    if (p100_status st = allow_smem(kern, fatc::smem_bytes<D>(), configured, "cudaFuncSetAttribute(fa_paged_tc)")) return st;
-    kern<<<sms, fatc::kThreads, fatc::smem_bytes<D>(), stream>>>(prm, tmk, tmv);
+    constexpr size_t fixed = fatc::smem_bytes<D>();
+    if (p100_status st = allow_smem(kern, fixed + paged::Lengths::bytes(paged::kMaxSeq), configured,
+                                    "cudaFuncSetAttribute(fa_paged_tc)"))
+        return st;
+    kern<<<sms, fatc::kThreads, fixed + paged::Lengths::bytes(prm.d.n_seq), stream>>>(prm, tmk, tmv);
     return cuda_status(cudaGetLastError(), "fa_paged_tc_kernel launch");
 }
 template <typename T>
@@ -164,8 +168,11 @@ template <typename T, int D>
 p100_status launch_fa_paged_mma(const fap::Params& prm, int sms, cudaStream_t stream) {
     static thread_local int configured[64] = {};
     auto kern = fap::fa_paged_kernel<T, D>;
-    if (p100_status st = allow_smem(kern, fap::smem_bytes<D>(), configured, "cudaFuncSetAttribute(fa_paged)")) return st;
-    kern<<<sms * kMmaCtas, fap::kThreads, fap::smem_bytes<D>(), stream>>>(prm);
+    constexpr size_t fixed = fap::smem_bytes<D>();
+    if (p100_status st = allow_smem(kern, fixed + paged::Lengths::bytes(paged::kMaxSeq), configured,
+                                    "cudaFuncSetAttribute(fa_paged)"))
+        return st;
+    kern<<<sms * kMmaCtas, fap::kThreads, fixed + paged::Lengths::bytes(prm.d.n_seq), stream>>>(prm);
     return cuda_status(cudaGetLastError(), "fa_paged_kernel launch");
 }
 
