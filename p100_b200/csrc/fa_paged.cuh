@@ -21,8 +21,6 @@
 // than kDirect parts are joined in groups first, each by its last CTA, so that
 // no CTA reads more than about the square root of their number.
 #pragma once
-#include <climits>
-
 #include "paged.cuh"
 
 namespace p100b {
@@ -37,8 +35,8 @@ constexpr int kRows = 16, kKeys = 64;
 constexpr int kOver = 1;   // what a row tile costs beyond its keys, in units
 constexpr int kStages = 3;
 constexpr int kOffs = 5;   // tiles whose row offsets are held
-constexpr int kDirect = 16;   // parts that one CTA joins
-constexpr int kMaxJoin = 32;  // at most so many in one join (kDirect, or the square root of the CTAs)
+constexpr int kDirect = 48;   // parts that one CTA joins (two levels cost 2.4 us more than one of 37 parts)
+constexpr int kMaxJoin = 48;  // at most so many in one join
 constexpr int kMinUnits = 2;  // of a share, where there is less work than CTAs
 
 struct Params {
@@ -124,45 +122,57 @@ struct Out {
     }
 };
 
-// Joins the partials of parts first, first + step, ... (n of them) of the row
-// tile whose part 0 belongs to CTA c0, in that order: into the output, or back
-// into the first one's place.  Every thread of the CTA calls it; scratch:
-// (2 n + 2) x kRows floats.
+// Joins the partials of parts first, first + step, ... (n <= kMaxJoin of them)
+// of the row tile whose part 0 belongs to CTA c0, in that order: into the
+// output, or back into the first one's place.  Every thread of the CTA calls
+// it; scratch: (2 kMaxJoin + 1) x kRows floats.  Its loops stay rolled up to
+// a few loads in flight: it runs once a CTA, and straight-line code costs more
+// to fetch than it saves.
 template <typename T, int D>
-__device__ void join_parts(const Params& p, const Out& out, int c0, int first, int step, int n, bool final, float* scratch) {
+__device__ __forceinline__ void join_parts(const Params& p, const Out& out, int c0, int first, int step, int n, bool final,
+                                           float* scratch) {
+    constexpr int kLanes = kThreads / kRows;   // threads of a row's statistics
     const int tid = threadIdx.x;
-    float* s_w = scratch;                    // [n][kRows] m, then the weight
-    float* s_l = s_w + n * kRows;            // [n][kRows]
-    float* s_top = s_l + n * kRows;          // [kRows]
-    float* s_sum = s_top + kRows;            // [kRows]
-    auto slot = [&](int i) { return 2LL * (c0 + i) + (i == 0); };
-    for (int i = tid; i < n * kRows; i += kThreads) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + slot(first + i / kRows * step) * kRows + i % kRows);
-        s_w[i] = ml.x;
-        s_l[i] = ml.y;
-    }
-    __syncthreads();
-    if (tid < kRows) {
-        float top = -INFINITY, sum = 0.f;
-        for (int i = 0; i < n; ++i) top = fmaxf(top, s_w[i * kRows + tid]);
-        const float base = top == -INFINITY ? 0.f : top;
-        for (int i = 0; i < n; ++i) {
-            const float w = paged::exp2_approx(s_w[i * kRows + tid] - base);
-            s_w[i * kRows + tid] = w;
-            sum = fmaf(w, s_l[i * kRows + tid], sum);
+    float* s_w = scratch;                      // [n][kRows] m, then the weight
+    float* s_l = s_w + kMaxJoin * kRows;       // [n][kRows]
+    float* s_sum = s_l + kMaxJoin * kRows;     // [kRows]
+    auto slot = [&](int i) { return 2 * (c0 + first + i * step) + (first + i * step == 0); };
+    {
+        const int r = tid / kLanes, q = tid % kLanes;
+        float top = -INFINITY;
+#pragma unroll 2
+        for (int i = q; i < n; i += kLanes) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + slot(i) * kRows + r);
+            s_w[i * kRows + r] = ml.x;
+            s_l[i * kRows + r] = ml.y;
+            top = fmaxf(top, ml.x);
         }
-        s_top[tid] = top;
-        s_sum[tid] = sum;
-        if (final && tid < out.rows) out.write_lse(p, tid, top, sum);
-        if (!final) reinterpret_cast<float2*>(p.ws_ml)[slot(first) * kRows + tid] = make_float2(top, sum);
+#pragma unroll
+        for (int off = 1; off < kLanes; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+#pragma unroll 1
+        for (int i = q; i < n; i += kLanes) {
+            const float w = paged::exp2_approx(s_w[i * kRows + r] - base);
+            s_w[i * kRows + r] = w;
+            sum = fmaf(w, s_l[i * kRows + r], sum);
+        }
+#pragma unroll
+        for (int off = 1; off < kLanes; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (q == 0) {
+            s_sum[r] = sum;
+            if (final && r < out.rows) out.write_lse(p, r, top, sum);
+            if (!final) reinterpret_cast<float2*>(p.ws_ml)[slot(0) * kRows + r] = make_float2(top, sum);
+        }
     }
     __syncthreads();
+#pragma unroll 1
     for (int e = tid; e < out.rows * (D / 4); e += kThreads) {
         const int r = e / (D / 4), c = (e - r * (D / 4)) * 4;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
         for (int i = 0; i < n; ++i) {
-            const float4 o = __ldcg(reinterpret_cast<const float4*>(p.ws_o + (slot(first + i * step) * kRows + r) * D + c));
+            const float4 o = __ldcg(reinterpret_cast<const float4*>(p.ws_o + (slot(i) * kRows + r) * D + c));
             const float w = s_w[i * kRows + r];
             a.x = fmaf(w, o.x, a.x);
             a.y = fmaf(w, o.y, a.y);
@@ -170,7 +180,7 @@ __device__ void join_parts(const Params& p, const Out& out, int c0, int first, i
             a.w = fmaf(w, o.w, a.w);
         }
         if (final) out.write4<T, D>(p, r, c, a, s_sum[r]);
-        else *reinterpret_cast<float4*>(p.ws_o + (slot(first) * kRows + r) * D + c) = a;
+        else *reinterpret_cast<float4*>(p.ws_o + (slot(0) * kRows + r) * D + c) = a;
     }
 }
 
@@ -188,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_kernel(const Params p) {
     const Desc& d = p.d;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    paged::read_lengths<kRows, kKeys, kOver, kThreads>(d, len, LLONG_MAX);
+    paged::read_lengths<kRows, kKeys, kOver, kThreads, false>(d, len, 0);
     if (!len.head->ok) return;
     // every share has a unit, so every CTA between a cut tile's first and last
     // holds a part of it

@@ -652,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         prefetch_tensormap(&tmk);
         prefetch_tensormap(&tmv);
     }
-    paged::read_lengths<kRows, kKeys, kOver, kThreads>(p.d, len, (long long)kWholeFrom * gridDim.x);
+    paged::read_lengths<kRows, kKeys, kOver, kThreads, true>(p.d, len, (long long)kWholeFrom * gridDim.x);
     const int parts = len.head->ok ? int(min((long long)gridDim.x, len.head->total)) : 0;
     if (int(blockIdx.x) >= parts) return;
     if (threadIdx.x == 0) {

@@ -122,71 +122,101 @@ __device__ __forceinline__ int tile_units(const Desc& d, int n, int kv, int tile
     return max(1, (key_end<ROWS>(d, n, kv, tile) + KEYS - 1) / KEYS);
 }
 
+// Units of one kv head of a lane's sequence, every lane of the warp its own:
+// few row tiles alone, many by the whole warp.
+template <int ROWS, int KEYS, int OVER>
+__device__ __forceinline__ unsigned head_units(const Desc& d, int n, int kv, int tiles) {
+    const int lane = threadIdx.x & 31;
+    unsigned sum = 0;
+    if (tiles <= 4)
+        for (int t = 0; t < tiles; ++t) sum += tile_units<ROWS, KEYS>(d, n, kv, t) + OVER;
+    unsigned left = __ballot_sync(0xffffffffu, tiles > 4);
+    while (left) {
+        const int l = __ffs(left) - 1;
+        left &= left - 1;
+        const int ln = __shfl_sync(0xffffffffu, n, l), lkv = __shfl_sync(0xffffffffu, kv, l),
+                  lt = __shfl_sync(0xffffffffu, tiles, l);
+        unsigned part = 0;
+        for (int t = lane; t < lt; t += 32) part += tile_units<ROWS, KEYS>(d, ln, lkv, t) + OVER;
+        part = __reduce_add_sync(0xffffffffu, part);
+        if (lane == l) sum = part;
+    }
+    return sum;
+}
+
 // Reads and checks the lengths and counts the units; every thread of the CTA
 // calls it.  Lengths that are out of order or out of range raise the device
-// flag and make the call do nothing.  Row tiles are dealt out whole from
-// whole_from of them on.
-template <int ROWS, int KEYS, int OVER, int THREADS>
+// flag and make the call do nothing.  With MAY_BE_WHOLE, row tiles are dealt
+// out whole from whole_from of them on.  A thread takes a sequence: one round
+// of loads, and few meetings of the CTA, stand before the first copies.
+template <int ROWS, int KEYS, int OVER, int THREADS, bool MAY_BE_WHOLE>
 __device__ void read_lengths(const Desc& d, const Lengths& s, long long whole_from) {
+    constexpr int W = (THREADS + 31) / 32;
+    __shared__ unsigned long long s_part[W];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (tid == 0) s.head->ok = 1, s.head->total = 0;
-    for (int i = tid; i <= d.n_seq; i += THREADS) s.q0[i] = d.q_start[i];
-    for (int i = tid; i < d.n_seq; i += THREADS) s.kv[i] = d.kv_len[i];
-    __syncthreads();
+    bool good = true;
+    long long mine = 0;   // row tiles of the thread's sequences, of all heads
     for (int i = tid; i < d.n_seq; i += THREADS) {
-        const int n = s.q0[i + 1] - s.q0[i];
-        if (s.q0[i] < 0 || n < 0 || n > d.max_q || s.q0[i + 1] > d.n_tokens || s.kv[i] < 0 ||
-            (long long)s.kv[i] > (long long)d.max_pages * d.page_size)
-            s.head->ok = 0;
-        else
-            s.per_head[i] = row_tiles<ROWS>(d, n);
+        const int q0 = d.q_start[i], q1 = d.q_start[i + 1], kv = d.kv_len[i];
+        const int n = q1 - q0;
+        good = good && q0 >= 0 && q1 >= q0 && n <= d.max_q && q1 <= d.n_tokens && kv >= 0 &&
+               (long long)kv <= (long long)d.max_pages * d.page_size;
+        s.q0[i] = q0;
+        if (i + 1 == d.n_seq) s.q0[i + 1] = q1;
+        s.kv[i] = kv;
+        if (MAY_BE_WHOLE && good) mine += (long long)row_tiles<ROWS>(d, n) * d.n_head_kv;
     }
-    __syncthreads();
-    if (!s.head->ok) {
-        if (tid == 0) flag_input();
+    if (MAY_BE_WHOLE) {
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, off);
+        if (lane == 0) s_part[warp] = (unsigned long long)mine;
+    }
+    if (!__syncthreads_and(good)) {
+        if (tid == 0) s.head->ok = 0, flag_input();
+        __syncthreads();
         return;
     }
-    long long tiles = 0;
-    for (int i = tid; i < d.n_seq; i += THREADS) tiles += s.per_head[i];
-    tiles *= d.n_head_kv;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, off);
-    if (lane == 0 && tiles) atomicAdd(reinterpret_cast<unsigned long long*>(&s.head->total), (unsigned long long)tiles);
-    __syncthreads();
-    const bool whole = s.head->total >= whole_from;
-    if (!whole) {
-        // sequences of few row tiles a thread each, longer ones a warp each
-        for (int i = tid; i < d.n_seq; i += THREADS) {
-            const int n = s.q0[i + 1] - s.q0[i], tiles = int(s.per_head[i]);
-            if (tiles > 4) continue;
-            unsigned sum = 0;
-            for (int t = 0; t < tiles; ++t) sum += tile_units<ROWS, KEYS>(d, n, s.kv[i], t) + OVER;
-            s.per_head[i] = sum;
-        }
-        for (int i = warp; i < d.n_seq; i += THREADS / 32) {
-            const int n = s.q0[i + 1] - s.q0[i], tiles = row_tiles<ROWS>(d, n);
-            if (tiles <= 4) continue;
-            unsigned sum = 0;
-            for (int t = lane; t < tiles; t += 32) sum += tile_units<ROWS, KEYS>(d, n, s.kv[i], t) + OVER;
-            sum = __reduce_add_sync(0xffffffffu, sum);
-            if (lane == 0) s.per_head[i] = sum;
-        }
+    bool whole = false;
+    if (MAY_BE_WHOLE) {
+        long long tiles = 0;
+        for (int w = 0; w < W; ++w) tiles += (long long)s_part[w];
+        whole = tiles >= whole_from;
+        __syncthreads();   // s_part is free
     }
-    __syncthreads();
-    if (warp == 0) {
-        unsigned long long at = 0;
-        for (int i = 0; i < d.n_seq; i += 32) {
-            unsigned long long v = i + lane < d.n_seq ? (unsigned long long)s.per_head[i + lane] * d.n_head_kv : 0;
-            const unsigned long long own = v;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const unsigned long long u = __shfl_up_sync(0xffffffffu, v, off);
-                if (lane >= off) v += u;
-            }
-            if (i + lane < d.n_seq) s.first[i + lane] = at + v - own;
-            at += __shfl_sync(0xffffffffu, v, 31);
+    unsigned long long before = 0;   // units of the sequences of earlier rounds
+    for (int i0 = 0; i0 < d.n_seq; i0 += THREADS) {
+        const int i = i0 + tid;
+        int n = 0, kv = 0, tiles = 0;
+        if (i < d.n_seq) {
+            n = s.q0[i + 1] - s.q0[i];
+            kv = s.kv[i];
+            tiles = row_tiles<ROWS>(d, n);
         }
-        if (lane == 0) s.head->total = (long long)at, s.head->whole = whole;
+        const unsigned own = whole ? unsigned(tiles) : head_units<ROWS, KEYS, OVER>(d, n, kv, tiles);
+        const unsigned long long all = (unsigned long long)own * d.n_head_kv;
+        unsigned long long v = all;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const unsigned long long u = __shfl_up_sync(0xffffffffu, v, off);
+            if (lane >= off) v += u;
+        }
+        if (lane == 31) s_part[warp] = v;
+        __syncthreads();
+        unsigned long long base = before;
+        for (int w = 0; w < W; ++w) {
+            if (w < warp) base += s_part[w];
+            before += s_part[w];
+        }
+        if (i < d.n_seq) {
+            s.per_head[i] = own;
+            s.first[i] = base + v - all;
+        }
+        __syncthreads();
+    }
+    if (tid == 0) {
+        s.head->total = (long long)before;
+        s.head->whole = whole;
+        s.head->ok = 1;
     }
     __syncthreads();
 }
