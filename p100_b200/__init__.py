@@ -378,27 +378,28 @@ def _dtype_of(t, what):
     return kinds[t.dtype]
 
 
-def _need(t, what, dtype=None, values=None, dense=True):
-    """Refuses a tensor that a kernel of the current device could not read as it expects to."""
-    torch = _torch()
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
-        raise InvalidArgument(ERR_INVALID, f"{what} must be on the current device cuda:{torch.cuda.current_device()}, "
-                                           f"not {t.device}")
+def _need(t, what, dev, dtype=None, values=0, dense=True):
+    """Refuses a tensor that a kernel of the current device, dev, could not read as it expects to."""
+    if t.get_device() != dev:
+        raise InvalidArgument(ERR_INVALID, f"{what} must be on the current device cuda:{dev}, not {t.device}")
     if dtype is not None and t.dtype != dtype:
         raise InvalidArgument(ERR_INVALID, f"{what} must be {dtype}, not {t.dtype}")
     if dense and not t.is_contiguous():
         raise InvalidArgument(ERR_INVALID, f"{what} must be contiguous")
-    if values is not None and t.numel() < values:
+    if t.numel() < values:
         raise InvalidArgument(ERR_INVALID, f"{what} needs {values} values, has {t.numel()}")
 
 
 def _alloc(stream, make):
     """make() with its allocation and fill ordered on the stream of the call."""
-    torch = _torch()
     if stream is None:
         return make()
-    with torch.cuda.stream(stream):
+    with _torch().cuda.stream(stream):
         return make()
+
+
+def _raw_stream(stream, dev):
+    return (stream if stream is not None else _torch().cuda.current_stream(dev)).cuda_stream
 
 
 def _paged_type(desc):
@@ -406,40 +407,45 @@ def _paged_type(desc):
     return torch.bfloat16 if desc.dtype == BF16 else torch.float16
 
 
-def _rows_of(t, what, desc, dtype, stride):
+def _rows_of(t, what, dev, desc, dtype, stride):
     """A q or o tensor: n_tokens rows of n_head_q * head_dim, `stride` elements apart."""
     width = desc.n_head_q * desc.head_dim
-    _need(t, what, dtype, dense=False)
-    step = stride or width
-    if t.shape[0] < desc.n_tokens or t.numel() // max(1, t.shape[0]) < width:
+    _need(t, what, dev, dtype, dense=False)
+    shape = t.shape
+    if shape[0] < desc.n_tokens or t.numel() < shape[0] * width:
         raise InvalidArgument(ERR_INVALID, f"{what} needs {desc.n_tokens} rows of {width} values")
-    inner = 1
-    for size, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+    if t.is_contiguous() and t.numel() == shape[0] * width and stride in (0, width):
+        return
+    inner, strides = 1, t.stride()
+    for size, st in zip(reversed(shape[1:]), reversed(strides[1:])):
         if size != 1 and st != inner:
             raise InvalidArgument(ERR_INVALID, f"{what} must be contiguous within a row")
         inner *= size
-    if desc.n_tokens > 1 and t.stride(0) != step:
-        raise InvalidArgument(ERR_INVALID, f"{what} has rows {t.stride(0)} elements apart, the descriptor {step}")
+    if desc.n_tokens > 1 and strides[0] != (stride or width):
+        raise InvalidArgument(ERR_INVALID, f"{what} has rows {strides[0]} elements apart, the descriptor "
+                                           f"{stride or width}")
 
 
-def _pages_of(t, what, desc):
-    _need(t, what, _paged_type(desc), dense=False)
-    d = desc.head_dim
+def _pages_of(k_pages, v_pages, dev, desc):
+    dtype = _paged_type(desc)
+    d, n = desc.head_dim, desc.n_pages
     token = desc.token_stride or d
     head = desc.head_stride or desc.page_size * d
     page = desc.page_stride or desc.n_head_kv * desc.page_size * d
-    have = t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
-    need = ((desc.n_pages - 1) * page + (desc.n_head_kv - 1) * head + (desc.page_size - 1) * token + d
-            if desc.n_pages > 0 else 0)
-    if have < need:
-        raise InvalidArgument(ERR_INVALID, f"{what} needs {need} values behind its first, has {have}")
+    need = (n - 1) * page + (desc.n_head_kv - 1) * head + (desc.page_size - 1) * token + d if n > 0 else 0
+    for t, what in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        _need(t, what, dev, dtype, dense=False)
+        have = t.untyped_storage().nbytes() // 2 - t.storage_offset()
+        if have < need:
+            raise InvalidArgument(ERR_INVALID, f"{what} needs {need} values behind its first, has {have}")
 
 
-def _lengths_of(desc, block_table, q_start, kv_len):
-    torch = _torch()
-    _need(block_table, "block_table", torch.int32, desc.n_seq * desc.max_pages)
-    _need(q_start, "q_start", torch.int32, desc.n_seq + 1)
-    _need(kv_len, "kv_len", torch.int32, desc.n_seq)
+def _lengths_of(dev, desc, block_table, q_start, kv_len):
+    int32 = _torch().int32
+    n = desc.n_seq
+    _need(block_table, "block_table", dev, int32, n * desc.max_pages)
+    _need(q_start, "q_start", dev, int32, n + 1)
+    _need(kv_len, "kv_len", dev, int32, n)
 
 
 def paged_append(desc, qkv, block_table, q_start, kv_len, k_pages, v_pages, rope_cs=None, q_norm=None, k_norm=None,
@@ -448,33 +454,38 @@ def paged_append(desc, qkv, block_table, q_start, kv_len, k_pages, v_pages, rope
     [n_tokens, (n_head_q + 2 n_head_kv) head_dim] (float32, float16 or bfloat16), k and v to their pages, the
     queries returned as q [n_tokens, n_head_q, head_dim] of the cache's type."""
     torch = _torch()
+    dev = torch.cuda.current_device()
     width = (desc.n_head_q + 2 * desc.n_head_kv) * desc.head_dim
     qkv_type = _dtype_of(qkv, "qkv")
-    _need(qkv, "qkv", dense=False)
-    if qkv.dim() != 2 or qkv.shape[0] < desc.n_tokens or qkv.shape[1] != width or (qkv.stride(1) != 1):
+    _need(qkv, "qkv", dev, dense=False)
+    if qkv.dim() != 2 or qkv.shape[0] < desc.n_tokens or qkv.shape[1] != width or qkv.stride(1) != 1:
         raise InvalidArgument(ERR_INVALID, f"qkv must be [{desc.n_tokens}, {width}] with contiguous rows")
-    _lengths_of(desc, block_table, q_start, kv_len)
-    _pages_of(k_pages, "k_pages", desc)
-    _pages_of(v_pages, "v_pages", desc)
+    _lengths_of(dev, desc, block_table, q_start, kv_len)
+    _pages_of(k_pages, v_pages, dev, desc)
     for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
         if w is not None:
-            _need(w, what, torch.float32, desc.head_dim)
+            _need(w, what, dev, torch.float32, desc.head_dim)
     max_pos = 0
     if rope_cs is not None:
-        _need(rope_cs, "rope_cs", torch.float32)
+        _need(rope_cs, "rope_cs", dev, torch.float32)
         max_pos = rope_cs.numel() // desc.head_dim
     if q is None:
-        q = _alloc(stream, lambda: torch.empty_strided((desc.n_tokens, desc.n_head_q, desc.head_dim),
-                                                       (desc.q_stride or desc.n_head_q * desc.head_dim,
-                                                        desc.head_dim, 1), dtype=_paged_type(desc),
-                                                       device=qkv.device))
+        q = _alloc(stream, lambda: _new_rows(desc, _paged_type(desc), desc.q_stride, qkv.device))
     else:
-        _rows_of(q, "q", desc, _paged_type(desc), desc.q_stride)
-    stride = qkv.stride(0) if qkv.shape[0] > 1 else 0
-    check(lib().p100_paged_append(C.byref(desc), _ptr(qkv), qkv_type, stride, _ptr(q_norm), _ptr(k_norm), eps,
-                                  _ptr(rope_cs), max_pos, int(bool(rope_half)), _ptr(block_table), _ptr(q_start),
-                                  _ptr(kv_len), _ptr(q), _ptr(k_pages), _ptr(v_pages), _stream(stream)))
+        _rows_of(q, "q", dev, desc, _paged_type(desc), desc.q_stride)
+    check(lib().p100_paged_append(C.byref(desc), qkv.data_ptr(), qkv_type, qkv.stride(0) if qkv.shape[0] > 1 else 0,
+                                  _ptr(q_norm), _ptr(k_norm), eps, _ptr(rope_cs), max_pos, int(bool(rope_half)),
+                                  block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), q.data_ptr(),
+                                  k_pages.data_ptr(), v_pages.data_ptr(), _raw_stream(stream, dev)))
     return q
+
+
+def _new_rows(desc, dtype, stride, device):
+    torch = _torch()
+    shape = (desc.n_tokens, desc.n_head_q, desc.head_dim)
+    if not stride:
+        return torch.empty(shape, dtype=dtype, device=device)
+    return torch.empty_strided(shape, (stride, desc.head_dim, 1), dtype=dtype, device=device)
 
 
 def fa_paged_workspace(desc, stream=None):
@@ -493,27 +504,26 @@ def fa_paged(desc, q, k_pages, v_pages, block_table, q_start, kv_len, o=None, ls
     """Attention of the new tokens over a paged cache (p100_fa_paged): q [n_tokens, n_head_q, head_dim] of the
     cache's type -> o of the same shape (float32 with desc.o_fp32), lse fp32 [n_tokens, n_head_q]."""
     torch = _torch()
+    dev = torch.cuda.current_device()
     o_type = torch.float32 if desc.o_fp32 else _paged_type(desc)
-    _rows_of(q, "q", desc, _paged_type(desc), desc.q_stride)
-    _lengths_of(desc, block_table, q_start, kv_len)
-    _pages_of(k_pages, "k_pages", desc)
-    _pages_of(v_pages, "v_pages", desc)
+    _rows_of(q, "q", dev, desc, _paged_type(desc), desc.q_stride)
+    _lengths_of(dev, desc, block_table, q_start, kv_len)
+    _pages_of(k_pages, v_pages, dev, desc)
     if o is None:
-        o = _alloc(stream, lambda: torch.empty_strided((desc.n_tokens, desc.n_head_q, desc.head_dim),
-                                                       (desc.o_stride or desc.n_head_q * desc.head_dim,
-                                                        desc.head_dim, 1), dtype=o_type, device=q.device))
+        o = _alloc(stream, lambda: _new_rows(desc, o_type, desc.o_stride, q.device))
     else:
-        _rows_of(o, "o", desc, o_type, desc.o_stride)
+        _rows_of(o, "o", dev, desc, o_type, desc.o_stride)
     if lse is None:
-        lse = _alloc(stream, lambda: torch.empty(desc.n_tokens, desc.n_head_q, dtype=torch.float32, device=q.device))
+        lse = _alloc(stream, lambda: torch.empty((desc.n_tokens, desc.n_head_q), dtype=torch.float32, device=q.device))
     else:
-        _need(lse, "lse", torch.float32, desc.n_tokens * desc.n_head_q)
+        _need(lse, "lse", dev, torch.float32, desc.n_tokens * desc.n_head_q)
     if ws is None:
         ws = fa_paged_workspace(desc, stream)
     else:
-        _need(ws, "ws", torch.uint8)
-    check(lib().p100_fa_paged(C.byref(desc), _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(block_table), _ptr(q_start),
-                              _ptr(kv_len), _ptr(o), _ptr(lse), _ptr(ws), ws.numel(), _stream(stream)))
+        _need(ws, "ws", dev, torch.uint8)
+    check(lib().p100_fa_paged(C.byref(desc), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                              block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), o.data_ptr(),
+                              lse.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream(stream, dev)))
     return o, lse
 
 
@@ -533,32 +543,32 @@ def logprobs(logits, tokens=None, top_k=0, ws=None, stream=None):
     """Log probability, entropy, rank and top alternatives of rows of logits [rows, n] (p100_logprobs); tokens
     int32 [rows], -1 for none.  Returns LogProbs."""
     torch = _torch()
+    dev = torch.cuda.current_device()
     dtype = _dtype_of(logits, "logits")
-    _need(logits, "logits", dense=False)
+    _need(logits, "logits", dev, dense=False)
     if logits.dim() != 2 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise InvalidArgument(ERR_INVALID, "logits must be [rows, n] with contiguous rows")
     rows, n = logits.shape
     if not 0 <= top_k <= LOGPROBS_MAX_TOP:
         raise InvalidArgument(ERR_INVALID, "top_k must be between 0 and 32")
     if tokens is not None:
-        _need(tokens, "tokens", torch.int32, rows)
-
-    def outputs():
-        f = dict(dtype=torch.float32, device=logits.device)
-        i = dict(dtype=torch.int32, device=logits.device)
-        return LogProbs(torch.empty(rows, **f) if tokens is not None else None, torch.empty(rows, **f),
-                        torch.empty(rows, **i) if tokens is not None else None, torch.empty(rows, top_k, **i),
-                        torch.empty(rows, top_k, **f))
-
-    out = _alloc(stream, outputs)
+        _need(tokens, "tokens", dev, torch.int32, rows)
+    # one allocation: logprob, entropy, top_logprob as float32, then rank, top_index as int32
+    buf = _alloc(stream, lambda: torch.empty(rows * (3 + 2 * top_k), dtype=torch.float32, device=logits.device))
+    at = rows * (2 + top_k)
+    whole = buf[at:].view(torch.int32)
+    given = tokens is not None
+    out = LogProbs(buf[:rows] if given else None, buf[rows:2 * rows], whole[:rows] if given else None,
+                   whole[rows:].view(rows, top_k), buf[2 * rows:at].view(rows, top_k))
     if ws is None:
         ws = logprobs_workspace(rows, n, top_k, dtype, stream)
     else:
-        _need(ws, "ws", torch.uint8)
-    stride = logits.stride(0) if rows > 1 else 0
-    check(lib().p100_logprobs(_ptr(logits), dtype, n, rows, stride, _ptr(tokens), top_k, _ptr(out.logprob),
-                              _ptr(out.entropy), _ptr(out.rank), _ptr(out.top_index), _ptr(out.top_logprob), _ptr(ws),
-                              ws.numel() if ws is not None else 0, _stream(stream)))
+        _need(ws, "ws", dev, torch.uint8)
+    first = buf.data_ptr()
+    check(lib().p100_logprobs(logits.data_ptr(), dtype, n, rows, logits.stride(0) if rows > 1 else 0, _ptr(tokens),
+                              top_k, first if given else None, first + 4 * rows, first + 4 * at if given else None,
+                              first + 4 * (at + rows), first + 8 * rows, _ptr(ws), ws.numel() if ws is not None else 0,
+                              _raw_stream(stream, dev)))
     return out
 
 
