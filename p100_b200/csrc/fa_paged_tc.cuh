@@ -44,6 +44,10 @@ namespace fatc {
 using paged::Desc;
 using paged::Item;
 using paged::Lengths;
+using paged::add2;
+using paged::fma2;
+using paged::pair;
+using paged::unpair;
 
 constexpr int kRows = 256, kKeys = 128;
 constexpr int kOver = 4;                  // what a row tile costs beyond its keys, in units
@@ -199,31 +203,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* a
             return false;
         }
     }
-}
-
-// ------------------------------------------------------------ pairs of floats
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
 }
 
 // ------------------------------------------------------------ roles

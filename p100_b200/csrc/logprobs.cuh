@@ -8,15 +8,18 @@
 // the parts' triples are joined at the end.  -inf and NaN count as masked.
 //
 // The top alternatives need no second read of the row: the k-th largest of
-// the threads' maxima is a lower bound of the row's k-th largest value, and
-// only threads whose own maximum reaches it can hold one of the k.  On random
-// rows barely more than k threads do, so the block reads just their vectors
-// again (from L2), keeps the values that reach the bound and ranks them by
-// (value, lowest index).  Rows with more such values than the buffer holds
-// (long runs of equal logits) take k passes over the part instead, each
-// finding the largest key below the previous one.
+// the maxima of 32 groups of threads is a lower bound of the row's k-th
+// largest value, and only threads whose own maximum reaches it can hold one of
+// the k.  On random rows that is one to two times k threads, so the block
+// reads just their vectors again (from L2), keeps the values that reach the
+// bound and ranks them by (value, lowest index).  Rows with more such values
+// than the buffer holds (long runs of equal logits) take k passes over the
+// part instead, each finding the largest key below the previous one.
 //
-// Bytes bound it (the logits are read once).  Few rows are split over
+// Bytes bound it (the logits are read once); next come the exponentials, one a
+// logit, 0.7 of the time that 16-bit logits take to read.  So the rest is kept
+// small: 16-bit logits are masked, compared and counted two at a time before
+// their conversion, the sums run on pairs of FP32.  Few rows are split over
 // several CTAs; the last one of a row (an atomic ticket, no waiting) joins the
 // parts.
 #pragma once
@@ -27,8 +30,8 @@ namespace lp {
 
 constexpr int kThreads = 512;
 constexpr int kMaxTop = 32;
-constexpr int kCand = 2048;       // candidates kept in shared memory
-constexpr int kMaxParts = 64;     // parts x top <= kCand
+constexpr int kCand = 2048;       // candidates kept in shared memory, twice kMaxParts x kMaxTop
+constexpr int kMaxParts = 32;     // a lane each; parts x top <= kCand
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -68,43 +71,150 @@ __device__ __forceinline__ void join(float& m, float& s, float& u, float m2, flo
     m = mm;
 }
 
+// Logits at or below the floor of their type count as masked in the first
+// pass; a part whose largest is not above it, or not below `ceil` (where m
+// log2 e nears FP32's range), is summed again logit by logit.
 template <typename T>
-struct Vec {
-    static constexpr int N = 16 / sizeof(T);
-    __device__ static __forceinline__ void load(const T* p, float (&f)[N]) { unpack(*reinterpret_cast<const uint4*>(p), f); }
-    __device__ static __forceinline__ void unpack(const uint4& w, float (&f)[N]) {
-        const T* s = reinterpret_cast<const T*>(&w);
-#pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = paged::to_float<T>(s[i]);
-    }
+struct Range {
+    static constexpr float floor = -8.507059173023462e37f, ceil = 8.507059173023462e37f;   // 2^126, of FP32 and bfloat16
+};
+template <>
+struct Range<__half> {
+    static constexpr float floor = -65504.f, ceil = 3.402823466e38f;
 };
 
+// ------------------------------------------------------------ 16 bytes of logits
+// N logits: keep() replaces NaN and what lies below the floor by it, largest()
+// is their maximum, count() how many reach `ge`, get() the logits in FP32.
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+    static constexpr int N = 4;
+    float f[4];
+    __device__ __forceinline__ explicit Vec(const uint4& w) {
+        f[0] = __uint_as_float(w.x);
+        f[1] = __uint_as_float(w.y);
+        f[2] = __uint_as_float(w.z);
+        f[3] = __uint_as_float(w.w);
+    }
+    __device__ __forceinline__ int count(float ge) const {
+        return (f[0] >= ge) + (f[1] >= ge) + (f[2] >= ge) + (f[3] >= ge);
+    }
+    __device__ __forceinline__ void keep() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = fmaxf(f[i], Range<float>::floor);
+    }
+    __device__ __forceinline__ float largest() const { return fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])); }
+    __device__ __forceinline__ void get(float (&o)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = f[i];
+    }
+};
+template <typename T, typename T2>
+struct Vec16 {
+    static constexpr int N = 8;
+    T2 h[4];
+    __device__ __forceinline__ explicit Vec16(const uint4& w) {
+        const unsigned v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<const T2*>(&v[i]);
+    }
+    __device__ __forceinline__ int count(T2 ge) const {   // a byte's worth of 16-bit masks, four of them
+        const unsigned a = __hge2_mask(h[0], ge), b = __hge2_mask(h[1], ge), c = __hge2_mask(h[2], ge),
+                       d = __hge2_mask(h[3], ge);
+        return __popc((a & 0x00010001u) | (b & 0x00020002u) | (c & 0x00040004u) | (d & 0x00080008u));
+    }
+    __device__ __forceinline__ void keep(T2 lowest) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = __hmax2(h[i], lowest);
+    }
+    __device__ __forceinline__ float largest() const {
+        const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        return fmaxf(paged::to_float<T>(m.x), paged::to_float<T>(m.y));
+    }
+    __device__ __forceinline__ void get(float (&o)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            o[2 * i] = paged::to_float<T>(h[i].x);
+            o[2 * i + 1] = paged::to_float<T>(h[i].y);
+        }
+    }
+};
+template <>
+struct Vec<__half> : Vec16<__half, __half2> {
+    using Vec16::Vec16;
+    __device__ __forceinline__ int count(float ge) const { return Vec16::count(__float2half2_rn(ge)); }
+    __device__ __forceinline__ void keep() { Vec16::keep(__half2half2(__ushort_as_half(0xfbff))); }
+};
+template <>
+struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16, __nv_bfloat162> {
+    using Vec16::Vec16;
+    __device__ __forceinline__ int count(float ge) const { return Vec16::count(__float2bfloat162_rn(ge)); }
+    __device__ __forceinline__ void keep() { Vec16::keep(__bfloat162bfloat162(__ushort_as_bfloat16(0xfe80))); }
+};
+// The next larger value of T (`ge` of the logits behind the token).
+template <typename T>
+__device__ __forceinline__ float next_above(float x);
+template <>
+__device__ __forceinline__ float next_above<float>(float x) { return nextafterf(x, INFINITY); }
+__device__ __forceinline__ unsigned short next_bits(unsigned short b) {   // of a 16-bit float below +inf
+    return (b & 0x7fff) == 0 ? 1 : b & 0x8000 ? b - 1 : b + 1;
+}
+template <>
+__device__ __forceinline__ float next_above<__half>(float x) {
+    return __half2float(__ushort_as_half(next_bits(__half_as_ushort(__float2half_rn(x)))));
+}
+template <>
+__device__ __forceinline__ float next_above<__nv_bfloat16>(float x) {
+    return __bfloat162float(__ushort_as_bfloat16(next_bits(__bfloat16_as_ushort(__float2bfloat16_rn(x)))));
+}
+
+// A thread's running sums.
 struct Running {
     float m = -3.402823466e38f, s = 0.f, u = 0.f;
-    int above = 0;
+    uint64_t s2 = 0, u2 = 0;   // the same sums over pairs, since the last rise of m
 
-    // ge: a value counts above the token if it is >= ge.
+    __device__ __forceinline__ void fold() {
+        float a, b;
+        paged::unpair(s2, a, b);
+        s += a + b;
+        paged::unpair(u2, a, b);
+        u += a + b;
+        s2 = u2 = 0;
+    }
+    __device__ __forceinline__ void rise(float c) {
+        const float d = fmaxf((m - c) * kLog2e, -1e4f);
+        const float a = paged::exp2_approx(d);
+        u = a * fmaf(d, s, u);
+        s *= a;
+        m = c;
+    }
+    // N logits within the range of their type, the largest c.
     template <int N>
-    __device__ __forceinline__ void add(const float (&f)[N], float ge) {
-        float c = f[0];
-#pragma unroll
-        for (int i = 1; i < N; ++i) c = fmaxf(c, f[i]);
+    __device__ __forceinline__ void add(const float (&f)[N], float c) {
         if (c > m) {
-            const float d = fmaxf((m - c) * kLog2e, -1e4f);
-            const float a = paged::exp2_approx(d);
-            u = a * fmaf(d, s, u);
-            s *= a;
-            m = c;
+            fold();
+            rise(c);
         }
-        // the difference first: m log2 e would overflow for a row of the type's lowest value
+        const uint64_t l2 = paged::pair(kLog2e, kLog2e), b2 = paged::pair(-m * kLog2e, -m * kLog2e);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float d = fmaxf((f[i] - m) * kLog2e, -1e4f);
-            const float e = paged::exp2_approx(d);
-            s += e;
-            u = fmaf(e, d, u);
-            above += f[i] >= ge;
+        for (int i = 0; i < N; i += 2) {
+            const uint64_t d2 = paged::fma2(paged::pair(f[i], f[i + 1]), l2, b2);
+            float a, b;
+            paged::unpair(d2, a, b);
+            const uint64_t e2 = paged::pair(paged::exp2_approx(a), paged::exp2_approx(b));
+            s2 = paged::add2(s2, e2);
+            u2 = paged::fma2(e2, d2, u2);
         }
+    }
+    // One logit of any size but -inf: the difference first, which cannot overflow.
+    __device__ __forceinline__ void add_one(float f) {
+        if (f > m) rise(f);
+        const float d = fmaxf((f - m) * kLog2e, -1e4f);
+        const float e = paged::exp2_approx(d);
+        s += e;
+        u = fmaf(e, d, u);
     }
 };
 
@@ -129,12 +239,13 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
     constexpr int W = kThreads / 32;
     __shared__ unsigned long long s_key[kCand];
     __shared__ unsigned long long s_best[kMaxTop];
-    __shared__ float s_max[kThreads];
+    __shared__ unsigned long long s_word[W];
     __shared__ float s_m[W], s_s[W], s_u[W];
+    __shared__ float s_group[2 * W];
     __shared__ int s_above[W];
     __shared__ int s_hit[kThreads];
     __shared__ int s_count, s_hits, s_last;
-    __shared__ unsigned long long s_word[W];
+    static_assert(2 * W == 32 && kMaxTop <= 32, "a lane for each group of 16 threads");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int row = blockIdx.x / p.parts, part = blockIdx.x - row * p.parts;
@@ -142,16 +253,18 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
     // elements [lo, hi) of the row are this part's; vectors start at the row's
     // first 16-byte boundary, `head` elements in
     const int head = min(p.n, int(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
-    const long long part_lo = part ? (long long)head + (long long)part * p.part_len : 0;
-    const int lo = int(min((long long)p.n, part_lo));
+    const int lo = part ? int(min((long long)p.n, (long long)head + (long long)part * p.part_len)) : 0;
     const int hi = part + 1 == p.parts ? p.n : int(min((long long)p.n, (long long)head + (long long)(part + 1) * p.part_len));
     const int vlo = part ? lo : head;                 // first vector element
     const int nvec = max(0, hi - vlo) / N;
     const int tail = vlo + nvec * N;                  // elements behind the vectors
+    const int nfront = vlo - lo, nsingle = nfront + hi - tail;   // elements outside the vectors, a thread each
+    const int single = tid < nfront ? lo + tid : tail + tid - nfront;
 
     // the token's logit: values >= it count before its index, > it behind
+    const float nan = __int_as_float(0x7fc00000);
     int tok = -1;
-    float xt = -INFINITY, gt = INFINITY;
+    float xt = -INFINITY, ge = nan, gt = nan;
     if (p.token) {
         tok = p.token[row];
         if (tok < 0 || tok >= p.n) {
@@ -160,14 +273,22 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
         } else {
             xt = paged::to_float<T>(x[tok]);
             if (isnan(xt)) xt = -INFINITY;
+            ge = xt;
+            if (xt < INFINITY) gt = next_above<T>(xt);
         }
     }
-    gt = xt == INFINITY ? __int_as_float(0x7fc00000) : nextafterf(xt, INFINITY);
-    if (tok < 0) gt = __int_as_float(0x7fc00000);
-    const float ge = tok < 0 ? gt : xt;
 
     Running r;
+    int above = 0;
     const uint4* v = reinterpret_cast<const uint4*>(x + vlo);
+    auto take = [&](const uint4& w, int i) {
+        Vec<T> q(w);
+        above += q.count(vlo + i * N < tok ? ge : gt);
+        q.keep();
+        float f[N];
+        q.get(f);
+        r.add(f, q.largest());
+    };
     constexpr int U = 4;   // vectors in flight a thread
     int i = tid;
     for (; i + (U - 1) * kThreads < nvec; i += U * kThreads) {
@@ -175,92 +296,107 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
 #pragma unroll
         for (int j = 0; j < U; ++j) w[j] = v[i + j * kThreads];
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            float f[N];
-            Vec<T>::unpack(w[j], f);
-            r.add(f, vlo + (i + j * kThreads) * N < tok ? ge : gt);
-        }
+        for (int j = 0; j < U; ++j) take(w[j], i + j * kThreads);
     }
-    for (; i < nvec; i += kThreads) {
-        float f[N];
-        Vec<T>::unpack(v[i], f);
-        r.add(f, vlo + i * N < tok ? ge : gt);
-    }
-    // single elements in front of and behind the vectors
-    const int nfront = vlo - lo, nback = hi - tail;
-    if (tid < nfront + nback) {
-        const int idx = tid < nfront ? lo + tid : tail + tid - nfront;
-        float f[1] = {paged::to_float<T>(x[idx])};
-        r.add(f, idx < tok ? ge : gt);
+    for (; i < nvec; i += kThreads) take(v[i], i);
+    r.fold();
+    if (tid < nsingle) {
+        const float f = paged::to_float<T>(x[single]);
+        above += f >= (single < tok ? ge : gt);
+        if (f > Range<T>::floor) r.add_one(f);
     }
     // the vector that holds the token counted its equals as if all were in
-    // front of it (it starts before the token) : take those behind it out
+    // front of it (it starts before the token): take those behind it out
     if (tok >= vlo && tok < tail && tid == 0) {
         const int base = vlo + (tok - vlo) / N * N;
         if (base < tok)
-            for (int e = tok; e < base + N; ++e) r.above -= paged::to_float<T>(x[e]) == xt;
+            for (int e = tok; e < base + N; ++e) above -= paged::to_float<T>(x[e]) == xt;
     }
 
     // join the threads
-    s_max[tid] = r.m;
-    float m = r.m, s = r.s, u = r.u;
-    int above = r.above;
-    if (s == 0.f && m != INFINITY) s_max[tid] = -INFINITY;   // nothing but masked logits
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, off), s2 = __shfl_xor_sync(0xffffffffu, s, off),
-                    u2 = __shfl_xor_sync(0xffffffffu, u, off);
-        join(m, s, u, m2, s2, u2);
-    }
     above = __reduce_add_sync(0xffffffffu, above);
-    if (lane == 0) s_m[warp] = m, s_s[warp] = s, s_u[warp] = u, s_above[warp] = above;
+    if (lane == 0) s_above[warp] = above;
     if (tid == 0) s_count = s_hits = 0;
-    __syncthreads();
-    m = s_m[0], s = s_s[0], u = s_u[0], above = s_above[0];
+    float m, s, u;
+    auto join_threads = [&]() {
+        m = r.m, s = r.s, u = r.u;
+        float group = r.m;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            if (off < 16) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, off));
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, off), s2 = __shfl_xor_sync(0xffffffffu, s, off),
+                        u2 = __shfl_xor_sync(0xffffffffu, u, off);
+            join(m, s, u, m2, s2, u2);
+        }
+        if ((lane & 15) == 0) s_group[tid >> 4] = group;
+        if (lane == 0) s_m[warp] = m, s_s[warp] = s, s_u[warp] = u;
+        __syncthreads();
+        m = s_m[lane % W], s = s_s[lane % W], u = s_u[lane % W];
+#pragma unroll
+        for (int off = 1; off < W; off <<= 1) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, off), s2 = __shfl_xor_sync(0xffffffffu, s, off),
+                        u2 = __shfl_xor_sync(0xffffffffu, u, off);
+            join(m, s, u, m2, s2, u2);
+        }
+    };
+    join_threads();
+    above = __reduce_add_sync(0xffffffffu, lane < W ? s_above[lane] : 0);
+    float bottom = Range<T>::floor;   // maxima not above it are of masked logits
+    if (!(m > Range<T>::floor && m < Range<T>::ceil)) {
+        bottom = -INFINITY;
+        r = Running();
+        bool any = false;
+        auto again = [&](float f) {
+            if (f > -INFINITY) {
+                r.add_one(f);
+                any = true;
+            }
+        };
 #pragma unroll 1
-    for (int j = 1; j < W; ++j) {
-        join(m, s, u, s_m[j], s_s[j], s_u[j]);
-        above += s_above[j];
+        for (int k = tid; k < nvec; k += kThreads)   // the thread's own vectors, as before
+#pragma unroll 1
+            for (int e = 0; e < N; ++e) again(paged::to_float<T>(x[vlo + k * N + e]));
+        if (tid < nsingle) again(paged::to_float<T>(x[single]));
+        const float own = r.m;
+        __syncthreads();   // everyone has read the first sums
+        if (!any) r.m = -INFINITY;
+        join_threads();
+        r.m = any ? own : -INFINITY;
+        if (m == -INFINITY) m = -3.402823466e38f, s = u = 0.f;   // every logit masked
     }
 
     const int top = p.top;
     if (top > 0) {
-        // the top-th largest of the threads' maxima, by a search over the
-        // ordered bits (the largest t with at least `top` maxima >= t)
-        const unsigned mine = unsigned(make_key(s_max[tid], 0) >> 32);
-        unsigned t = 0;
-#pragma unroll 1
-        for (int b = 31; b >= 0; --b) {
-            const unsigned c = t | (1u << b);
-            if (__syncthreads_count(mine >= c) >= top) t = c;
+        // the top-th largest of the groups' maxima
+        const float group = s_group[lane];
+        int better = 0;
+#pragma unroll 8
+        for (int j = 0; j < 32; ++j) {
+            const float o = s_group[j];
+            better += o > group || (o == group && j < lane);
         }
-        const float bound = __uint_as_float(t & 0x80000000u ? t & 0x7fffffffu : ~t);
-        if (s_max[tid] >= bound && s_max[tid] > -INFINITY) s_hit[atomicAdd(&s_hits, 1)] = tid;
+        float bound = __shfl_sync(0xffffffffu, group, __ffs(__ballot_sync(0xffffffffu, better == top - 1)) - 1);
+        if (bound <= bottom) bound = -INFINITY;
+        if (bound > -INFINITY ? r.m >= bound : r.m > -INFINITY) s_hit[atomicAdd(&s_hits, 1)] = tid;
         __syncthreads();
         // the hit threads' vectors, shared out over the block
-        const int per = (nvec + kThreads - 1) / kThreads;
-        const long long work = (long long)s_hits * per;
-        for (long long k = tid; k < work; k += kThreads) {
-            const int h = int(k / per);
-            const int at = s_hit[h] + int(k - (long long)h * per) * kThreads;
-            if (at >= nvec) continue;
-            float f[N];
-            Vec<T>::unpack(v[at], f);
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (f[e] >= bound && f[e] > -INFINITY) {
-                    const int c = atomicAdd(&s_count, 1);
-                    if (c < kCand) s_key[c] = make_key(f[e], unsigned(vlo + at * N + e));
-                }
-        }
-        if (tid < nfront + nback) {
-            const int idx = tid < nfront ? lo + tid : tail + tid - nfront;
-            const float f = paged::to_float<T>(x[idx]);
+        const int per = (nvec + kThreads - 1) / kThreads, hits = s_hits;
+        auto keep = [&](float f, int idx) {
             if (f >= bound && f > -INFINITY) {
                 const int c = atomicAdd(&s_count, 1);
                 if (c < kCand) s_key[c] = make_key(f, unsigned(idx));
             }
+        };
+        for (int k = tid; k < hits * per; k += kThreads) {
+            const int h = k / per;
+            const int at = s_hit[h] + (k - h * per) * kThreads;
+            if (at >= nvec) continue;
+            float f[N];
+            Vec<T>(v[at]).get(f);
+#pragma unroll
+            for (int e = 0; e < N; ++e) keep(f[e], vlo + at * N + e);
         }
+        if (tid < nsingle) keep(paged::to_float<T>(x[single]), single);
         __syncthreads();
         if (s_count <= kCand) {
             rank_keys(s_key, s_count, top, s_best);
@@ -294,9 +430,12 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
     }
 
     if (p.parts > 1) {
-        const long long at = (long long)row * p.parts + part;
+        const int at = row * p.parts + part;
         if (tid < top) p.ws_keys[at * top + tid] = s_best[tid];
-        if (tid == 0) p.ws_sums[at] = make_float4(m, s, u, __int_as_float(above));
+        if (tid == 0) {
+            p.ws_sums[at] = make_float4(m, s, u, __int_as_float(above));
+            s_count = 0;
+        }
         __threadfence();
         __syncthreads();
         if (tid == 0) s_last = atomicAdd(p.tickets + row, 1u) == unsigned(p.parts - 1);
@@ -304,31 +443,51 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
         if (!s_last) return;
         __threadfence();
         if (tid == 0) p.tickets[row] = 0;   // ready for the next call
-        const long long first = (long long)row * p.parts;
-        if (tid < p.parts) {
-            const float4 w = __ldcg(p.ws_sums + first + tid);
-            s_max[tid] = w.x;
-            s_max[kMaxParts + tid] = w.y;
-            s_max[2 * kMaxParts + tid] = w.z;
-            s_hit[tid] = __float_as_int(w.w);
-        }
+        const int first = row * p.parts;
         for (int k = tid; k < p.parts * top; k += kThreads) s_key[k] = __ldcg(p.ws_keys + first * top + k);
-        __syncthreads();
-        m = s_max[0], s = s_max[kMaxParts], u = s_max[2 * kMaxParts], above = s_hit[0];
-        for (int j = 1; j < p.parts; ++j) {
-            join(m, s, u, s_max[j], s_max[kMaxParts + j], s_max[2 * kMaxParts + j]);
-            above += s_hit[j];
+        // a part a lane, in every warp
+        const float4 w = lane < p.parts ? __ldcg(p.ws_sums + first + lane) : make_float4(-3.402823466e38f, 0.f, 0.f, 0.f);
+        m = w.x, s = w.y, u = w.z;
+        above = __reduce_add_sync(0xffffffffu, __float_as_int(w.w));
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, off), s2 = __shfl_xor_sync(0xffffffffu, s, off),
+                        u2 = __shfl_xor_sync(0xffffffffu, u, off);
+            join(m, s, u, m2, s2, u2);
         }
         if (top > 0) {
-            // keys of absent alternatives are 0 and equal: they rank behind every other
-            rank_keys(s_key, p.parts * top, top, s_best);
+            __syncthreads();
+            // a lower bound of the top-th key: the top-th of the parts' best
+            // ones, or, of fewer parts, the least of the parts' j-th ones,
+            // j x parts >= top; absent keys are 0
+            unsigned long long bound = 0;
+            if (p.parts >= top) {
+                const unsigned long long own = lane < p.parts ? s_key[lane * top] : 0;
+                int better = 0;
+                for (int j = 0; j < p.parts; ++j) {
+                    const unsigned long long o = s_key[j * top];
+                    better += o > own || (o == own && j < lane);
+                }
+                bound = __shfl_sync(0xffffffffu, own, __ffs(__ballot_sync(0xffffffffu, lane < p.parts && better == top - 1)) - 1);
+            } else {
+                bound = lane < p.parts ? s_key[lane * top + (top - 1) / p.parts] : ~0ull;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const unsigned long long o = __shfl_xor_sync(0xffffffffu, bound, off);
+                    if (o < bound) bound = o;
+                }
+            }
+            unsigned long long* kept = s_key + kMaxParts * kMaxTop;
+            for (int k = tid; k < p.parts * top; k += kThreads)
+                if (s_key[k] != 0 && s_key[k] >= bound) kept[atomicAdd(&s_count, 1)] = s_key[k];
+            __syncthreads();
+            rank_keys(kept, s_count, top, s_best);
         }
     }
 
     const bool infinite = m == INFINITY;   // a row with +inf has no finite log probabilities
     const bool empty = s == 0.f && !infinite;
     const float ls = kLn2 * log2f(s);
-    const float nan = __int_as_float(0x7fc00000);
     if (tid == 0) {
         if (p.logprob) p.logprob[row] = tok < 0 ? 0.f : infinite ? nan : empty ? -INFINITY : (xt - m) - ls;
         if (p.rank) p.rank[row] = tok < 0 ? -1 : above;
