@@ -381,7 +381,7 @@ p100_status p100_fa_paged(const p100_paged_desc* desc, const void* q, const void
                           const int* block_table, const int* q_start, const int* kv_len, void* o, float* lse, void* ws,
                           size_t ws_bytes, p100_stream_t stream);
 
-/* Scores rows of n logits (dtype P100_F32, P100_F16 or P100_BF16, rows
+/* Scores rows of n <= 2^24 logits (dtype P100_F32, P100_F16 or P100_BF16, rows
  * row_stride elements apart, 0 = n) in one read, every sum in FP32:
  *   logprob[r] = x[token[r]] - lse, entropy[r] = -sum p ln p,
  *   rank[r]: how many logits are larger than the token's, or equal with a

@@ -8,11 +8,11 @@
 // the parts' triples are joined at the end.  -inf and NaN count as masked.
 //
 // The top alternatives need no second read of the row: the k-th largest of
-// the maxima of 32 groups of threads is a lower bound of the row's k-th
-// largest value, and only threads whose own maximum reaches it can hold one of
-// the k.  On random rows that is one to two times k threads, so the block
-// reads just their vectors again (from L2), keeps the values that reach the
-// bound and ranks them by (value, lowest index).  Rows with more such values
+// the maxima of 64 groups of threads is a lower bound of the row's k-th
+// largest value, and only a thread's eighth of the row whose maximum reaches it
+// can hold one of the k.  On random rows that is one to two times k eighths,
+// so the block reads just their vectors again (from L2), keeps the values that
+// reach the bound and ranks them by (value, lowest index).  Rows with more such values
 // than the buffer holds (long runs of equal logits) take k passes over the
 // part instead, each finding the largest key below the previous one.
 //
@@ -23,14 +23,21 @@
 // several CTAs; the last one of a row (an atomic ticket, no waiting) joins the
 // parts.
 #pragma once
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace p100b {
 namespace lp {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 128;
+constexpr int kCtas = 8;           // of an SM
+constexpr int kSpans = 8;          // parts of a thread's vectors with a maximum of their own
+constexpr int kAhead = 4;          // vectors a thread has on their way
+constexpr int kGroups = 64, kGroup = kThreads / kGroups;   // groups of threads, each with a maximum
 constexpr int kMaxTop = 32;
 constexpr int kCand = 2048;       // candidates kept in shared memory, twice kMaxParts x kMaxTop
+constexpr int kMaxLogits = 1 << 24;
 constexpr int kMaxParts = 32;     // a lane each; parts x top <= kCand
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -98,9 +105,12 @@ struct Vec<float> {
         f[2] = __uint_as_float(w.z);
         f[3] = __uint_as_float(w.w);
     }
-    __device__ __forceinline__ int count(float ge) const {
-        return (f[0] >= ge) + (f[1] >= ge) + (f[2] >= ge) + (f[3] >= ge);
+    using Bound = float;
+    __device__ static __forceinline__ Bound bound(float ge) { return ge; }
+    __device__ __forceinline__ void count(Bound ge, unsigned& n) const {
+        n += (f[0] >= ge) + (f[1] >= ge) + (f[2] >= ge) + (f[3] >= ge);
     }
+    __device__ static __forceinline__ int counted(unsigned n) { return int(n); }
     __device__ __forceinline__ void keep() {
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[i] = fmaxf(f[i], Range<float>::floor);
@@ -120,10 +130,16 @@ struct Vec16 {
 #pragma unroll
         for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<const T2*>(&v[i]);
     }
-    __device__ __forceinline__ int count(T2 ge) const {   // a byte's worth of 16-bit masks, four of them
-        const unsigned a = __hge2_mask(h[0], ge), b = __hge2_mask(h[1], ge), c = __hge2_mask(h[2], ge),
-                       d = __hge2_mask(h[3], ge);
-        return __popc((a & 0x00010001u) | (b & 0x00020002u) | (c & 0x00040004u) | (d & 0x00080008u));
+    // Each pair's comparison is 0xffff in the half that holds; added up as one
+    // word, lo and hi of them make 65535 lo - 65536 hi modulo 2^32.
+    using Bound = T2;
+    __device__ __forceinline__ void count(Bound ge, unsigned& n) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n += __hge2_mask(h[i], ge);
+    }
+    __device__ static __forceinline__ int counted(unsigned n) {   // lo, hi < 2^16: kMaxLogits
+        const unsigned lo = -n & 0xffffu;
+        return int(lo + ((lo - ((n + lo) >> 16)) & 0xffffu));
     }
     __device__ __forceinline__ void keep(T2 lowest) {
 #pragma unroll
@@ -144,13 +160,13 @@ struct Vec16 {
 template <>
 struct Vec<__half> : Vec16<__half, __half2> {
     using Vec16::Vec16;
-    __device__ __forceinline__ int count(float ge) const { return Vec16::count(__float2half2_rn(ge)); }
+    __device__ static __forceinline__ Bound bound(float ge) { return __float2half2_rn(ge); }
     __device__ __forceinline__ void keep() { Vec16::keep(__half2half2(__ushort_as_half(0xfbff))); }
 };
 template <>
 struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16, __nv_bfloat162> {
     using Vec16::Vec16;
-    __device__ __forceinline__ int count(float ge) const { return Vec16::count(__float2bfloat162_rn(ge)); }
+    __device__ static __forceinline__ Bound bound(float ge) { return __float2bfloat162_rn(ge); }
     __device__ __forceinline__ void keep() { Vec16::keep(__bfloat162bfloat162(__ushort_as_bfloat16(0xfe80))); }
 };
 // The next larger value of T (`ge` of the logits behind the token).
@@ -170,34 +186,32 @@ __device__ __forceinline__ float next_above<__nv_bfloat16>(float x) {
     return __bfloat162float(__ushort_as_bfloat16(next_bits(__bfloat16_as_ushort(__float2bfloat16_rn(x)))));
 }
 
-// A thread's running sums.
+// A thread's running sums, relative to a logit m of the row that none of the
+// thread's exceeds.  (A lower reference would be cheaper to keep but costs the
+// entropy of rows with one dominant logit its last digits.)
 struct Running {
-    float m = -3.402823466e38f, s = 0.f, u = 0.f;
-    uint64_t s2 = 0, u2 = 0;   // the same sums over pairs, since the last rise of m
+    float m = -3.402823466e38f;
+    float top = -3.402823466e38f;   // the largest logit
+    uint64_t s2 = 0, u2 = 0;        // the sums, in two halves
+    uint64_t b2 = 0;                // -m log2 e, twice
 
-    __device__ __forceinline__ void fold() {
-        float a, b;
-        paged::unpair(s2, a, b);
-        s += a + b;
-        paged::unpair(u2, a, b);
-        u += a + b;
-        s2 = u2 = 0;
-    }
     __device__ __forceinline__ void rise(float c) {
         const float d = fmaxf((m - c) * kLog2e, -1e4f);
         const float a = paged::exp2_approx(d);
-        u = a * fmaf(d, s, u);
-        s *= a;
+        u2 = paged::mul2(paged::pair(a, a), paged::fma2(paged::pair(d, d), s2, u2));
+        s2 = paged::mul2(paged::pair(a, a), s2);
         m = c;
+        b2 = paged::pair(-m * kLog2e, -m * kLog2e);
     }
-    // N logits within the range of their type, the largest c.
+    // The largest of the logits that add() gets next.
+    __device__ __forceinline__ void reach(float c) {
+        top = fmaxf(top, c);
+        if (c > m) rise(c);
+    }
+    // N logits within the range of their type.
     template <int N>
-    __device__ __forceinline__ void add(const float (&f)[N], float c) {
-        if (c > m) {
-            fold();
-            rise(c);
-        }
-        const uint64_t l2 = paged::pair(kLog2e, kLog2e), b2 = paged::pair(-m * kLog2e, -m * kLog2e);
+    __device__ __forceinline__ void add(const float (&f)[N]) {
+        const uint64_t l2 = paged::pair(kLog2e, kLog2e);
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
             const uint64_t d2 = paged::fma2(paged::pair(f[i], f[i + 1]), l2, b2);
@@ -210,11 +224,21 @@ struct Running {
     }
     // One logit of any size but -inf: the difference first, which cannot overflow.
     __device__ __forceinline__ void add_one(float f) {
-        if (f > m) rise(f);
+        reach(f);
         const float d = fmaxf((f - m) * kLog2e, -1e4f);
         const float e = paged::exp2_approx(d);
-        s += e;
-        u = fmaf(e, d, u);
+        s2 = paged::add2(s2, paged::pair(e, 0.f));
+        u2 = paged::add2(u2, paged::pair(e * d, 0.f));
+    }
+    __device__ __forceinline__ float sum() const {
+        float a, b;
+        paged::unpair(s2, a, b);
+        return a + b;
+    }
+    __device__ __forceinline__ float weighted() const {
+        float a, b;
+        paged::unpair(u2, a, b);
+        return a + b;
     }
 };
 
@@ -233,73 +257,183 @@ __device__ __forceinline__ void rank_keys(const unsigned long long* s_key, int c
     __syncthreads();
 }
 
+// One part of a row, and where its vectors lie.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
+struct Part {
+    int row, part;
+    const T* x;
+    int lo, hi;       // its logits
+    int vlo, nvec;    // first logit and number of its vectors
+    int tok;          // the row's token, -1 for none
+    float given;      // its logit
+
+    __device__ __forceinline__ Part(const Params& p, int item) {
+        constexpr int N = Vec<T>::N;
+        row = item / p.parts;
+        part = item - row * p.parts;
+        x = static_cast<const T*>(p.x) + row * p.stride;
+        // vectors start at the row's first 16-byte boundary, `head` logits in
+        const int head = min(p.n, int(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
+        lo = part ? int(min((long long)p.n, (long long)head + (long long)part * p.part_len)) : 0;
+        hi = part + 1 == p.parts ? p.n : int(min((long long)p.n, (long long)head + (long long)(part + 1) * p.part_len));
+        vlo = part ? lo : head;
+        nvec = max(0, hi - vlo) / N;
+    }
+    __device__ __forceinline__ void load_token(const Params& p) {
+        tok = p.token ? p.token[row] : -1;
+        given = -INFINITY;
+        if (tok >= 0 && tok < p.n) given = paged::to_float<T>(x[tok]);
+    }
+    __device__ __forceinline__ void fetch(uint4 (&w)[kAhead]) const {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (int(threadIdx.x) + j * kThreads < nvec)
+                w[j] = reinterpret_cast<const uint4*>(x + vlo)[threadIdx.x + j * kThreads];
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, kCtas) logprobs_kernel(const Params p) {
     constexpr int N = Vec<T>::N;
     constexpr int W = kThreads / 32;
     __shared__ unsigned long long s_key[kCand];
     __shared__ unsigned long long s_best[kMaxTop];
     __shared__ unsigned long long s_word[W];
     __shared__ float s_m[W], s_s[W], s_u[W];
-    __shared__ float s_group[2 * W];
+    __shared__ float s_group[kGroups];
+    __shared__ float s_span[kSpans][kThreads];
+    uint64_t(*s_save)[kThreads] = reinterpret_cast<uint64_t(*)[kThreads]>(s_key);   // a thread's state before a span
+    unsigned(*s_back)[kThreads] = reinterpret_cast<unsigned(*)[kThreads]>(s_key + 2 * kThreads);
     __shared__ int s_above[W];
-    __shared__ int s_hit[kThreads];
     __shared__ int s_count, s_hits, s_last;
-    static_assert(2 * W == 32 && kMaxTop <= 32, "a lane for each group of 16 threads");
+    int* s_hit = reinterpret_cast<int*>(s_key + kCand / 2);   // spans to read again: kSpans x kThreads
+    static_assert(kGroups == 64 && kMaxTop <= 32 && kMaxParts <= 32, "a lane for each group, alternative and part");
+    static_assert(kSpans * kThreads * sizeof(int) <= kCand / 2 * sizeof(unsigned long long), "spans beside half of the keys");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int row = blockIdx.x / p.parts, part = blockIdx.x - row * p.parts;
-    const T* x = static_cast<const T*>(p.x) + row * p.stride;
-    // elements [lo, hi) of the row are this part's; vectors start at the row's
-    // first 16-byte boundary, `head` elements in
-    const int head = min(p.n, int(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
-    const int lo = part ? int(min((long long)p.n, (long long)head + (long long)part * p.part_len)) : 0;
-    const int hi = part + 1 == p.parts ? p.n : int(min((long long)p.n, (long long)head + (long long)(part + 1) * p.part_len));
-    const int vlo = part ? lo : head;                 // first vector element
-    const int nvec = max(0, hi - vlo) / N;
-    const int tail = vlo + nvec * N;                  // elements behind the vectors
-    const int nfront = vlo - lo, nsingle = nfront + hi - tail;   // elements outside the vectors, a thread each
+    uint4 w[kAhead];
+    Part<T> it(p, blockIdx.x);
+    it.fetch(w);
+    it.load_token(p);
+    const int row = it.row, part = it.part, lo = it.lo, hi = it.hi, vlo = it.vlo, nvec = it.nvec;
+    const T* x = it.x;
+    const int tail = vlo + nvec * N;                  // logits behind the vectors
+    const int nfront = vlo - lo, nsingle = nfront + hi - tail;   // logits outside the vectors, a thread each
     const int single = tid < nfront ? lo + tid : tail + tid - nfront;
 
     // the token's logit: values >= it count before its index, > it behind
     const float nan = __int_as_float(0x7fc00000);
-    int tok = -1;
+    int tok = it.tok;
     float xt = -INFINITY, ge = nan, gt = nan;
-    if (p.token) {
-        tok = p.token[row];
-        if (tok < 0 || tok >= p.n) {
-            if (tok != -1 && part == 0 && tid == 0) paged::flag_input();
-            tok = -1;
-        } else {
-            xt = paged::to_float<T>(x[tok]);
-            if (isnan(xt)) xt = -INFINITY;
-            ge = xt;
-            if (xt < INFINITY) gt = next_above<T>(xt);
-        }
+    if (tok < 0 || tok >= p.n) {
+        if (tok != -1 && part == 0 && tid == 0) paged::flag_input();
+        tok = -1;
+    } else {
+        xt = isnan(it.given) ? -INFINITY : it.given;
+        ge = xt;
+        if (xt < INFINITY) gt = next_above<T>(xt);
     }
 
     Running r;
-    int above = 0;
+    unsigned reached = 0;
+    const typename Vec<T>::Bound bge = Vec<T>::bound(ge), bgt = Vec<T>::bound(gt);
     const uint4* v = reinterpret_cast<const uint4*>(x + vlo);
-    auto take = [&](const uint4& w, int i) {
-        Vec<T> q(w);
-        above += q.count(vlo + i * N < tok ? ge : gt);
+    auto take = [&](const uint4& q4, int i) {
+        Vec<T> q(q4);
+        q.count(vlo + i * N < tok ? bge : bgt, reached);
         q.keep();
         float f[N];
         q.get(f);
-        r.add(f, q.largest());
+        r.reach(q.largest());
+        r.add(f);
     };
-    constexpr int U = 4;   // vectors in flight a thread
-    int i = tid;
-    for (; i + (U - 1) * kThreads < nvec; i += U * kThreads) {
-        uint4 w[U];
+    bool masked;   // the row seems to hold masked logits
+    {
+        // The block's first vectors give every thread its first reference:
+        // their maximum, which few of the later logits exceed.
+        float c = -3.402823466e38f;
+        bool low = false;
 #pragma unroll
-        for (int j = 0; j < U; ++j) w[j] = v[i + j * kThreads];
+        for (int j = 0; j < kAhead; ++j)
+            if (tid + j * kThreads < nvec) {
+                Vec<T> q(w[j]);
+                float f[N];
+                q.get(f);
 #pragma unroll
-        for (int j = 0; j < U; ++j) take(w[j], i + j * kThreads);
+                for (int e = 0; e < N; ++e) low = low || !(f[e] > Range<T>::floor);
+                q.keep();
+                c = fmaxf(c, q.largest());
+            }
+        c = warp_max(c);
+        if (lane == 0) s_m[warp] = c;
+        masked = __syncthreads_or(low);
+        c = s_m[0];
+        for (int j = 1; j < W; ++j) c = fmaxf(c, s_m[j]);
+        if (c > r.m) r.rise(c);
     }
-    for (; i < nvec; i += kThreads) take(v[i], i);
-    r.fold();
+    // a span: `per` vectors of every thread, a multiple of kAhead
+    const int rounds = (nvec + kAhead * kThreads - 1) / (kAhead * kThreads);
+    const int per = (rounds + kSpans - 1) / kSpans * kAhead;
+    float best = r.top;   // the thread's largest logit
+    auto run = [&](int k, int end, auto mask, bool loaded) {
+#pragma unroll 1
+        for (; k < end && (k + kAhead) * kThreads <= nvec; k += kAhead) {   // nobody's vectors end here
+            const int i = tid + k * kThreads;
+            if (!loaded) {
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) w[j] = v[i + j * kThreads];
+            }
+            loaded = false;
+            float c = -3.402823466e38f;
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                Vec<T> q(w[j]);
+                q.count(vlo + (i + j * kThreads) * N < tok ? bge : bgt, reached);
+                if (decltype(mask)::value) q.keep();
+                c = fmaxf(c, q.largest());
+            }
+            r.reach(c);
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                Vec<T> q(w[j]);
+                if (decltype(mask)::value) q.keep();
+                float f[N];
+                q.get(f);
+                r.add(f);
+            }
+        }
+#pragma unroll 1
+        for (; k < end; ++k)
+            if (tid + k * kThreads < nvec) take(v[tid + k * kThreads], tid + k * kThreads);
+    };
+    for (int span = 0; span < kSpans; ++span) {
+        r.top = -3.402823466e38f;
+        const int begin = min(span * per, rounds * kAhead), end = min(begin + per, rounds * kAhead);
+        if (begin < end) {
+            if (!masked) {
+                s_save[0][tid] = r.s2;
+                s_save[1][tid] = r.u2;
+                s_back[0][tid] = __float_as_uint(r.m);
+                s_back[1][tid] = reached;
+                run(begin, end, std::false_type(), begin == 0);
+            }
+            if (masked || isnan(r.weighted())) {
+                if (!masked) {
+                    r.s2 = s_save[0][tid];
+                    r.u2 = s_save[1][tid];
+                    r.m = __uint_as_float(s_back[0][tid]);
+                    r.b2 = paged::pair(-r.m * kLog2e, -r.m * kLog2e);
+                    r.top = -3.402823466e38f;
+                    reached = s_back[1][tid];
+                }
+                run(begin, end, std::true_type(), false);
+            }
+        }
+        s_span[span][tid] = r.top;
+        best = fmaxf(best, r.top);
+    }
+    r.top = best;
+    int above = Vec<T>::counted(reached);
     if (tid < nsingle) {
         const float f = paged::to_float<T>(x[single]);
         above += f >= (single < tok ? ge : gt);
@@ -312,26 +446,29 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
         if (base < tok)
             for (int e = tok; e < base + N; ++e) above -= paged::to_float<T>(x[e]) == xt;
     }
-
     // join the threads
     above = __reduce_add_sync(0xffffffffu, above);
     if (lane == 0) s_above[warp] = above;
     if (tid == 0) s_count = s_hits = 0;
-    float m, s, u;
+    __syncthreads();   // s_m has been read
+    float m, s, u, most;   // most: the part's largest logit
     auto join_threads = [&]() {
-        m = r.m, s = r.s, u = r.u;
-        float group = r.m;
+        m = r.m, s = r.sum(), u = r.weighted();
+        float group = r.top;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            if (off < 16) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, off));
+            if (off < kGroup) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, off));
             const float m2 = __shfl_xor_sync(0xffffffffu, m, off), s2 = __shfl_xor_sync(0xffffffffu, s, off),
                         u2 = __shfl_xor_sync(0xffffffffu, u, off);
             join(m, s, u, m2, s2, u2);
         }
-        if ((lane & 15) == 0) s_group[tid >> 4] = group;
+        if (lane % kGroup == 0) s_group[tid / kGroup] = group;
         if (lane == 0) s_m[warp] = m, s_s[warp] = s, s_u[warp] = u;
         __syncthreads();
         m = s_m[lane % W], s = s_s[lane % W], u = s_u[lane % W];
+        most = fmaxf(s_group[lane], s_group[lane + 32]);
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
 #pragma unroll
         for (int off = 1; off < W; off <<= 1) {
             const float m2 = __shfl_xor_sync(0xffffffffu, m, off), s2 = __shfl_xor_sync(0xffffffffu, s, off),
@@ -342,7 +479,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
     join_threads();
     above = __reduce_add_sync(0xffffffffu, lane < W ? s_above[lane] : 0);
     float bottom = Range<T>::floor;   // maxima not above it are of masked logits
-    if (!(m > Range<T>::floor && m < Range<T>::ceil)) {
+    if (!(most > Range<T>::floor && most < Range<T>::ceil)) {
         bottom = -INFINITY;
         r = Running();
         bool any = false;
@@ -352,44 +489,55 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
                 any = true;
             }
         };
+        float best = -INFINITY;
 #pragma unroll 1
-        for (int k = tid; k < nvec; k += kThreads)   // the thread's own vectors, as before
+        for (int span = 0; span < kSpans; ++span) {   // the thread's own vectors, as before
+            r.top = -INFINITY;
 #pragma unroll 1
-            for (int e = 0; e < N; ++e) again(paged::to_float<T>(x[vlo + k * N + e]));
+            for (int k = span * per; k < (span + 1) * per && tid + k * kThreads < nvec; ++k)
+#pragma unroll 1
+                for (int e = 0; e < N; ++e) again(paged::to_float<T>(x[vlo + (tid + k * kThreads) * N + e]));
+            s_span[span][tid] = r.top;
+            best = fmaxf(best, r.top);
+        }
+        r.top = best;
         if (tid < nsingle) again(paged::to_float<T>(x[single]));
-        const float own = r.m;
+        if (!any) r.top = -INFINITY;
         __syncthreads();   // everyone has read the first sums
-        if (!any) r.m = -INFINITY;
         join_threads();
-        r.m = any ? own : -INFINITY;
-        if (m == -INFINITY) m = -3.402823466e38f, s = u = 0.f;   // every logit masked
     }
 
     const int top = p.top;
     if (top > 0) {
         // the top-th largest of the groups' maxima
-        const float group = s_group[lane];
-        int better = 0;
-#pragma unroll 8
-        for (int j = 0; j < 32; ++j) {
+        const float g0 = s_group[lane], g1 = s_group[lane + 32];
+        int b0 = 0, b1 = 0;   // better ones
+#pragma unroll 4
+        for (int j = 0; j < kGroups; ++j) {
             const float o = s_group[j];
-            better += o > group || (o == group && j < lane);
+            b0 += o > g0 || (o == g0 && j < lane);
+            b1 += o > g1 || (o == g1 && j < lane + 32);
         }
-        float bound = __shfl_sync(0xffffffffu, group, __ffs(__ballot_sync(0xffffffffu, better == top - 1)) - 1);
+        const float found = b0 == top - 1 ? g0 : g1;
+        float bound = __shfl_sync(0xffffffffu, found,
+                                  __ffs(__ballot_sync(0xffffffffu, b0 == top - 1 || b1 == top - 1)) - 1);
         if (bound <= bottom) bound = -INFINITY;
-        if (bound > -INFINITY ? r.m >= bound : r.m > -INFINITY) s_hit[atomicAdd(&s_hits, 1)] = tid;
+        for (int span = 0; span < kSpans; ++span) {
+            const float t = s_span[span][tid];
+            if (bound > -INFINITY ? t >= bound : t > -INFINITY) s_hit[atomicAdd(&s_hits, 1)] = span * kThreads + tid;
+        }
         __syncthreads();
-        // the hit threads' vectors, shared out over the block
-        const int per = (nvec + kThreads - 1) / kThreads, hits = s_hits;
+        // the hit spans' vectors, shared out over the block
+        const int hits = s_hits;
         auto keep = [&](float f, int idx) {
             if (f >= bound && f > -INFINITY) {
                 const int c = atomicAdd(&s_count, 1);
-                if (c < kCand) s_key[c] = make_key(f, unsigned(idx));
+                if (c < kCand / 2) s_key[c] = make_key(f, unsigned(idx));
             }
         };
         for (int k = tid; k < hits * per; k += kThreads) {
-            const int h = k / per;
-            const int at = s_hit[h] + (k - h * per) * kThreads;
+            const int h = k / per, hit = s_hit[h];
+            const int at = hit % kThreads + (hit / kThreads * per + k - h * per) * kThreads;
             if (at >= nvec) continue;
             float f[N];
             Vec<T>(v[at]).get(f);
@@ -398,7 +546,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
         }
         if (tid < nsingle) keep(paged::to_float<T>(x[single]), single);
         __syncthreads();
-        if (s_count <= kCand) {
+        if (s_count <= kCand / 2) {
             rank_keys(s_key, s_count, top, s_best);
         } else {
             unsigned long long below = ~0ull;

@@ -194,27 +194,28 @@ p100_status launch_append_to(const paged::AppendParams& prm, int dtype, int head
 size_t dtype_bytes(int t) { return t == P100_F32 ? 4 : 2; }
 const char* logprobs_reason(int rows, int n, int dtype, int top_k) {
     if (rows < 0 || n <= 0) return "rows must not be negative and n must be positive";
+    if (n > lp::kMaxLogits) return "n exceeds 2^24";
     if (dtype != P100_F32 && dtype != P100_F16 && dtype != P100_BF16) return "unknown logit type";
     if (top_k < 0 || top_k > lp::kMaxTop) return "top_k must be between 0 and 32";
     return nullptr;
 }
-// Parts of a row: enough CTAs for three on every SM, each with a vector or
-// more for every thread.
+// Parts of a row: as many CTAs as the device holds at once, each with two
+// vectors or more for every thread.
 int logprobs_parts(int rows, int n, int dtype, int sms) {
     const long long vec = 16 / (long long)dtype_bytes(dtype);
-    const long long most = std::min<long long>(lp::kMaxParts, std::max(1LL, n / (vec * lp::kThreads)));
-    return int(std::max(1LL, std::min(most, 3LL * sms / std::max(1, rows))));
+    const long long most = std::min<long long>(lp::kMaxParts, n / (2 * vec * lp::kThreads));
+    return int(std::max(1LL, std::min(most, (long long)lp::kCtas * sms / std::max(1, rows))));
 }
 struct LogprobsWs {
     size_t tickets, sums, keys, total;
 };
-// Rows are split while there are at most 3 sms / 2 of them; the tickets' place
+// Rows are split while there are at most kCtas / 2 sms of them; the tickets' place
 // does not depend on the call, so one workspace serves calls of other shapes.
 LogprobsWs logprobs_ws(int rows, int parts, int top_k, int sms) {
     LogprobsWs w = {};
     if (parts > 1 && rows > 0) {
         const size_t cells = size_t(rows) * parts;
-        w.tickets = round256(size_t(sms) * 2 * sizeof(unsigned));
+        w.tickets = round256(size_t(sms) * lp::kCtas / 2 * sizeof(unsigned));
         w.sums = round256(cells * sizeof(float4));
         w.keys = round256(cells * top_k * sizeof(unsigned long long));
         w.total = w.tickets + w.sums + w.keys;
