@@ -248,7 +248,8 @@ p100_status p100_paged_append(const p100_paged_desc* desc, const void* qkv, int 
     if ((q_norm || k_norm) && !(std::isfinite(eps) && eps >= 0.0f))
         return set_error(P100_ERR_INVALID, "eps must be finite and non-negative");
     if (rope_cs && max_pos <= 0) return set_error(P100_ERR_INVALID, "max_pos must be positive");
-    if (p100_status st = require_sm100(nullptr, nullptr)) return st;
+    int sms = 0;
+    if (p100_status st = require_sm100(nullptr, &sms)) return st;
     if (desc->n_tokens == 0 || desc->n_seq == 0) return P100_OK;
     if (!qkv || !block_table || !q_start || !kv_len || !q || !k_pages || !v_pages)
         return set_error(P100_ERR_INVALID, "null buffer");
@@ -269,8 +270,15 @@ p100_status p100_paged_append(const p100_paged_desc* desc, const void* qkv, int 
     prm.q = q;
     prm.k = k_pages;
     prm.v = v_pages;
-    const long long groups = (heads + paged::kAppendHeads - 1) / paged::kAppendHeads;
-    const long long blocks = (desc->n_tokens * groups + paged::kAppendThreads / 32 - 1) / (paged::kAppendThreads / 32);
+    // as many warps a token as give every SM kAppendWarps of them, and no warp
+    // more than kAppendMost steps
+    const int at_once = qkv_type == P100_F32 ? 32 * paged::append_values<float>() / desc->head_dim
+                                             : 32 * paged::append_values<__half>() / desc->head_dim;
+    const int together = qkv_type == P100_F32 ? paged::append_steps<float>() : paged::append_steps<__half>();
+    const long long steps = paged::Steps(desc->n_head_q, desc->n_head_kv, at_once).all();
+    const long long fill = std::min((steps + together - 1) / together, (long long)sms * paged::kAppendWarps / desc->n_tokens);
+    prm.warps = int(std::max({1LL, fill, (steps + paged::kAppendMost - 1) / paged::kAppendMost}));
+    const long long blocks = ((long long)desc->n_tokens * prm.warps + paged::kAppendThreads / 32 - 1) / (paged::kAppendThreads / 32);
     if (blocks > INT_MAX) return set_error(P100_ERR_INVALID, "too many heads and tokens for one call");
     switch (qkv_type) {
         case P100_F32: return launch_append_to<float>(prm, desc->dtype, desc->head_dim, unsigned(blocks), stream);
