@@ -205,6 +205,30 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* a
     }
 }
 
+// Capped scores without the special-function unit, whose three operations a
+// score (this takes none) would bound the kernel: for |y| <= 1/2, y = near x,
+// (cap / scale) tanh(y) = x p(x^2) with tanh(y) / y as a polynomial of degree 4
+// in y^2, fitted to the least relative error (7e-8 with FP32's roundings).
+struct Cap {
+    uint64_t k[5];       // the coefficients of x^2, each twice
+    float in, out;       // cap_score's arguments for larger scores
+    float most;          // the largest |x| for the polynomial
+    __device__ __forceinline__ Cap(float scale, float softcap) {
+        const float near = scale / softcap, n2 = near * near, n4 = n2 * n2;
+        const float c[5] = {1.0f, -0.3333306908607483f * n2, 0.13324779272079468f * n4, -0.052986063063144684f * n4 * n2,
+                            0.017134996131062508f * n4 * n4};
+#pragma unroll
+        for (int i = 0; i < 5; ++i) k[i] = pair(c[i], c[i]);
+        in = 2.f * scale * 1.4426950408889634f / softcap;
+        out = softcap / scale;
+        most = near > 1e-4f ? 0.5f / near : -1.f;   // below, the powers would leave FP32's range
+    }
+    __device__ __forceinline__ uint64_t near_zero(uint64_t x) const {
+        const uint64_t z = paged::mul2(x, x);
+        return paged::mul2(x, fma2(z, fma2(z, fma2(z, fma2(z, k[4], k[3]), k[2]), k[1]), k[0]));
+    }
+};
+
 // ------------------------------------------------------------ roles
 // Hands out the CTA's items and brings their K and V tiles into the ring, in
 // the order the products take them.
@@ -395,9 +419,8 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
     const int w = threadIdx.x >> 7, row = threadIdx.x & 127;
     const uint32_t lanes = uint32_t(row & ~31) << 16;
     const uint32_t t_s = tmem + w * 128 + lanes, t_o = tmem + 256 + w * D + lanes;
-    // the scores' unit: log2 e / scale, or log2 once capped
-    const float c = CAP ? 1.0f : fabsf(p.scale) * kLog2e;
-    const float cap_in = CAP ? 2.f * fabsf(p.scale) * kLog2e / p.softcap : 0.f, cap = p.softcap * kLog2e;
+    const float c = fabsf(p.scale) * kLog2e;   // of the scores, capped ones too, to units of log2
+    const Cap cap(fabsf(p.scale), CAP ? p.softcap : 1.f);
     unsigned done = 0, used = 0;   // phases of s_full passed; key tiles of the CTA before this item
     bool loaded = false;           // the item's query row is on its way
     for (unsigned j = 0;; ++j) {
@@ -436,12 +459,25 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
                     loaded = true;
                 }
             }
+            const bool masked = __any_sync(0xffffffffu, limit < key0 + kKeys);
+            const int lim = limit - key0;
             if (CAP) {
+                if (masked) {   // whatever stands there must not look large
 #pragma unroll
-                for (int i = 0; i < 128; ++i) s[i] = fap::cap_score(s[i], cap_in, cap);
+                    for (int i = 0; i < 128; ++i) s[i] = i < lim ? s[i] : 0.f;
+                }
+                float far = 0.f;
+#pragma unroll
+                for (int i = 0; i < 128; ++i) far = fmaxf(far, fabsf(s[i]));
+                if (__all_sync(0xffffffffu, far <= cap.most)) {
+#pragma unroll
+                    for (int i = 0; i < 128; i += 2) unpair(cap.near_zero(pair(s[i], s[i + 1])), s[i], s[i + 1]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) s[i] = fap::cap_score(s[i], cap.in, cap.out);
+                }
             }
-            if (__any_sync(0xffffffffu, limit < key0 + kKeys)) {
-                const int lim = limit - key0;
+            if (masked) {
 #pragma unroll
                 for (int i = 0; i < 128; ++i) s[i] = i < lim ? s[i] : -INFINITY;
             }
