@@ -118,6 +118,68 @@ inline void attention_decode(const p100_attn_desc& d, const float* q, const void
     check(p100_fa_decode(&d, q, k, v, mask, o, lse, ws.data(), ws.size(), stream));
 }
 
+// New tokens of a batch of sequences and their paged K/V cache; zero fields
+// take p100_paged_desc's defaults.
+struct PagedDesc : p100_paged_desc {
+    PagedDesc() : p100_paged_desc{} {
+        head_dim = 128;
+        dtype = P100_F16;
+        causal = 1;
+    }
+};
+
+// Owns a workspace for attention_paged calls of one descriptor's heads; calls
+// that may run at the same time need one each.
+class FaPagedWorkspace {
+public:
+    FaPagedWorkspace() = default;
+    FaPagedWorkspace(const PagedDesc& d, cudaStream_t stream) : bytes_(p100_fa_paged_workspace_size(&d)) {
+        if (bytes_ == 0) throw std::invalid_argument(p100_last_error());
+        if (cudaMalloc(&ptr_, bytes_) != cudaSuccess) {
+            (void)cudaGetLastError();
+            throw Error(P100_ERR_CUDA, "cudaMalloc(paged attention workspace) failed");
+        }
+        if (const p100_status st = p100_fa_paged_workspace_init(ptr_, bytes_, stream)) {
+            cudaFree(ptr_);
+            check(st);
+        }
+    }
+    ~FaPagedWorkspace() {
+        if (ptr_) cudaFree(ptr_);
+    }
+    FaPagedWorkspace(FaPagedWorkspace&& o) noexcept : ptr_(std::exchange(o.ptr_, nullptr)), bytes_(std::exchange(o.bytes_, 0)) {}
+    FaPagedWorkspace& operator=(FaPagedWorkspace&& o) noexcept {
+        std::swap(ptr_, o.ptr_);
+        std::swap(bytes_, o.bytes_);
+        return *this;
+    }
+    FaPagedWorkspace(const FaPagedWorkspace&) = delete;
+    FaPagedWorkspace& operator=(const FaPagedWorkspace&) = delete;
+    void* data() const { return ptr_; }
+    std::size_t size() const { return bytes_; }
+
+private:
+    void* ptr_ = nullptr;
+    std::size_t bytes_ = 0;
+};
+
+// Per-head norms and rotation of fused fp32, fp16 or bf16 rows; k and v to the
+// pages, the queries to q (p100_paged_append).
+inline void paged_append(const PagedDesc& d, const void* qkv, p100_dtype qkv_type, long long qkv_stride, const float* q_norm,
+                         const float* k_norm, float eps, const float* rope_cs, int max_pos, bool rope_half,
+                         const int* block_table, const int* q_start, const int* kv_len, void* q, void* k_pages,
+                         void* v_pages, cudaStream_t stream) {
+    check(p100_paged_append(&d, qkv, qkv_type, qkv_stride, q_norm, k_norm, eps, rope_cs, max_pos, rope_half ? 1 : 0,
+                            block_table, q_start, kv_len, q, k_pages, v_pages, stream));
+}
+
+// Attention of the new tokens over the pages (p100_fa_paged).
+inline void attention_paged(const PagedDesc& d, const void* q, const void* k_pages, const void* v_pages,
+                            const int* block_table, const int* q_start, const int* kv_len, void* o, float* lse,
+                            const FaPagedWorkspace& ws, cudaStream_t stream) {
+    check(p100_fa_paged(&d, q, k_pages, v_pages, block_table, q_start, kv_len, o, lse, ws.data(), ws.size(), stream));
+}
+
 // One rank of a row-split tensor-parallel group.
 class TensorParallel {
 public:

@@ -370,12 +370,18 @@ def fa_decode(desc, q, k, v, mask=None, o=None, lse=None, ws=None, stream=None):
 
 
 # ------------------------------------------- paged cache: prompts and batches
+_kinds = None
+
+
 def _dtype_of(t, what):
-    torch = _torch()
-    kinds = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    if t.dtype not in kinds:
+    global _kinds
+    if _kinds is None:
+        torch = _torch()
+        _kinds = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    kind = _kinds.get(t.dtype)
+    if kind is None:
         raise InvalidArgument(ERR_INVALID, f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
-    return kinds[t.dtype]
+    return kind
 
 
 def _need(t, what, dev, dtype=None, values=0, dense=True):
@@ -470,7 +476,7 @@ def paged_append(desc, qkv, block_table, q_start, kv_len, k_pages, v_pages, rope
         _need(rope_cs, "rope_cs", dev, torch.float32)
         max_pos = rope_cs.numel() // desc.head_dim
     if q is None:
-        q = _alloc(stream, lambda: _new_rows(desc, _paged_type(desc), desc.q_stride, qkv.device))
+        q = _alloc(stream, lambda: _new_rows(qkv, desc, _paged_type(desc), desc.q_stride))
     else:
         _rows_of(q, "q", dev, desc, _paged_type(desc), desc.q_stride)
     check(lib().p100_paged_append(C.byref(desc), qkv.data_ptr(), qkv_type, qkv.stride(0) if qkv.shape[0] > 1 else 0,
@@ -480,12 +486,11 @@ def paged_append(desc, qkv, block_table, q_start, kv_len, k_pages, v_pages, rope
     return q
 
 
-def _new_rows(desc, dtype, stride, device):
-    torch = _torch()
+def _new_rows(like, desc, dtype, stride):
     shape = (desc.n_tokens, desc.n_head_q, desc.head_dim)
     if not stride:
-        return torch.empty(shape, dtype=dtype, device=device)
-    return torch.empty_strided(shape, (stride, desc.head_dim, 1), dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
+    return like.new_empty_strided(shape, (stride, desc.head_dim, 1), dtype=dtype)
 
 
 def fa_paged_workspace(desc, stream=None):
@@ -510,11 +515,11 @@ def fa_paged(desc, q, k_pages, v_pages, block_table, q_start, kv_len, o=None, ls
     _lengths_of(dev, desc, block_table, q_start, kv_len)
     _pages_of(k_pages, v_pages, dev, desc)
     if o is None:
-        o = _alloc(stream, lambda: _new_rows(desc, o_type, desc.o_stride, q.device))
+        o = _alloc(stream, lambda: _new_rows(q, desc, o_type, desc.o_stride))
     else:
         _rows_of(o, "o", dev, desc, o_type, desc.o_stride)
     if lse is None:
-        lse = _alloc(stream, lambda: torch.empty((desc.n_tokens, desc.n_head_q), dtype=torch.float32, device=q.device))
+        lse = _alloc(stream, lambda: q.new_empty((desc.n_tokens, desc.n_head_q), dtype=torch.float32))
     else:
         _need(lse, "lse", dev, torch.float32, desc.n_tokens * desc.n_head_q)
     if ws is None:
@@ -553,22 +558,23 @@ def logprobs(logits, tokens=None, top_k=0, ws=None, stream=None):
         raise InvalidArgument(ERR_INVALID, "top_k must be between 0 and 32")
     if tokens is not None:
         _need(tokens, "tokens", dev, torch.int32, rows)
-    # one allocation: logprob, entropy, top_logprob as float32, then rank, top_index as int32
-    buf = _alloc(stream, lambda: torch.empty(rows * (3 + 2 * top_k), dtype=torch.float32, device=logits.device))
-    at = rows * (2 + top_k)
-    whole = buf[at:].view(torch.int32)
     given = tokens is not None
-    out = LogProbs(buf[:rows] if given else None, buf[rows:2 * rows], whole[:rows] if given else None,
-                   whole[rows:].view(rows, top_k), buf[2 * rows:at].view(rows, top_k))
+
+    def outputs():
+        make, f, i = logits.new_empty, torch.float32, torch.int32
+        return LogProbs(make(rows, dtype=f) if given else None, make(rows, dtype=f),
+                        make(rows, dtype=i) if given else None, make((rows, top_k), dtype=i),
+                        make((rows, top_k), dtype=f))
+
+    out = _alloc(stream, outputs)
     if ws is None:
         ws = logprobs_workspace(rows, n, top_k, dtype, stream)
     else:
         _need(ws, "ws", dev, torch.uint8)
-    first = buf.data_ptr()
     check(lib().p100_logprobs(logits.data_ptr(), dtype, n, rows, logits.stride(0) if rows > 1 else 0, _ptr(tokens),
-                              top_k, first if given else None, first + 4 * rows, first + 4 * at if given else None,
-                              first + 4 * (at + rows), first + 8 * rows, _ptr(ws), ws.numel() if ws is not None else 0,
-                              _raw_stream(stream, dev)))
+                              top_k, _ptr(out.logprob), out.entropy.data_ptr(), _ptr(out.rank),
+                              out.top_index.data_ptr(), out.top_logprob.data_ptr(), _ptr(ws),
+                              ws.numel() if ws is not None else 0, _raw_stream(stream, dev)))
     return out
 
 
