@@ -84,7 +84,9 @@ struct Job {
     int count;           // key tiles; 0: no more items
     int key_tile, row0;  // first key tile; first row of the row tile in its kv head
     int q0, n, kv, end, head;
-    int whole, c0, c1;   // no other CTA has a part, or the CTAs that do
+    int whole;           // no other CTA has a part
+    int units;           // else the key tiles of the whole row tile,
+    long long first;     // and its first unit
 };
 constexpr int kJobs = 4;
 
@@ -263,10 +265,8 @@ __device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tm
                 job.end = end;
                 job.head = it.head;
                 job.whole = it.count == it.units;
-                if (!job.whole) {
-                    job.c0 = paged::share_of(it.tile_first, len.head->total, share.parts);
-                    job.c1 = paged::share_of(it.tile_first + it.units - 1, len.head->total, share.parts);
-                }
+                job.units = it.units;
+                job.first = it.tile_first;
             }
             mbar_arrive(&bars.job_full[j % kJobs]);
         }
@@ -412,7 +412,8 @@ __device__ __forceinline__ void load_query(const Params& p, const Job& job, int 
 }
 
 template <typename T, int D, bool CAP>
-__device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, uint32_t q_smem, uint8_t* ring, uint32_t tmem) {
+__device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, uint32_t q_smem, uint8_t* ring, uint32_t tmem,
+                                             long long total_units, int parts) {
     constexpr int NS = slots<D>();
     constexpr float kLog2e = 1.4426950408889634f;
     const Desc& d = p.d;
@@ -586,7 +587,8 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
             }
             write_lse(base, l);
         } else {
-            const int c0 = job.c0, c1 = job.c1;
+            // the CTAs that have a part
+            const int c0 = paged::share_of(job.first, total_units, parts), c1 = paged::share_of(job.first + job.units - 1, total_units, parts);
             const long long slot = (long long)(blockIdx.x * 2 + (job.key_tile == 0)) * 2 + w;
             float4* dst = reinterpret_cast<float4*>(p.ws_o) + slot * (D / 4) * 128 + row;
 #pragma unroll
@@ -612,34 +614,63 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
                 const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + w * 128 + row;
                 const float4* po = reinterpret_cast<const float4*>(p.ws_o) + (long long)w * (D / 4) * 128 + row;
                 auto part = [&](int q) { return ((long long)q * 2 + (q == c0)) * 2; };
-                float top = -INFINITY;
+                constexpr int kFew = 4;   // parts whose loads are all in flight together
+                const int np = c1 - c0 + 1;
+                float top = -INFINITY, total = 0.f, wt[kFew] = {0.f, 0.f, 0.f, 0.f};
+                if (np <= kFew) {
+                    float2 v[kFew];
+#pragma unroll
+                    for (int k = 0; k < kFew; ++k) v[k] = k < np ? __ldcg(ml + part(c0 + k) * 128) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+                    for (int k = 0; k < kFew; ++k) top = fmaxf(top, v[k].x);
+#pragma unroll
+                    for (int k = 0; k < kFew; ++k) {
+                        wt[k] = paged::exp2_approx(v[k].x - (top == -INFINITY ? 0.f : top));
+                        total = fmaf(wt[k], v[k].y, total);
+                    }
+                } else {
 #pragma unroll 4
-                for (int q = c0; q <= c1; ++q) top = fmaxf(top, __ldcg(ml + part(q) * 128).x);
-                const float safe = top == -INFINITY ? 0.f : top;
-                float total = 0.f;
+                    for (int q = c0; q <= c1; ++q) top = fmaxf(top, __ldcg(ml + part(q) * 128).x);
 #pragma unroll 4
-                for (int q = c0; q <= c1; ++q) {
-                    const float2 v = __ldcg(ml + part(q) * 128);
-                    total = fmaf(paged::exp2_approx(v.x - safe), v.y, total);
+                    for (int q = c0; q <= c1; ++q) {
+                        const float2 v = __ldcg(ml + part(q) * 128);
+                        total = fmaf(paged::exp2_approx(v.x - (top == -INFINITY ? 0.f : top)), v.y, total);
+                    }
                 }
+                const float safe = top == -INFINITY ? 0.f : top;
                 const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll 1
                 for (int i = 0; i < D / 32; ++i) {
                     float o[32];
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = 0.f;
-#pragma unroll 3
-                    for (int q = c0; q <= c1; ++q) {
-                        const float f = paged::exp2_approx(__ldcg(ml + part(q) * 128).x - safe);
-                        float4 v[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = __ldcg(po + (part(q) * (D / 4) + i * 8 + e) * 128);
+                    auto add = [&](const float4 (&v)[8], float f) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             o[4 * e] = fmaf(f, v[e].x, o[4 * e]);
                             o[4 * e + 1] = fmaf(f, v[e].y, o[4 * e + 1]);
                             o[4 * e + 2] = fmaf(f, v[e].z, o[4 * e + 2]);
                             o[4 * e + 3] = fmaf(f, v[e].w, o[4 * e + 3]);
+                        }
+                    };
+                    if (np <= kFew) {
+                        float4 v[kFew][8];
+#pragma unroll
+                        for (int k = 0; k < kFew; ++k)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                v[k][e] = k < np ? __ldcg(po + (part(c0 + k) * (D / 4) + i * 8 + e) * 128)
+                                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                        for (int k = 0; k < kFew; ++k) add(v[k], wt[k]);
+                    } else {
+#pragma unroll 2
+                        for (int q = c0; q <= c1; ++q) {
+                            const float f = paged::exp2_approx(__ldcg(ml + part(q) * 128).x - safe);
+                            float4 v[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[e] = __ldcg(po + (part(q) * (D / 4) + i * 8 + e) * 128);
+                            add(v, f);
                         }
                     }
                     write(i, o, inv);
@@ -702,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem);
     if (warp < kMmaWarp) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-        softmax_role<T, D, CAP>(p, bars, smem_addr(q_smem), ring, tmem);
+        softmax_role<T, D, CAP>(p, bars, smem_addr(q_smem), ring, tmem, len.head->total, parts);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
         if (warp == kLoadWarp) {
