@@ -375,7 +375,9 @@ p100_status p100_fa_paged_workspace_init(void* ws, size_t ws_bytes, p100_stream_
  * probabilities are rounded once to dtype for the product with V.  A row that
  * sees no key gives o = 0 and lse = -inf.  Within [0, kv_len), values that
  * are not finite reach the rows whose tile holds them even where causal hides
- * them.  lse [n_tokens][n_head_q] (natural log) may be NULL.
+ * them.  lse [n_tokens][n_head_q] (natural log) may be NULL; o must not overlap
+ * q.  Sequences may share pages.  Page sizes that are no multiple of 8 tokens
+ * take the kernel for single tokens, which is slow for prompts.
  * Results do not depend on the order in which blocks run. */
 p100_status p100_fa_paged(const p100_paged_desc* desc, const void* q, const void* k_pages, const void* v_pages,
                           const int* block_table, const int* q_start, const int* kv_len, void* o, float* lse, void* ws,

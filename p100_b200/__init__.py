@@ -450,6 +450,8 @@ def _lengths_of(dev, desc, block_table, q_start, kv_len):
     int32 = _torch().int32
     n = desc.n_seq
     _need(block_table, "block_table", dev, int32, n * desc.max_pages)
+    if block_table.dim() != 2 or block_table.shape[1] != desc.max_pages:
+        raise InvalidArgument(ERR_INVALID, f"block_table must be [n_seq, {desc.max_pages}]")
     _need(q_start, "q_start", dev, int32, n + 1)
     _need(kv_len, "kv_len", dev, int32, n)
 
@@ -474,7 +476,9 @@ def paged_append(desc, qkv, block_table, q_start, kv_len, k_pages, v_pages, rope
     max_pos = 0
     if rope_cs is not None:
         _need(rope_cs, "rope_cs", dev, torch.float32)
-        max_pos = rope_cs.numel() // desc.head_dim
+        if rope_cs.dim() != 3 or rope_cs.shape[1] != desc.head_dim // 2 or rope_cs.shape[2] != 2:
+            raise InvalidArgument(ERR_INVALID, f"rope_cs must be [max_pos, {desc.head_dim // 2}, 2]")
+        max_pos = rope_cs.shape[0]
     if q is None:
         q = _alloc(stream, lambda: _new_rows(qkv, desc, _paged_type(desc), desc.q_stride))
     else:

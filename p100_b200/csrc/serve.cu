@@ -97,6 +97,12 @@ bool fa_paged_on_tc(const paged::Desc& d) {
     return (long long)d.max_q * d.group > fap::kRows && d.page_size % 8 == 0 && d.n_pages > 0;
 }
 
+// Units of a sequence's kv head are counted in 32 bits.
+bool fa_paged_too_long(const paged::Desc& d, int rows, int keys, int over) {
+    const double tiles = std::ceil(double(d.max_q) * d.group / rows);
+    return tiles * (double(d.max_pages) * d.page_size / keys + 1 + over) >= 4294967295.0;
+}
+
 // Partials of both kernels share one place: their calls follow one another.
 struct FaPagedWs {
     size_t tickets, o, ml, total;
@@ -324,8 +330,13 @@ p100_status p100_fa_paged(const p100_paged_desc* desc, const void* q, const void
     if (desc->n_tokens == 0 || desc->n_seq == 0) return P100_OK;
     if (!q || !k_pages || !v_pages || !block_table || !q_start || !kv_len || !o)
         return set_error(P100_ERR_INVALID, "null buffer");
+    if (o == q) return set_error(P100_ERR_INVALID, "o must not be q");
     if (!aligned(q, 16) || !aligned(o, 16) || !aligned(k_pages, 16) || !aligned(v_pages, 16))
         return set_error(P100_ERR_INVALID, "q, o and the pages must be 16-byte aligned");
+    const bool on_tc = fa_paged_on_tc(prm.d);
+    if (on_tc ? fa_paged_too_long(prm.d, fatc::kRows, fatc::kKeys, fatc::kOver)
+              : fa_paged_too_long(prm.d, fap::kRows, fap::kKeys, fap::kOver))
+        return set_error(P100_ERR_INVALID, "max_q x max_pages x page_size is too long for one call");
     const FaPagedWs w = fa_paged_ws(*desc, sms);
     if (ws_bytes < w.total || !ws)
         return set_error(P100_ERR_INVALID, "workspace of %zu bytes needed, %zu given", w.total, ws ? ws_bytes : size_t(0));
@@ -345,7 +356,7 @@ p100_status p100_fa_paged(const p100_paged_desc* desc, const void* q, const void
     prm.ws_ml = reinterpret_cast<float*>(at + w.tickets + w.o);
     prm.scale = desc->scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(desc->head_dim)) : desc->scale;
     prm.softcap = desc->softcap;
-    if (fa_paged_on_tc(prm.d)) {
+    if (on_tc) {
         fatc::Params t = {};
         t.d = prm.d;
         t.q = prm.q;

@@ -133,6 +133,30 @@ def test_tokens_that_are_masked_or_missing(cuda):
     assert cuda.equal(r.top_index, want(cuda, x, tokens, 2)[3])
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_masked_logits_that_start_late(cuda, dtype):
+    """A padded vocabulary, and single masked logits far into rows that begin without any."""
+    x = logits(cuda, 6, 70001, dtype, 6)
+    x[0, 69000:] = -math.inf
+    x[1, 40000] = -math.inf
+    x[2, 50001] = math.nan
+    x[3, 30000:] = cuda.finfo(x.dtype).min
+    x[4, 20000::7] = -math.inf
+    x[5, 69999:] = math.nan
+    tokens = some_tokens(cuda, 6, 20000, 7)
+    check(cuda, x, tokens, 16)
+    check(cuda, x[1:2], tokens[1:2], 16)
+
+
+def test_rows_beyond_32_bits(cuda):
+    """Rows 400 MB apart: the last starts 2.2 billion elements behind the first."""
+    gap, rows, n = 200_000_003, 12, 5003
+    store = cuda.empty((rows - 1) * gap + n, dtype=cuda.float16, device="cuda")
+    x = store.as_strided((rows, n), (gap, 1))
+    x.copy_(logits(cuda, rows, n, "float16", 8))
+    check(cuda, x, some_tokens(cuda, rows, n, 8), 4)
+
+
 def test_infinite_logit(cuda):
     x = logits(cuda, 2, 3000, "float32", 4)
     x[0, 77] = math.inf

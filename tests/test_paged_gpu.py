@@ -319,6 +319,84 @@ def test_bad_lengths_and_pages_are_reported(cuda, q_lens, page):
     check(torch, b, o, lse, attend64(b, q))
 
 
+@pytest.mark.parametrize("n,long", [(130, 1), (300, 20), (1024, 1), (1024, 18)])
+def test_many_sequences(cuda, n, long):
+    """More sequences than a block has threads, up to the largest batch."""
+    rng = np.random.RandomState(n)
+    q_lens = [int(x) for x in rng.randint(0, long + 1, n)]
+    q_lens[-1] = long
+    kv_lens = [int(q + rng.randint(0, 90)) for q in q_lens]
+    b = Batch(cuda, q_lens, kv_lens, 2, 1, 64, "f16", 16, seed=n)
+    b.fill()
+    q = b.queries()
+    check(cuda, b, *attend(b, q), attend64(b, q))
+
+
+@pytest.mark.parametrize("q_len,page", [(1, 16), (40, 16), (40, 6)])
+def test_offsets_beyond_32_bits(cuda, q_len, page):
+    """Pages 3 GB apart: the last one starts 6 billion elements behind the first."""
+    torch = cuda
+    n_pages, hkv, dim, gap = 5, 2, 64, 1_500_000_000 // 8 * 8
+    kv = n_pages * page - 3
+    store = torch.empty((n_pages - 1) * gap + hkv * page * dim, dtype=torch.float16, device="cuda")
+    b = Batch(torch, [q_len], [kv if kv > q_len else q_len], 4, hkv, dim, "f16", page, seed=50, spare=0)
+    n_pages = b.n_pages
+    shape, strides = (n_pages, hkv, page, dim), (gap, page * dim, dim, 1)
+    if (n_pages - 1) * gap + hkv * page * dim > store.numel():
+        store = torch.empty((n_pages - 1) * gap + hkv * page * dim, dtype=torch.float16, device="cuda")
+    b.k = store.as_strided(shape, strides)
+    b.v = torch.empty_like(store).as_strided(shape, strides)
+    b.k.fill_(math.nan)
+    b.v.fill_(math.nan)
+    first = b.kv_lens[0] - q_len
+    b.fill()
+    qkv = torch.randn(q_len, (4 + 2 * hkv) * dim, generator=b.gen, device="cuda")
+    d = b.desc(page_stride=gap)
+    q = P.paged_append(d, qkv, b.table, b.q_start, b.kv_len, b.k, b.v)
+    want, length, ks = append64(b, qkv, None, None, None, 0.0, False)
+    near(torch, b.t, q, want, length)
+    near(torch, b.t, b.rows(b.k, 0, first), ks[0][0], ks[0][1])
+    o, lse = P.fa_paged(d, q, b.k, b.v, b.table, b.q_start, b.kv_len)
+    P.check(P.device_error())
+    check(torch, b, o, lse, attend64(b, q))
+
+
+@pytest.mark.parametrize("q_lens", [[1, 1, 1], [60, 200, 1]])
+def test_sequences_that_share_pages(cuda, q_lens):
+    """A common prefix held once: three block tables begin with the same pages."""
+    b = Batch(cuda, q_lens, [100 + 64 + n for n in q_lens], 8, 2, 128, "bf16", 32, seed=51)
+    for i in (1, 2):
+        b.table_host[i, :4] = b.table_host[0, :4]
+    b.table.copy_(cuda.from_numpy(b.table_host))
+    b.fill()
+    q = b.queries()
+    check(cuda, b, *attend(b, q), attend64(b, q))
+
+
+@pytest.mark.parametrize("q_lens", [[1, 1], [300, 1]])
+def test_two_calls_at_once_and_no_lse(cuda, q_lens):
+    """Two streams with a workspace each; lse left out through the C interface."""
+    import ctypes as C
+    torch = cuda
+    b = Batch(torch, q_lens, [3000, 2000], 16, 4, 128, "f16", 16, seed=52)
+    b.fill()
+    qs = [b.queries() for _ in range(2)]
+    d = b.desc()
+    want = [P.fa_paged(d, q, b.k, b.v, b.table, b.q_start, b.kv_len)[0].clone() for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    spaces = [P.fa_paged_workspace(d) for _ in range(2)]
+    outs = [torch.empty_like(w) for w in want]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for q, st, ws, o in zip(qs, streams, spaces, outs):
+            P.check(P.lib().p100_fa_paged(C.byref(d), q.data_ptr(), b.k.data_ptr(), b.v.data_ptr(), b.table.data_ptr(),
+                                          b.q_start.data_ptr(), b.kv_len.data_ptr(), o.data_ptr(), None, ws.data_ptr(),
+                                          ws.numel(), st.cuda_stream))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    P.check(P.device_error())
+
+
 # ------------------------------------------------------------------ append
 def append64(b, qkv, rope, q_norm, k_norm, eps, half):
     """(q [n_tokens, hq, dim], k and v per sequence, the pairs' lengths of q and k) in 64 bits."""

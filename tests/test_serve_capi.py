@@ -75,6 +75,7 @@ def test_logprobs_refusals(lib):
     for kw, why in ((dict(dtype=5), "unknown logit type"), (dict(n=0), "rows must not be negative and n must be positive"),
                     (dict(rows=-1), "rows must not be negative and n must be positive"),
                     (dict(k=33), "top_k must be between 0 and 32"), (dict(k=-1), "top_k must be between 0 and 32"),
+                    (dict(n=(1 << 24) + 1), "n exceeds 2^24"),
                     (dict(stride=99), "row_stride must be at least n"),
                     (dict(token=None), "logprob and rank need tokens"),
                     (dict(index=None), "top_k needs top_index and top_logprob")):
@@ -105,6 +106,11 @@ def test_refusals_on_the_device(cuda, lib):
     assert lib.p100_fa_paged(C.byref(d), Z, Z, Z, Z, Z, Z, Z, None, Z, size - 1, None) == P.ERR_INVALID
     assert lib.p100_fa_paged(C.byref(d), Z, Z, Z, Z, Z, Z, Z, None, None, size, None) == P.ERR_INVALID
     assert lib.p100_fa_paged(C.byref(d), Z, Z, Z, Z, Z, Z, Z, None, odd, size, None) == P.ERR_INVALID
+    assert lib.p100_fa_paged(C.byref(d), Z, Z, Z, Z, Z, Z, Z, None, Z, size, None) == P.ERR_INVALID
+    assert P.last_error() == "o must not be q"
+    far = desc(n_tokens=1 << 27, max_q=1 << 27, n_head_q=8, page_size=9, max_pages=(1 << 31) // 9 - 1)
+    assert lib.p100_fa_paged(C.byref(far), Z, Z, Z, Z, Z, Z, C.c_void_p(512), None, Z, size, None) == P.ERR_INVALID
+    assert P.last_error() == "max_q x max_pages x page_size is too long for one call"
     assert append(lib, d, qkv=odd) == P.ERR_INVALID
     assert lib.p100_logprobs(C.c_void_p(258), P.F32, 100, 1, 0, None, 0, None, Z, None, None, None, None, 0,
                              None) == P.ERR_INVALID
@@ -127,6 +133,13 @@ def test_refusals_on_the_device(cuda, lib):
                 (x.transpose(1, 2).contiguous().transpose(1, 2), pages, pages, table, starts, lens)):
         with pytest.raises(P.InvalidArgument):
             P.fa_paged(d, *bad)
+    with pytest.raises(P.InvalidArgument):   # rows of the table that are longer than the descriptor's
+        P.fa_paged(d, x, pages, pages, torch.zeros(2, 6, dtype=torch.int32, device="cuda"), starts, lens)
+    with pytest.raises(P.InvalidArgument):
+        P.fa_paged(d, x, pages, pages, table, starts, lens, o=x)
+    with pytest.raises(P.InvalidArgument):   # a table of angles for another head size
+        P.paged_append(d, torch.zeros(10, 1536, device="cuda"), table, starts, lens, pages, pages,
+                       rope_cs=torch.zeros(64, 32, 2, device="cuda"))
     with pytest.raises(P.InvalidArgument):
         P.paged_append(d, torch.zeros(10, 1535, device="cuda"), table, starts, lens, pages, pages)
     with pytest.raises(P.InvalidArgument):
