@@ -13,12 +13,14 @@
 //                   running maximum and sum in FP32, the probabilities rounded
 //                   to the cache's 16-bit type into tensor memory, in the
 //                   scores' place; at the end the accumulator, normalised
-//   warp 8          one lane issues every tcgen05.mma: S = Q K^T (both from
-//                   shared memory, K-major, 128-byte swizzle) and O += P V (P
-//                   from tensor memory, V as it lies, N-major), M = 128 rows
-//   warp 9          TMA: K and V tiles into a ring, one box per page or the
-//                   largest power of two of rows that divides a page (so pages
-//                   of any multiple of 8 tokens may end inside a tile)
+//   warp 8          issues every tcgen05.mma: S = Q K^T (both from shared
+//                   memory, K-major, 128-byte swizzle) and O += P V (P from
+//                   tensor memory, V as it lies, N-major), M = 128 rows
+//   warp 9          hands out the items and loads K and V tiles by TMA into a
+//                   ring, one box per page or the largest power of two of rows
+//                   that divides a page (so pages of any multiple of 8 tokens
+//                   may end inside a tile)
+//   warps 10, 11    complete the warpgroup, which a register split needs
 //
 // The accumulator is rescaled only when a row's maximum has risen by more
 // than 2^8 since the reference it uses (the probabilities then stay below 2^8,
@@ -27,9 +29,13 @@
 // Rows of V behind the last visible key are zeroed in shared memory before
 // their product, so what a page holds there reaches nothing.
 //
-// Tensor work bounds it: 4 x 128 x 128 x D MACs a unit.  One exponential per
-// score on the special-function units takes as many cycles as the products.
-// Every wait is bounded; a role that gives up raises the device flag and the
+// Tensor work bounds it: 4 x 128 x 128 x D MACs a unit (2048 cycles at D =
+// 128).  One exponential per score on the special-function units takes as many
+// cycles as the products.  Measured: 3800 cycles a unit; an 8192-token prompt
+// of 32 / 8 heads of 128 in 521 us at full clock, 557 us (987 TFLOP/s) under
+// the 1000 W cap; the same with two 64-key chains a row tile 581, two threads a
+// row 593, two issuing warps 694, some of the exponentials by a polynomial 580
+// and more.  Every wait is bounded; a role that gives up raises the device flag and the
 // CTA's abort word, the others see it and leave.
 #pragma once
 #include <cuda.h>
@@ -51,7 +57,7 @@ using paged::unpair;
 
 constexpr int kRows = 256, kKeys = 128;
 constexpr int kOver = 4;                  // what a row tile costs beyond its keys, in units
-constexpr int kWholeFrom = 4;             // row tiles per CTA from which they are dealt out whole
+constexpr int kWholeFrom = 4;             // row tiles per CTA from which they are dealt out whole (1024 tiles: 557 us, cut 599)
 constexpr int kThreads = 384;             // two softmax warpgroups; one of the two issuing warps and two idle ones
 constexpr int kMmaWarp = 8, kLoadWarp = 9;
 // Registers a thread after the split; 256 x 192 + 128 x 120 is what the block
