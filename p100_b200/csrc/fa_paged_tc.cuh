@@ -20,7 +20,8 @@
 //                   ring, one box per page or the largest power of two of rows
 //                   that divides a page (so pages of any multiple of 8 tokens
 //                   may end inside a tile)
-//   warps 10, 11    complete the warpgroup, which a register split needs
+//   warps 10, 11    load the tiles instead where a page is no multiple of 8
+//                   tokens: rows gathered by 16-byte asynchronous copies
 //
 // The accumulator is rescaled only when a row's maximum has risen by more
 // than 2^8 since the reference it uses (the probabilities then stay below 2^8,
@@ -58,8 +59,8 @@ using paged::unpair;
 constexpr int kRows = 256, kKeys = 128;
 constexpr int kOver = 4;                  // what a row tile costs beyond its keys, in units
 constexpr int kWholeFrom = 4;             // row tiles per CTA from which they are dealt out whole (1024 tiles: 557 us, cut 599)
-constexpr int kThreads = 384;             // two softmax warpgroups; one of the two issuing warps and two idle ones
-constexpr int kMmaWarp = 8, kLoadWarp = 9;
+constexpr int kThreads = 384;             // two softmax warpgroups; one of the issuing warp and the loading ones
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kGatherWarp = 10;
 // Registers a thread after the split; 256 x 192 + 128 x 120 is what the block
 // is launched with (384 x 168).
 constexpr int kSoftmaxRegs = 192, kIssueRegs = 120;
@@ -82,12 +83,14 @@ struct Params {
     float* ws_ml;       // [CTAs][2][2][128] float2
     unsigned* tickets;  // [CTAs][2]
     float scale, softcap;
-    int box;            // rows of a TMA box
+    int box;            // rows of a TMA box, 0: gathered rows
+    const void *k, *v;
 };
 
 // An item as the load warp hands it to the others, kJobs of them in a ring.
 struct Job {
     int count;           // key tiles; 0: no more items
+    int seq;
     int key_tile, row0;  // first key tile; first row of the row tile in its kv head
     int q0, n, kv, end, head;
     int whole;           // no other CTA has a part
@@ -246,7 +249,7 @@ __device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tm
     constexpr int NS = slots<D>();
     const Desc& d = p.d;
     const int lane = threadIdx.x & 31;
-    const int boxes = kKeys / p.box;                 // of a tile, at most 16
+    const int boxes = p.box ? kKeys / p.box : 1;     // of a tile, at most 16
     const int i = lane & (boxes - 1), half = lane / boxes;
     const bool mine = half < D / 64;
     const uint32_t at = uint32_t(half) * kSub + uint32_t(i) * p.box * 128;
@@ -263,6 +266,7 @@ __device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tm
             Job& job = bars.jobs[j % kJobs];
             job.count = more ? it.count : 0;
             if (more) {
+                job.seq = it.seq;
                 job.key_tile = it.key_tile;
                 job.row0 = it.tile * kRows;
                 job.q0 = len.q0[it.seq];
@@ -277,6 +281,7 @@ __device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tm
             mbar_arrive(&bars.job_full[j % kJobs]);
         }
         if (!more) break;
+        if (p.box == 0) continue;   // the gathering warps load
         const int* table = d.block_table + (long long)it.seq * d.max_pages;
         auto find = [&](int t, int& page, int& off) {
             const int key = (it.key_tile + t) * kKeys + i * p.box;
@@ -322,6 +327,68 @@ __device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tm
     }
     if (!ok)   // leave only when the copies in flight have landed
         for (unsigned u = used > NS ? used - NS : 0; u < used; ++u) mbar_wait(&bars.full[u % NS], (u / NS) & 1);
+}
+
+// The tiles of pages of any size: each of two warps gathers 64 keys' rows.  A
+// slot is announced when the next one's copies are under way, its own have
+// landed and are visible to the tensor cores.
+template <typename T, int D>
+__device__ __forceinline__ void gather_role(const Params& p, Barriers& bars, uint32_t ring) {
+    constexpr int NS = slots<D>();
+    constexpr int kChunks = D / 8, kStep = 32 / kChunks;   // 16-byte chunks of a row; rows of a copy of the warp
+    const Desc& d = p.d;
+    const int lane = threadIdx.x & 31, first = int((threadIdx.x >> 5) - kGatherWarp) * 64;
+    const int chunk = lane % kChunks, sub = lane / kChunks;
+    unsigned used = 0;
+    auto announce = [&](unsigned u) {
+        fence_async();
+        mbar_arrive(&bars.full[u % NS]);
+    };
+    for (unsigned j = 0;; ++j) {
+        if (!warp_wait(&bars.job_full[j % kJobs], (j / kJobs) & 1, &bars.abort)) return;
+        const Job& job = bars.jobs[j % kJobs];
+        const int count = job.count, end = job.end, key0 = job.key_tile * kKeys + first + lane;
+        if (count == 0) return;
+        const int* table = d.block_table + (long long)job.seq * d.max_pages;
+        const long long head = job.head * d.head_stride + chunk * 8;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.job_empty[j % kJobs]);
+        for (int t = 0; t < count; ++t) {
+            long long at[2];   // where the rows of keys `lane` and `lane + 32` begin, -1: not read
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int key = key0 + t * kKeys + h * 32;
+                at[h] = -1;
+                if (key < end) {
+                    const int n = key / d.page_size, page = table[n];
+                    if (page < 0 || page >= d.n_pages) paged::flag_input();
+                    else at[h] = page * d.page_stride + (long long)(key - n * d.page_size) * d.token_stride;
+                }
+            }
+#pragma unroll 1
+            for (int kv = 0; kv < 2; ++kv, ++used) {
+                if (used >= NS && !warp_wait(&bars.empty[used % NS], (used / NS - 1) & 1, &bars.abort)) {
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    return;
+                }
+                const T* from = static_cast<const T*>(kv ? p.v : p.k) + head;
+                const uint32_t slot = ring + (used % NS) * tile_bytes<D>() + (chunk >> 3) * kSub;
+#pragma unroll 8
+                for (int i = 0; i < 64; i += kStep) {
+                    const long long o = __shfl_sync(0xffffffffu, i < 32 ? at[0] : at[1], (i & 31) + sub);
+                    const int r = first + i + sub;
+                    fap::cp_async16(slot + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), from + (o < 0 ? 0 : o), o >= 0);
+                }
+                fap::cp_commit();
+                if (t + kv > 0) {
+                    fap::cp_wait<1>();
+                    announce(used - 1);
+                }
+            }
+        }
+        fap::cp_wait<0>();
+        announce(used - 1);
+    }
 }
 
 // Issues the products; false when a wait was given up.
@@ -700,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Lengths len(reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(&bars + 1) + 15) & ~uintptr_t(15)), p.d.n_seq);
     const int warp = threadIdx.x >> 5;
 
-    if (threadIdx.x == kLoadWarp * 32) {
+    if (threadIdx.x == kLoadWarp * 32 && p.box) {
         prefetch_tensormap(&tmk);
         prefetch_tensormap(&tmv);
     }
@@ -709,7 +776,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (int(blockIdx.x) >= parts) return;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 8; ++i) {
-            mbar_init(&bars.full[i], 1);
+            mbar_init(&bars.full[i], p.box ? 1 : 64);
             mbar_init(&bars.empty[i], 1);
         }
         for (int w = 0; w < 2; ++w) {
@@ -721,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < kJobs; ++i) {
             mbar_init(&bars.job_full[i], 1);
-            mbar_init(&bars.job_empty[i], 9);   // the softmax warps and the issuing one
+            mbar_init(&bars.job_empty[i], p.box ? 9 : 11);   // the softmax warps, the issuing one, the gathering ones
         }
         mbar_init(&bars.drain, 1);
         bars.abort = 0;
@@ -754,6 +821,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 mbar_wait(&bars.drain, 0);
             }
+        } else if (p.box == 0) {
+            gather_role<T, D>(p, bars, smem_addr(ring));
         }
     }
 

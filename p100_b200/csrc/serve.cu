@@ -91,11 +91,8 @@ constexpr int kMmaCtas = 2;
 static_assert(paged::kMaxSeq == P100_PAGED_MAX_SEQ, "lengths in shared memory");
 
 // The tensor-core kernel takes calls in which a sequence may have more rows
-// (new tokens x query heads per kv head) than the mma.sync kernel's row tile,
-// if the pages can be copied by boxes of whole rows.
-bool fa_paged_on_tc(const paged::Desc& d) {
-    return (long long)d.max_q * d.group > fap::kRows && d.page_size % 8 == 0 && d.n_pages > 0;
-}
+// (new tokens x query heads per kv head) than the mma.sync kernel's row tile.
+bool fa_paged_on_tc(const paged::Desc& d) { return (long long)d.max_q * d.group > fap::kRows && d.n_pages > 0; }
 
 // Units of a sequence's kv head are counted in 32 bits.
 bool fa_paged_too_long(const paged::Desc& d, int rows, int keys, int over) {
@@ -368,10 +365,17 @@ p100_status p100_fa_paged(const p100_paged_desc* desc, const void* q, const void
         t.tickets = prm.tickets;
         t.scale = prm.scale;
         t.softcap = prm.softcap;
+        t.k = k_pages;
+        t.v = v_pages;
+        // boxes of whole rows where 8 or more divide a page, else gathered rows
         t.box = std::min(fatc::kKeys, prm.d.page_size & -prm.d.page_size);
-        CUtensorMap tmk, tmv;
-        if (p100_status st = page_map(&tmk, k_pages, *desc, prm.d, t.box)) return st;
-        if (p100_status st = page_map(&tmv, v_pages, *desc, prm.d, t.box)) return st;
+        CUtensorMap tmk = {}, tmv = {};
+        if (t.box < 8) {
+            t.box = 0;
+        } else {
+            if (p100_status st = page_map(&tmk, k_pages, *desc, prm.d, t.box)) return st;
+            if (p100_status st = page_map(&tmv, v_pages, *desc, prm.d, t.box)) return st;
+        }
         return desc->dtype == P100_F16 ? launch_fa_paged_tc_d<__half>(t, desc->head_dim, tmk, tmv, sms, stream)
                                        : launch_fa_paged_tc_d<__nv_bfloat16>(t, desc->head_dim, tmk, tmv, sms, stream);
     }
