@@ -376,8 +376,7 @@ p100_status p100_fa_paged_workspace_init(void* ws, size_t ws_bytes, p100_stream_
  * sees no key gives o = 0 and lse = -inf.  Within [0, kv_len), values that
  * are not finite reach the rows whose tile holds them even where causal hides
  * them.  lse [n_tokens][n_head_q] (natural log) may be NULL; o must not overlap
- * q.  Sequences may share pages.  Page sizes that are no multiple of 8 tokens
- * take the kernel for single tokens, which is slow for prompts.
+ * q.  Sequences may share pages.
  * Results do not depend on the order in which blocks run. */
 p100_status p100_fa_paged(const p100_paged_desc* desc, const void* q, const void* k_pages, const void* v_pages,
                           const int* block_table, const int* q_start, const int* kv_len, void* o, float* lse, void* ws,

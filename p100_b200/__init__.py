@@ -441,6 +441,8 @@ def _pages_of(k_pages, v_pages, dev, desc):
     need = (n - 1) * page + (desc.n_head_kv - 1) * head + (desc.page_size - 1) * token + d if n > 0 else 0
     for t, what in ((k_pages, "k_pages"), (v_pages, "v_pages")):
         _need(t, what, dev, dtype, dense=False)
+        if t.numel() >= need and t.is_contiguous():
+            continue
         have = t.untyped_storage().nbytes() // 2 - t.storage_offset()
         if have < need:
             raise InvalidArgument(ERR_INVALID, f"{what} needs {need} values behind its first, has {have}")

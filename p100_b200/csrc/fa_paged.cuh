@@ -1,6 +1,5 @@
 // fa_paged.cuh — attention of new tokens over a paged cache on mma.sync: the
-// kernel for single tokens (16 query rows of a kv head or fewer) and for page
-// sizes that tensor copies cannot take.
+// kernel for single tokens (16 query rows of a kv head or fewer).
 //
 //   s_ij = scale q_i k_j  (then cap tanh(s / cap)),  j < limit_i
 //   o_i = sum_j e^(s_ij - m_i) v_j / sum_j e^(s_ij - m_i),  lse_i = m_i + ln sum

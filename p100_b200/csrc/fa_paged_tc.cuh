@@ -18,9 +18,8 @@
 //                   tensor memory, V as it lies, N-major), M = 128 rows
 //   warp 9          hands out the items and loads K and V tiles by TMA into a
 //                   ring, one box per page or the largest power of two of rows
-//                   that divides a page (so pages of any multiple of 8 tokens
-//                   may end inside a tile)
-//   warps 10, 11    load the tiles instead where a page is no multiple of 8
+//                   that divides a page (so pages may end inside a tile)
+//   warps 10, 11    load the tiles instead where a page is no multiple of 16
 //                   tokens: rows gathered by 16-byte asynchronous copies
 //
 // The accumulator is rescaled only when a row's maximum has risen by more
@@ -774,26 +773,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     paged::read_lengths<kRows, kKeys, kOver, kThreads, true>(p.d, len, (long long)kWholeFrom * gridDim.x);
     const int parts = len.head->ok ? int(min((long long)gridDim.x, len.head->total)) : 0;
     if (int(blockIdx.x) >= parts) return;
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < 8; ++i) {
-            mbar_init(&bars.full[i], p.box ? 1 : 64);
-            mbar_init(&bars.empty[i], 1);
-        }
-        for (int w = 0; w < 2; ++w) {
-            mbar_init(&bars.q_full[w], 128);
-            mbar_init(&bars.s_full[w], 1);
-            mbar_init(&bars.p_full[w][0], 128);
-            mbar_init(&bars.p_full[w][1], 128);
-            mbar_init(&bars.joined[w], 128);
-        }
-        for (int i = 0; i < kJobs; ++i) {
-            mbar_init(&bars.job_full[i], 1);
-            mbar_init(&bars.job_empty[i], p.box ? 9 : 11);   // the softmax warps, the issuing one, the gathering ones
-        }
+    // what the first copies wait for, side by side: the barriers, tensor memory
+    // and the load warp's place in the work
+    if (threadIdx.x < 8) {
+        mbar_init(&bars.full[threadIdx.x], p.box ? 1 : 64);
+        mbar_init(&bars.empty[threadIdx.x], 1);
+    } else if (threadIdx.x < 10) {
+        const int w = threadIdx.x - 8;
+        mbar_init(&bars.q_full[w], 128);
+        mbar_init(&bars.s_full[w], 1);
+        mbar_init(&bars.p_full[w][0], 128);
+        mbar_init(&bars.p_full[w][1], 128);
+        mbar_init(&bars.joined[w], 128);
+    } else if (threadIdx.x < 10 + kJobs) {
+        mbar_init(&bars.job_full[threadIdx.x - 10], 1);
+        mbar_init(&bars.job_empty[threadIdx.x - 10], p.box ? 9 : 11);   // the softmax warps, the issuing one, the gathering ones
+    } else if (threadIdx.x == 31) {
         mbar_init(&bars.drain, 1);
         bars.abort = 0;
-        fence_barrier_init();
     }
+    if (warp == 0) fence_barrier_init();
+    Units share;
+    if (warp == kLoadWarp) share.begin(p.d, len, blockIdx.x, parts);
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&bars.tmem)),
                      "r"(512u)
@@ -810,8 +811,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
         if (warp == kLoadWarp) {
-            Units share;
-            share.begin(p.d, len, blockIdx.x, parts);
             load_role<D>(p, &tmk, &tmv, len, bars, ring, share);
         } else if (warp == kMmaWarp) {
             if (!mma_role<T, D>(p.d, p.scale, bars, uniform(smem_addr(q_smem)), uniform(smem_addr(ring)),

@@ -257,6 +257,7 @@ struct Item {
 // The CTA whose share of `parts` holds unit u: the largest c with
 // total * c / parts <= u.
 __device__ __forceinline__ int share_of(long long u, long long total, int parts) {
+    if (total < (1LL << 31) / parts) return int((unsigned(u + 1) * unsigned(parts) - 1) / unsigned(total));
     return int(((u + 1) * parts - 1) / total);
 }
 
@@ -288,12 +289,18 @@ struct Share {
         parts = p;
         round = 0;
         if (s.head->whole) return;
-        at = s.head->total * cta / parts;
-        end = s.head->total * (cta + 1) / parts;
+        const long long total = s.head->total;
+        if (total < (1LL << 31) / parts) {   // short divisions
+            at = unsigned(total) * unsigned(cta) / unsigned(parts);
+            end = unsigned(total) * unsigned(cta + 1) / unsigned(parts);
+        } else {
+            at = total * cta / parts;
+            end = total * (cta + 1) / parts;
+        }
         if (at >= end) return;
         enter_seq(d, s, seq_of(d, s, at));
         const unsigned long long in_seq = (unsigned long long)at - s.first[seq];
-        head = int(in_seq / s.per_head[seq]);
+        head = in_seq >> 32 ? int(in_seq / s.per_head[seq]) : int(unsigned(in_seq) / s.per_head[seq]);
         unsigned rest = unsigned(in_seq - (unsigned long long)head * s.per_head[seq]);
         const int lane = threadIdx.x & 31;
         for (int t0 = 0;; t0 += 32) {   // the row tile that holds unit `rest` of the head
