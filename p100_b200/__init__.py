@@ -405,7 +405,12 @@ def _alloc(stream, make):
 
 
 def _raw_stream(stream, dev):
-    return (stream if stream is not None else _torch().cuda.current_stream(dev)).cuda_stream
+    # the handle of torch's current stream without making a Stream object (1 us of a 15 us call)
+    return stream.cuda_stream if stream is not None else _torch()._C._cuda_getCurrentRawStream(dev)
+
+
+def _addr(t):
+    return t.data_ptr() if t is not None else None
 
 
 def _paged_type(desc):
@@ -415,11 +420,11 @@ def _paged_type(desc):
 
 def _rows_of(t, what, dev, desc, dtype, stride):
     """A q or o tensor: n_tokens rows of n_head_q * head_dim, `stride` elements apart."""
-    width = desc.n_head_q * desc.head_dim
+    width, rows = desc.n_head_q * desc.head_dim, desc.n_tokens
     _need(t, what, dev, dtype, dense=False)
     shape = t.shape
-    if shape[0] < desc.n_tokens or t.numel() < shape[0] * width:
-        raise InvalidArgument(ERR_INVALID, f"{what} needs {desc.n_tokens} rows of {width} values")
+    if shape[0] < rows or t.numel() < shape[0] * width:
+        raise InvalidArgument(ERR_INVALID, f"{what} needs {rows} rows of {width} values")
     if t.is_contiguous() and t.numel() == shape[0] * width and stride in (0, width):
         return
     inner, strides = 1, t.stride()
@@ -434,11 +439,11 @@ def _rows_of(t, what, dev, desc, dtype, stride):
 
 def _pages_of(k_pages, v_pages, dev, desc):
     dtype = _paged_type(desc)
-    d, n = desc.head_dim, desc.n_pages
+    d, n, heads, size = desc.head_dim, desc.n_pages, desc.n_head_kv, desc.page_size
     token = desc.token_stride or d
-    head = desc.head_stride or desc.page_size * d
-    page = desc.page_stride or desc.n_head_kv * desc.page_size * d
-    need = (n - 1) * page + (desc.n_head_kv - 1) * head + (desc.page_size - 1) * token + d if n > 0 else 0
+    head = desc.head_stride or size * d
+    page = desc.page_stride or heads * size * d
+    need = (n - 1) * page + (heads - 1) * head + (size - 1) * token + d if n > 0 else 0
     for t, what in ((k_pages, "k_pages"), (v_pages, "v_pages")):
         _need(t, what, dev, dtype, dense=False)
         if t.numel() >= need and t.is_contiguous():
@@ -450,10 +455,10 @@ def _pages_of(k_pages, v_pages, dev, desc):
 
 def _lengths_of(dev, desc, block_table, q_start, kv_len):
     int32 = _torch().int32
-    n = desc.n_seq
-    _need(block_table, "block_table", dev, int32, n * desc.max_pages)
-    if block_table.dim() != 2 or block_table.shape[1] != desc.max_pages:
-        raise InvalidArgument(ERR_INVALID, f"block_table must be [n_seq, {desc.max_pages}]")
+    n, pages = desc.n_seq, desc.max_pages
+    _need(block_table, "block_table", dev, int32, n * pages)
+    if block_table.dim() != 2 or block_table.shape[1] != pages:
+        raise InvalidArgument(ERR_INVALID, f"block_table must be [n_seq, {pages}]")
     _need(q_start, "q_start", dev, int32, n + 1)
     _need(kv_len, "kv_len", dev, int32, n)
 
@@ -486,7 +491,7 @@ def paged_append(desc, qkv, block_table, q_start, kv_len, k_pages, v_pages, rope
     else:
         _rows_of(q, "q", dev, desc, _paged_type(desc), desc.q_stride)
     check(lib().p100_paged_append(C.byref(desc), qkv.data_ptr(), qkv_type, qkv.stride(0) if qkv.shape[0] > 1 else 0,
-                                  _ptr(q_norm), _ptr(k_norm), eps, _ptr(rope_cs), max_pos, int(bool(rope_half)),
+                                  _addr(q_norm), _addr(k_norm), eps, _addr(rope_cs), max_pos, int(bool(rope_half)),
                                   block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), q.data_ptr(),
                                   k_pages.data_ptr(), v_pages.data_ptr(), _raw_stream(stream, dev)))
     return q
@@ -507,7 +512,7 @@ def fa_paged_workspace(desc, stream=None):
     if n == 0:
         raise P100Error(ERR_INVALID, last_error())
     ws = _alloc(stream, lambda: torch.empty(n, dtype=torch.uint8, device="cuda"))
-    check(lib().p100_fa_paged_workspace_init(_ptr(ws), n, _stream(stream)))
+    check(lib().p100_fa_paged_workspace_init(_addr(ws), n, _stream(stream)))
     return ws
 
 
@@ -546,7 +551,7 @@ def logprobs_workspace(rows, n, top_k=0, dtype=F32, stream=None):
     if size == 0:
         return None   # none needed, or arguments that p100_logprobs reports with its status
     ws = _alloc(stream, lambda: torch.empty(size, dtype=torch.uint8, device="cuda"))
-    check(lib().p100_logprobs_workspace_init(_ptr(ws), size, _stream(stream)))
+    check(lib().p100_logprobs_workspace_init(_addr(ws), size, _stream(stream)))
     return ws
 
 
@@ -572,14 +577,14 @@ def logprobs(logits, tokens=None, top_k=0, ws=None, stream=None):
                         make(rows, dtype=i) if given else None, make((rows, top_k), dtype=i),
                         make((rows, top_k), dtype=f))
 
-    out = _alloc(stream, outputs)
+    out = outputs() if stream is None else _alloc(stream, outputs)
     if ws is None:
         ws = logprobs_workspace(rows, n, top_k, dtype, stream)
     else:
         _need(ws, "ws", dev, torch.uint8)
-    check(lib().p100_logprobs(logits.data_ptr(), dtype, n, rows, logits.stride(0) if rows > 1 else 0, _ptr(tokens),
-                              top_k, _ptr(out.logprob), out.entropy.data_ptr(), _ptr(out.rank),
-                              out.top_index.data_ptr(), out.top_logprob.data_ptr(), _ptr(ws),
+    check(lib().p100_logprobs(logits.data_ptr(), dtype, n, rows, logits.stride(0) if rows > 1 else 0, _addr(tokens),
+                              top_k, _addr(out.logprob), out.entropy.data_ptr(), _addr(out.rank),
+                              out.top_index.data_ptr(), out.top_logprob.data_ptr(), _addr(ws),
                               ws.numel() if ws is not None else 0, _raw_stream(stream, dev)))
     return out
 

@@ -185,6 +185,32 @@ def test_sharp_and_flat_rows(cuda):
     check(cuda, x, some_tokens(cuda, 3, 50000), 5)
 
 
+@pytest.mark.parametrize("dtype,base,step,n", [("float32", 1e6 / 3, 0.25, 5003), ("float32", -7.7e6, 1.0, 301),
+                                               ("float16", 50016.0, 32.0, 4097), ("bfloat16", 3.1e5, 2048.0, 700),
+                                               ("bfloat16", -3.3e30, 2.0 ** 95, 129), ("float32", 1.7e37, 2.0 ** 101, 65)])
+def test_large_logits(cuda, dtype, base, step, n):
+    """A common offset changes nothing: the differences are exact, so the tolerance has no term in the offset's size."""
+    g = cuda.Generator(device="cuda")
+    g.manual_seed(n)
+    y = cuda.randint(-6, 7, (5, n), generator=g, device="cuda").double() * step
+    x = (y + base).to(getattr(cuda, dtype))
+    check(cuda, x, some_tokens(cuda, 5, n, 9), 4)
+
+
+def test_confident_rows(cuda):
+    """One logit far above the rest: the small log probability of the top and the entropy keep their digits.  Terms of
+    e^-d carry 2^-22 and d's rounding, 2^-24 d; s = 1 + sum is rounded to 2^-24, and so are ln s and the entropy."""
+    for dtype, top in (("float32", 31.7), ("float16", 29.3), ("bfloat16", 33.25)):
+        x = logits(cuda, 16, 3001, dtype, 5, 1.0)
+        x[:, 77] = top
+        x[8:, 5:70] = -math.inf
+        tokens = cuda.full((16,), 77, dtype=cuda.int32, device="cuda")
+        r = check(cuda, x, tokens, 1)
+        lp, ent = want(cuda, x, tokens, 1)[:2]
+        assert float((r.logprob.double() - lp).abs().max()) <= 2.0 ** -22
+        assert float((r.entropy.double() - ent).abs().max()) <= 2.0 ** -22
+
+
 def test_graph_stream_and_shared_workspace(cuda):
     """One workspace for calls of several shapes, the same bits on every run, a captured call on new logits."""
     torch = cuda
