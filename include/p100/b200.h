@@ -365,7 +365,8 @@ p100_status p100_paged_append(const p100_paged_desc* desc, const void* qkv, int 
 /* Workspace bytes p100_fa_paged needs for desc on the current device: a
  * function of the head dimension and the heads' layout, not of the lengths. */
 size_t p100_fa_paged_workspace_size(const p100_paged_desc* desc);
-/* Makes a workspace ready for its first use (p100_fa_paged leaves it ready).
+/* Makes a workspace ready for its first use, and again after a call that ran
+ * into P100_ERR_TIMEOUT (p100_fa_paged leaves it ready otherwise).
  * Calls that may run at the same time need a workspace each. */
 p100_status p100_fa_paged_workspace_init(void* ws, size_t ws_bytes, p100_stream_t stream);
 /* Attention of the new tokens over their sequences' cached tokens, their own

@@ -423,7 +423,7 @@ def _rows_of(t, what, dev, desc, dtype, stride):
     width, rows = desc.n_head_q * desc.head_dim, desc.n_tokens
     _need(t, what, dev, dtype, dense=False)
     shape = t.shape
-    if shape[0] < rows or t.numel() < shape[0] * width:
+    if not shape or shape[0] < rows or t.numel() < shape[0] * width:
         raise InvalidArgument(ERR_INVALID, f"{what} needs {rows} rows of {width} values")
     if t.is_contiguous() and t.numel() == shape[0] * width and stride in (0, width):
         return
@@ -475,6 +475,8 @@ def paged_append(desc, qkv, block_table, q_start, kv_len, k_pages, v_pages, rope
     _need(qkv, "qkv", dev, dense=False)
     if qkv.dim() != 2 or qkv.shape[0] < desc.n_tokens or qkv.shape[1] != width or qkv.stride(1) != 1:
         raise InvalidArgument(ERR_INVALID, f"qkv must be [{desc.n_tokens}, {width}] with contiguous rows")
+    if qkv.shape[0] > 1 and qkv.stride(0) < width:   # 0, an expanded row, would mean the default
+        raise InvalidArgument(ERR_INVALID, "qkv's rows must not overlap")
     _lengths_of(dev, desc, block_table, q_start, kv_len)
     _pages_of(k_pages, v_pages, dev, desc)
     for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
@@ -564,6 +566,8 @@ def logprobs(logits, tokens=None, top_k=0, ws=None, stream=None):
     _need(logits, "logits", dev, dense=False)
     if logits.dim() != 2 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise InvalidArgument(ERR_INVALID, "logits must be [rows, n] with contiguous rows")
+    if logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]:   # 0, an expanded row, would mean the default
+        raise InvalidArgument(ERR_INVALID, "rows of logits must not overlap")
     rows, n = logits.shape
     if not 0 <= top_k <= LOGPROBS_MAX_TOP:
         raise InvalidArgument(ERR_INVALID, "top_k must be between 0 and 32")

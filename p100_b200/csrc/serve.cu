@@ -72,7 +72,7 @@ const char* paged_reason(const p100_paged_desc& in, paged::Desc& d) {
     d.causal = in.causal != 0;
     d.token_stride = in.token_stride ? in.token_stride : D;
     d.head_stride = in.head_stride ? in.head_stride : in.page_size * D;
-    d.page_stride = in.page_stride ? in.page_stride : in.n_head_kv * in.page_size * D;
+    d.page_stride = in.page_stride ? in.page_stride : (long long)in.n_head_kv * in.page_size * D;
     d.q_stride = in.q_stride ? in.q_stride : in.n_head_q * D;
     d.o_stride = in.o_stride ? in.o_stride : in.n_head_q * D;
     for (long long s : {d.token_stride, d.head_stride, d.page_stride}) {

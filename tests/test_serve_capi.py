@@ -153,3 +153,27 @@ def test_refusals_on_the_device(cuda, lib):
     with pytest.raises(P.InvalidArgument):
         P.logprobs(torch.zeros(4, 10, device="cuda"), top_k=33)
     P.check(P.device_error())
+
+
+@pytest.mark.gpu
+def test_rows_that_overlap_are_refused(cuda):
+    """Expanded rows have stride 0, which the C calls take for the contiguous default: refused before them."""
+    torch = cuda
+    d = desc()
+    pages = torch.zeros(8, 2, 16, 128, dtype=torch.float16, device="cuda")
+    table = torch.zeros(2, 4, dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, 4, 10], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([4, 6], dtype=torch.int32, device="cuda")
+    with pytest.raises(P.InvalidArgument):
+        P.logprobs(torch.zeros(1, 50, device="cuda").expand(4, 50))
+    with pytest.raises(P.InvalidArgument):
+        P.logprobs(torch.zeros(100, device="cuda").as_strided((4, 50), (8, 1)))
+    with pytest.raises(P.InvalidArgument):
+        P.paged_append(d, torch.zeros(1, 1536, device="cuda").expand(10, 1536), table, starts, lens, pages, pages)
+    with pytest.raises(P.InvalidArgument):
+        P.fa_paged(d, torch.zeros(1, 8, 128, dtype=torch.float16, device="cuda").expand(10, 8, 128), pages, pages,
+                   table, starts, lens)
+    with pytest.raises(P.InvalidArgument):
+        P.fa_paged(d, torch.zeros((), dtype=torch.float16, device="cuda"), pages, pages, table, starts, lens)
+    P.logprobs(torch.zeros(1, 50, device="cuda").expand(1, 50))
+    P.check(P.device_error())
