@@ -59,16 +59,19 @@ struct Params {
     unsigned* tickets;              // [rows]
 };
 
-// Larger value first, then lower index: one unsigned order.  -0 equals 0.
-__device__ __forceinline__ unsigned long long make_key(float v, unsigned idx) {
-    unsigned b = __float_as_uint(v + 0.0f);
-    b = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return ((unsigned long long)b << 32) | (~idx);
+// The unsigned order of values.  -0 equals 0.
+__device__ __forceinline__ unsigned ordered(float v) {
+    const unsigned b = __float_as_uint(v + 0.0f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float key_value(unsigned long long k) {
-    const unsigned b = unsigned(k >> 32);
+__device__ __forceinline__ float ordered_value(unsigned b) {
     return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
+// Larger value first, then lower index: one unsigned order.
+__device__ __forceinline__ unsigned long long make_key(float v, unsigned idx) {
+    return ((unsigned long long)ordered(v) << 32) | (~idx);
+}
+__device__ __forceinline__ float key_value(unsigned long long k) { return ordered_value(unsigned(k >> 32)); }
 __device__ __forceinline__ unsigned key_index(unsigned long long k) { return ~unsigned(k); }
 
 // (m, s, u) of the union of two disjoint sets.
@@ -305,13 +308,15 @@ __global__ void __launch_bounds__(kThreads, kCtas) logprobs_kernel(const Params 
     __shared__ unsigned long long s_word[W];
     __shared__ float s_m[W], s_s[W], s_u[W];
     __shared__ float s_group[kGroups];
+    __shared__ __align__(16) unsigned s_rank[kGroups];
+    __shared__ float s_bound;
     __shared__ float s_span[kSpans][kThreads];
     uint64_t(*s_save)[kThreads] = reinterpret_cast<uint64_t(*)[kThreads]>(s_key);   // a thread's state before a span
     unsigned(*s_back)[kThreads] = reinterpret_cast<unsigned(*)[kThreads]>(s_key + 2 * kThreads);
     __shared__ int s_above[W];
     __shared__ int s_count, s_hits, s_last;
     int* s_hit = reinterpret_cast<int*>(s_key + kCand / 2);   // spans to read again: kSpans x kThreads
-    static_assert(kGroups == 64 && kMaxTop <= 32 && kMaxParts <= 32, "a lane for each group, alternative and part");
+    static_assert(kGroups == 64 && W == 4 && kMaxTop <= 32 && kMaxParts <= 32, "a lane for each alternative and part, 16 groups a warp");
     static_assert(kSpans * kThreads * sizeof(int) <= kCand / 2 * sizeof(unsigned long long), "spans beside half of the keys");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -465,7 +470,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) logprobs_kernel(const Params 
                         u2 = __shfl_xor_sync(0xffffffffu, u, off);
             join(m, s, u, m2, s2, u2);
         }
-        if (lane % kGroup == 0) s_group[tid / kGroup] = group;
+        if (lane % kGroup == 0) {
+            s_group[tid / kGroup] = group;
+            s_rank[tid / kGroup] = ordered(group) / kGroups * kGroups + tid / kGroup;
+        }
         if (lane == 0) s_m[warp] = m, s_s[warp] = s, s_u[warp] = u;
         __syncthreads();
         m = s_m[lane % W], s = s_s[lane % W], u = s_u[lane % W];
@@ -512,19 +520,25 @@ __global__ void __launch_bounds__(kThreads, kCtas) logprobs_kernel(const Params 
 
     const int top = p.top;
     if (top > 0) {
-        // the top-th largest of the groups' maxima
-        const float g0 = s_group[lane], g1 = s_group[lane + 32];
-        int b0 = 0, b1 = 0;   // better ones
-#pragma unroll 4
-        for (int j = 0; j < kGroups; ++j) {
-            const float o = s_group[j];
-            b0 += o > g0 || (o == g0 && j < lane);
-            b1 += o > g1 || (o == g1 && j < lane + 32);
+        // the top-th largest of the groups' maxima, without their last bits,
+        // which tell equals apart: a warp ranks 16 of them, two lanes each
+        {
+            const unsigned own = s_rank[warp * 16 + lane % 16];
+            const uint4* others = reinterpret_cast<const uint4*>(s_rank) + lane / 16 * (kGroups / 8);
+            int better = 0;
+#pragma unroll 2
+            for (int j = 0; j < kGroups / 8; ++j) {
+                const uint4 o = others[j];
+                better += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
+            }
+            better += __shfl_xor_sync(0xffffffffu, better, 16);
+            if (better == top - 1 && lane < 16) {
+                const float b = ordered_value(own / kGroups * kGroups);
+                s_bound = b > bottom ? b : -INFINITY;
+            }
         }
-        const float found = b0 == top - 1 ? g0 : g1;
-        float bound = __shfl_sync(0xffffffffu, found,
-                                  __ffs(__ballot_sync(0xffffffffu, b0 == top - 1 || b1 == top - 1)) - 1);
-        if (bound <= bottom) bound = -INFINITY;
+        __syncthreads();
+        const float bound = s_bound;
         for (int span = 0; span < kSpans; ++span) {
             const float t = s_span[span][tid];
             if (bound > -INFINITY ? t >= bound : t > -INFINITY) s_hit[atomicAdd(&s_hits, 1)] = span * kThreads + tid;
