@@ -215,28 +215,31 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* a
     }
 }
 
-// Capped scores without the special-function unit, whose three operations a
-// score (this takes none) would bound the kernel: for |y| <= 1/2, y = near x,
-// (cap / scale) tanh(y) = x p(x^2) with tanh(y) / y as a polynomial of degree 4
-// in y^2, fitted to the least relative error (7e-8 with FP32's roundings).
+// Capped scores, in units of log2: softcap log2 e tanh(y), y = scale / softcap
+// times the score x.  For |y| <= 1/2 that is x p(x^2), tanh(y) / y a polynomial
+// of degree 4 in y^2 fitted to the least relative error (7e-8 with FP32's
+// roundings); larger scores go through the special-function unit first (three
+// operations a score, which would bound the kernel) and then through the
+// polynomial 1, so that both take the same way to the probabilities.
 struct Cap {
-    uint64_t k[5];       // the coefficients of x^2, each twice
-    float in, out;       // cap_score's arguments for larger scores
+    float k[5];          // the coefficients of x^2
+    float in, out;       // cap_score's arguments
     float most;          // the largest |x| for the polynomial
     __device__ __forceinline__ Cap(float scale, float softcap) {
-        const float near = scale / softcap, n2 = near * near, n4 = n2 * n2;
-        const float c[5] = {1.0f, -0.3333306908607483f * n2, 0.13324779272079468f * n4, -0.052986063063144684f * n4 * n2,
-                            0.017134996131062508f * n4 * n4};
-#pragma unroll
-        for (int i = 0; i < 5; ++i) k[i] = pair(c[i], c[i]);
-        in = 2.f * scale * 1.4426950408889634f / softcap;
-        out = softcap / scale;
-        most = near > 1e-4f ? 0.5f / near : -1.f;   // below, the powers would leave FP32's range
+        constexpr float kLog2e = 1.4426950408889634f;
+        const float near = scale / softcap, n2 = near * near, n4 = n2 * n2, c = scale * kLog2e;
+        k[0] = c;
+        k[1] = -0.3333306908607483f * (c * n2);
+        k[2] = 0.13324779272079468f * (c * n4);
+        k[3] = -0.052986063063144684f * (c * n4) * n2;
+        k[4] = 0.017134996131062508f * (c * n4) * n4;
+        in = 2.f * scale * kLog2e / softcap;
+        out = softcap * kLog2e;
+        // elsewhere the powers would leave FP32's range
+        most = near < 1e3f && k[4] > 1e-37f && k[4] < 1e30f ? 0.5f / near : -1.f;
     }
-    __device__ __forceinline__ uint64_t near_zero(uint64_t x) const {
-        const uint64_t z = paged::mul2(x, x);
-        return paged::mul2(x, fma2(z, fma2(z, fma2(z, fma2(z, k[4], k[3]), k[2]), k[1]), k[0]));
-    }
+    // A hidden score: x p(x^2) is far below every other's, and finite where p is 1.
+    __device__ __forceinline__ float hidden(bool far) const { return far ? -1e18f : -1000.f * most; }
 };
 
 // ------------------------------------------------------------ roles
@@ -492,7 +495,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
     const int w = threadIdx.x >> 7, row = threadIdx.x & 127;
     const uint32_t lanes = uint32_t(row & ~31) << 16;
     const uint32_t t_s = tmem + w * 128 + lanes, t_o = tmem + 256 + w * D + lanes;
-    const float c = fabsf(p.scale) * kLog2e;   // of the scores, capped ones too, to units of log2
+    const float c = fabsf(p.scale) * kLog2e;   // of the scores to units of log2
     const Cap cap(fabsf(p.scale), CAP ? p.softcap : 1.f);
     unsigned done = 0, used = 0;   // phases of s_full passed; key tiles of the CTA before this item
     bool loaded = false;           // the item's query row is on its way
@@ -534,25 +537,31 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
             }
             const bool masked = __any_sync(0xffffffffu, limit < key0 + kKeys);
             const int lim = limit - key0;
+            float hidden = -INFINITY, k[5];
             if (CAP) {
                 if (masked) {   // whatever stands there must not look large
 #pragma unroll
                     for (int i = 0; i < 128; ++i) s[i] = i < lim ? s[i] : 0.f;
                 }
-                float far = 0.f;
+                float far4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 128; ++i) far = fmaxf(far, fabsf(s[i]));
-                if (__all_sync(0xffffffffu, far <= cap.most)) {
+                for (int i = 0; i < 128; i += 8) {
 #pragma unroll
-                    for (int i = 0; i < 128; i += 2) unpair(cap.near_zero(pair(s[i], s[i + 1])), s[i], s[i + 1]);
-                } else {
+                    for (int e = 0; e < 4; ++e) far4[e] = fmaxf(fmaxf(far4[e], fabsf(s[i + e])), fabsf(s[i + 4 + e]));
+                }
+                const float largest = fmaxf(fmaxf(far4[0], far4[1]), fmaxf(far4[2], far4[3]));
+                const bool far = !__all_sync(0xffffffffu, largest <= cap.most);
+                if (far) {
 #pragma unroll
                     for (int i = 0; i < 128; ++i) s[i] = fap::cap_score(s[i], cap.in, cap.out);
                 }
+#pragma unroll
+                for (int i = 0; i < 5; ++i) k[i] = far ? float(i == 0) : cap.k[i];
+                hidden = cap.hidden(far);
             }
             if (masked) {
 #pragma unroll
-                for (int i = 0; i < 128; ++i) s[i] = i < lim ? s[i] : -INFINITY;
+                for (int i = 0; i < 128; ++i) s[i] = i < lim ? s[i] : hidden;
             }
             float mx4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -561,13 +570,19 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
                 for (int e = 0; e < 4; ++e)
                     mx4[e] = i + 4 + e < 128 ? fmaxf(fmaxf(mx4[e], s[i + e]), s[i + 4 + e]) : fmaxf(mx4[e], s[i + e]);
             }
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+            float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));   // then in units of log2
+            if (CAP) {
+                const float z = mx * mx;
+                mx = mx == hidden ? -INFINITY : mx * fmaf(z, fmaf(z, fmaf(z, fmaf(z, k[4], k[3]), k[2]), k[1]), k[0]);
+            } else {
+                mx *= c;
+            }
             if (t == 0) {
                 m = mx;
             } else {
-                const bool rise = (mx - m) * c > kRise;
+                const bool rise = mx - m > kRise;
                 if (__any_sync(0xffffffffu, rise)) {
-                    const float a = rise ? paged::exp2_approx((m - mx) * c) : 1.f;
+                    const float a = rise ? paged::exp2_approx(m - mx) : 1.f;
                     if (rise) m = mx;
                     l *= a;
 #pragma unroll 1
@@ -592,7 +607,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
                 }
                 fence_async();
             }
-            const float base = m == -INFINITY ? 0.f : m * c;
+            const float base = m == -INFINITY ? 0.f : m;
             const uint64_t c2 = pair(c, c), b2 = pair(-base, -base);
             uint64_t sum[2] = {0, 0};
 #pragma unroll
@@ -602,8 +617,16 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
                     uint32_t pk[8];
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
+                        const uint64_t x = pair(s[i * 16 + e], s[i * 16 + e + 1]);
+                        uint64_t f = c2;
+                        if (CAP) {
+                            const uint64_t z = paged::mul2(x, x);
+                            f = pair(k[4], k[4]);
+#pragma unroll
+                            for (int n = 3; n >= 0; --n) f = fma2(z, f, pair(k[n], k[n]));
+                        }
                         float a, b;
-                        unpair(fma2(pair(s[i * 16 + e], s[i * 16 + e + 1]), c2, b2), a, b);
+                        unpair(fma2(x, f, b2), a, b);
                         a = paged::exp2_approx(a);
                         b = paged::exp2_approx(b);
                         sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair(a, b));
@@ -625,7 +648,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
         if (!warp_wait(&bars.s_full[w], done++ & 1, &bars.abort)) return;   // the accumulator is complete
         fence_after();
         const Row r(d, job, w, row);
-        const float base = m == -INFINITY ? -INFINITY : m * c;
+        const float base = m;
         const long long o_at = r.at(d, job, d.o_stride, D);
         auto write = [&](int i, float (&o)[32], float inv) {   // columns 32 i .. 32 i + 31 of the row
             if (!r.live) return;

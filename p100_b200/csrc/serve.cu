@@ -57,6 +57,7 @@ const char* paged_reason(const p100_paged_desc& in, paged::Desc& d) {
     if (in.dtype != P100_F16 && in.dtype != P100_BF16) return "dtype must be P100_F16 or P100_BF16";
     if (!std::isfinite(in.scale)) return "scale must be finite";
     if (!std::isfinite(in.softcap) || in.softcap < 0.0f) return "softcap must be finite and non-negative";
+    if (in.softcap > 1e15f) return "softcap must be at most 1e15";   // hidden scores are set to -1e18
     if ((long long)in.n_tokens * in.n_head_q > INT_MAX) return "n_tokens * n_head_q exceeds 2^31 - 1";
     if ((long long)in.max_pages * in.page_size > INT_MAX) return "max_pages * page_size exceeds 2^31 - 1";
     const long long D = in.head_dim;
