@@ -40,6 +40,7 @@ constexpr int kAhead = 4;          // vectors a thread has on their way
 constexpr int kGroups = 64, kGroup = kThreads / kGroups;   // groups of threads, each with a maximum
 constexpr int kMaxTop = 32;
 constexpr int kCand = 2048;       // candidates kept in shared memory, twice kMaxParts x kMaxTop
+constexpr int kRanked = 32;       // rounds of comparisons that ranking may take for each alternative
 constexpr int kMaxLogits = 1 << 24;
 constexpr int kMaxParts = 32;     // a lane each; parts x top <= kCand
 constexpr float kLog2e = 1.4426950408889634f;
@@ -249,19 +250,53 @@ struct Running {
     }
 };
 
-// The keys in s_key[0, count) ranked: the best `top` into best[0, top), zeros
-// behind them.  Every thread of the block calls it.
-__device__ __forceinline__ void rank_keys(const unsigned long long* s_key, int count, int top,
-                                          unsigned long long* best) {
-    for (int i = threadIdx.x; i < top; i += kThreads) best[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < count; i += kThreads) {
-        const unsigned long long k = s_key[i];
-        int r = 0;
-        for (int j = 0; j < count; ++j) r += s_key[j] > k;
-        if (r < top) best[r] = k;
+// The best `top` keys of those that each(take) gives to take() on every thread,
+// one after the other, into best[0, top), zeros behind them.  Every thread of
+// the block calls it.
+template <typename Each>
+__device__ __forceinline__ void pick_keys(int top, unsigned long long* best, unsigned long long* word, Each each) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    unsigned long long below = ~0ull;
+#pragma unroll 1
+    for (int k = 0; k < top; ++k) {
+        unsigned long long most = 0;
+        each([&](unsigned long long key) {
+            if (key < below && key > most) most = key;
+        });
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) {
+            const unsigned long long o = __shfl_xor_sync(0xffffffffu, most, off);
+            if (o > most) most = o;
+        }
+        if (lane == 0) word[warp] = most;
+        __syncthreads();
+        most = word[0];
+        for (int j = 1; j < kThreads / 32; ++j)
+            if (word[j] > most) most = word[j];
+        if (threadIdx.x == 0) best[k] = most;
+        below = most;
+        __syncthreads();
     }
-    __syncthreads();
+}
+// The same of the keys in s_key[0, count): ranked, every pair compared, or
+// picked where they are many (1000 keys, top 20: 62 us ranked, 17 picked).
+__device__ __forceinline__ void best_keys(const unsigned long long* s_key, int count, int top, unsigned long long* best,
+                                          unsigned long long* word) {
+    if (count * ((count + kThreads - 1) / kThreads) <= kRanked * top) {
+        for (int i = threadIdx.x; i < top; i += kThreads) best[i] = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < count; i += kThreads) {
+            const unsigned long long k = s_key[i];
+            int r = 0;
+            for (int j = 0; j < count; ++j) r += s_key[j] > k;
+            if (r < top) best[r] = k;
+        }
+        __syncthreads();
+    } else {
+        pick_keys(top, best, word, [&](auto take) {
+            for (int i = threadIdx.x; i < count; i += kThreads) take(s_key[i]);
+        });
+    }
 }
 
 // One part of a row, and where its vectors lie.
@@ -564,33 +599,14 @@ __global__ void __launch_bounds__(kThreads, kCtas) logprobs_kernel(const Params 
         if (tid < nsingle) keep(paged::to_float<T>(x[single]), single);
         __syncthreads();
         if (s_count <= kCand / 2) {
-            rank_keys(s_key, s_count, top, s_best);
+            best_keys(s_key, s_count, top, s_best, s_word);
         } else {
-            unsigned long long below = ~0ull;
-#pragma unroll 1
-            for (int k = 0; k < top; ++k) {
-                unsigned long long best = 0;
+            pick_keys(top, s_best, s_word, [&](auto take) {
                 for (int e = lo + tid; e < hi; e += kThreads) {
                     const float f = paged::to_float<T>(x[e]);
-                    if (f > -INFINITY) {
-                        const unsigned long long key = make_key(f, unsigned(e));
-                        if (key < below && key > best) best = key;
-                    }
+                    if (f > -INFINITY) take(make_key(f, unsigned(e)));
                 }
-#pragma unroll
-                for (int off = 16; off > 0; off >>= 1) {
-                    const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, off);
-                    if (o > best) best = o;
-                }
-                if (lane == 0) s_word[warp] = best;
-                __syncthreads();
-                best = s_word[0];
-                for (int j = 1; j < W; ++j)
-                    if (s_word[j] > best) best = s_word[j];
-                if (tid == 0) s_best[k] = best;
-                below = best;
-                __syncthreads();
-            }
+            });
         }
     }
 
@@ -646,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) logprobs_kernel(const Params 
             for (int k = tid; k < p.parts * top; k += kThreads)
                 if (s_key[k] != 0 && s_key[k] >= bound) kept[atomicAdd(&s_count, 1)] = s_key[k];
             __syncthreads();
-            rank_keys(kept, s_count, top, s_best);
+            best_keys(kept, s_count, top, s_best, s_word);
         }
     }
 

@@ -94,6 +94,18 @@ def test_ties_go_to_the_lowest_index(cuda, dtype):
     check(cuda, x, some_tokens(cuda, 6, 30011, 3), 32)
 
 
+@pytest.mark.parametrize("n", [33, 130, 600, 1025, 9000, 70001])
+@pytest.mark.parametrize("k", [1, 7, 32])
+def test_equal_logits(cuda, n, k):
+    """Equal rows, and rows with a finite value in their masked places: few to many candidates of one value."""
+    x = cuda.zeros(3, n, device="cuda")
+    x[1] = -1e4
+    x[1, 5:9] = 1.0
+    x[2, ::2] = 3.5
+    r = check(cuda, x, some_tokens(cuda, 3, n, 6), k)
+    assert r.top_index[0].tolist() == list(range(k))
+
+
 def test_masked_rows(cuda):
     """-inf, NaN and the type's lowest value; a row with nothing, one with one logit, fewer than top_k."""
     for dtype in ("float32", "float16", "bfloat16"):
