@@ -335,7 +335,7 @@ typedef struct p100_paged_desc {
     int dtype;          /* of q, the pages and o: P100_F16 or P100_BF16 */
     int page_size, n_pages, max_pages;   /* tokens a page, pages, table entries a sequence */
     float scale;        /* of the scores; 0 means 1/sqrt(head_dim) */
-    float softcap;      /* cap tanh(score / cap); 0 means off      */
+    float softcap;      /* cap tanh(score / cap), at most 1e15; 0 means off */
     int causal;         /* bottom-right alignment                  */
     int o_fp32;         /* o is fp32 (unrounded) instead of dtype  */
     /* Strides in elements, multiples of 8; 0 = contiguous pages of

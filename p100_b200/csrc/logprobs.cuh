@@ -12,19 +12,19 @@
 // largest value, and only a thread's eighth of the row whose maximum reaches it
 // can hold one of the k.  On random rows that is one to two times k eighths,
 // so the block reads just their vectors again (from L2), keeps the values that
-// reach the bound and ranks them by (value, lowest index).  Rows with more such values
-// than the buffer holds (long runs of equal logits) take k passes over the
-// part instead, each finding the largest key below the previous one.
+// reach the bound and ranks them by (value, lowest index).  Where many do (long
+// runs of equal logits) k passes over them, or over the part where they are
+// more than the buffer holds, each find the largest key below the previous one.
 //
 // Bytes bound it (the logits are read once); next come the exponentials, one a
 // logit, 0.7 of the time that 16-bit logits take to read.  So the rest is kept
 // small: 16-bit logits are masked, compared and counted two at a time before
 // their conversion, the sums run on pairs of FP32.  Few rows are split over
 // several CTAs; the last one of a row (an atomic ticket, no waiting) joins the
-// parts.  Measured: 2048 rows of 128256 bf16 with 8 alternatives 122 us (4.3
-// TB/s), without alternatives 111, the loads alone 88; one fp32 row with 20
-// alternatives 12 us.  128 threads and 8 CTAs an SM: 118 us against 131 of 256
-// threads and 4.
+// parts.  Measured: 2048 rows of 128256 bf16 with 8 alternatives 120 us (4.4
+// TB/s), the loads alone 88; one fp32 row with 20 alternatives 12 us; 333 rows
+// of 32003 fp32 with 32 alternatives 22.6 us.  128 threads and 8 CTAs an SM: 118
+// us against 131 of 256 threads and 4.
 #pragma once
 #include <type_traits>
 
@@ -214,8 +214,8 @@ struct Running {
         if (c > m) rise(c);
     }
     // N logits within the range of their type.  The difference comes first, exact
-    // or nearly: x log2 e - m log2 e in one fma would save an operation (2048
-    // rows 120 us, not 122) but puts the rounding of m log2 e, up to 2^-24 |m|,
+    // or nearly: x log2 e - m log2 e in one fma would save an operation (2 us of
+    // 2048 rows' 120) but puts the rounding of m log2 e, up to 2^-24 |m|,
     // into every term, which large or sharply peaked rows show.
     template <int N>
     __device__ __forceinline__ void add(const float (&f)[N]) {
