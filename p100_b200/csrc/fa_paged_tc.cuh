@@ -216,25 +216,21 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* a
 }
 
 // Capped scores, in units of log2: softcap log2 e tanh(y), y = scale / softcap
-// times the score x.  For |y| <= 1/2 that is x p(x^2), tanh(y) / y a polynomial
-// of degree 4 in y^2 fitted to the least relative error (7e-8 with FP32's
-// roundings); larger scores go through the special-function unit first (three
-// operations a score, which would bound the kernel) and then through the
-// polynomial 1, so that both take the same way to the probabilities.
+// times the score x.  For |y| <= 1/2 that is x p(x^2) with cap_score's polynomial.
+// A tile with larger scores goes through cap_score first (its special-function
+// operations would bound the kernel) and then through the polynomial 1, so that
+// both take the same way to the probabilities.
 struct Cap {
     float k[5];          // the coefficients of x^2
-    float in, out;       // cap_score's arguments
+    float near, out;     // cap_score's arguments
     float most;          // the largest |x| for the polynomial
     __device__ __forceinline__ Cap(float scale, float softcap) {
         constexpr float kLog2e = 1.4426950408889634f;
-        const float near = scale / softcap, n2 = near * near, n4 = n2 * n2, c = scale * kLog2e;
-        k[0] = c;
-        k[1] = -0.3333306908607483f * (c * n2);
-        k[2] = 0.13324779272079468f * (c * n4);
-        k[3] = -0.052986063063144684f * (c * n4) * n2;
-        k[4] = 0.017134996131062508f * (c * n4) * n4;
-        in = 2.f * scale * kLog2e / softcap;
+        near = fap::cap_near(scale, softcap);
         out = softcap * kLog2e;
+        float c = scale * kLog2e;
+#pragma unroll
+        for (int i = 0; i < 5; ++i, c = c * near * near) k[i] = fap::kTanh[i] * c;
         // elsewhere the powers would leave FP32's range
         most = near < 1e3f && k[4] > 1e-37f && k[4] < 1e30f ? 0.5f / near : -1.f;
     }
@@ -553,7 +549,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
                 const bool far = !__all_sync(0xffffffffu, largest <= cap.most);
                 if (far) {
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) s[i] = fap::cap_score(s[i], cap.in, cap.out);
+                    for (int i = 0; i < 128; ++i) s[i] = fap::cap_score(s[i], cap.near, cap.out);
                 }
 #pragma unroll
                 for (int i = 0; i < 5; ++i) k[i] = far ? float(i == 0) : cap.k[i];

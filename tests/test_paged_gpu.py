@@ -195,6 +195,19 @@ def test_softcap_scale_and_fp32_output(cuda, q_lens, kv_lens, page, dtype):
         check(cuda, b, *attend(b, q, **kw), attend64(b, q, **kw))
 
 
+@pytest.mark.parametrize("softcap", [1e-6, 1e-3, 0.5, 5.0, 100.0, 2000.0, 1e6])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1, 1], [700, 5, 0]), ([300, 1, 40], [900, 3, 20])])
+def test_caps_of_any_size(cuda, q_lens, kv_lens, softcap):
+    """Caps below, among and far above the scores, rows without a key.  The bound allows the cap's rounding 2^-20 of it,
+    except for the largest: cap tanh(x / cap) then differs from x by x^3 / (3 cap^2) < 1e-8, and no more is allowed."""
+    b = Batch(cuda, q_lens, kv_lens, 6, 2, 64, "bf16", 16)
+    b.fill()
+    q = b.queries(2.0)
+    for scale in (0.0, -0.2):
+        o, lse = attend(b, q, softcap=softcap, scale=scale, causal=True, o_fp32=True)
+        check(cuda, b, o, lse, attend64(b, q, scale, softcap if softcap < 1e6 else 0.0, True))
+
+
 @pytest.mark.parametrize("rows", [1, 130])
 def test_large_scores_and_rising_maxima(cuda, rows):
     """Scores whose maximum rises from tile to tile by far more than a rounding, and rows that one key decides."""
