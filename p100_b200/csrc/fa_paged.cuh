@@ -53,6 +53,35 @@ struct Params {
     float scale, softcap;
 };
 
+// Shares of a call's units on so many CTAs.  Every share has a unit, so every
+// CTA between a cut tile's first and last holds a part of it.
+__host__ __device__ __forceinline__ int shares(long long total, int ctas) {
+    const long long most = (total + kMinUnits - 1) / kMinUnits;
+    return most < ctas ? int(most) : ctas;
+}
+
+// How the parts of a row tile cut over the CTAs c0 .. c0 + np - 1 are joined: up
+// to kDirect of them by the last one to finish, more in groups of `per`, each by
+// its last one, and the groups by the last group's.  The parts of a group count
+// on the ticket of the CTA of its first part.  No other tile counts on that word:
+// a tile that is cut starts in c0, or has its first part in a CTA strictly
+// between this tile's first and last one, and those hold nothing else.  Hence a
+// group of one part takes no ticket: its CTA can be the tile's last, in which
+// the next cut tile may start.
+struct Joins {
+    int np, per, groups;
+    __host__ __device__ explicit Joins(int n) : np(n), per(n) {
+        if (np > kDirect) {
+            per = int(ceilf(sqrtf(float(np))));
+            if (per > kMaxJoin) per = kMaxJoin;
+        }
+        groups = (np + per - 1) / per;
+    }
+    __host__ __device__ int first_of(int part) const { return part / per * per; }
+    __host__ __device__ int size_of(int first) const { return per < np - first ? per : np - first; }
+    __host__ __device__ bool counts(int first) const { return size_of(first) > 1; }
+};
+
 // Without the lengths, which lie behind.
 template <int D>
 constexpr size_t smem_bytes() {
@@ -211,9 +240,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_kernel(const Params p) {
 
     paged::read_lengths<kRows, kKeys, kOver, kThreads, false>(d, len, 0);
     if (!len.head->ok) return;
-    // every share has a unit, so every CTA between a cut tile's first and last
-    // holds a part of it
-    const int parts = int(min((long long)gridDim.x, (len.head->total + kMinUnits - 1) / kMinUnits));
+    const int parts = shares(len.head->total, int(gridDim.x));
     if (int(blockIdx.x) >= parts) return;
     paged::Share<kRows, kKeys, kOver> share;
     share.begin(d, len, blockIdx.x, parts);
@@ -421,33 +448,30 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_kernel(const Params p) {
         }
         if (!whole) {
             const int c0 = paged::share_of(it.tile_first, len.head->total, parts);
-            const int np = paged::share_of(it.tile_first + it.units - 1, len.head->total, parts) - c0 + 1;
-            int per = np;   // parts of a group
-            if (np > kDirect) {
-                per = int(ceilf(sqrtf(float(np))));
-                per = min(per, kMaxJoin);
-            }
-            const int groups = (np + per - 1) / per;
-            const int group = (int(blockIdx.x) - c0) / per, first = group * per;
-            const int n = min(per, np - first);
+            const Joins joins(paged::share_of(it.tile_first + it.units - 1, len.head->total, parts) - c0 + 1);
+            const int first = joins.first_of(int(blockIdx.x) - c0), n = joins.size_of(first);
             __threadfence();
             __syncthreads();
-            if (tid == 0) s_last = atomicAdd(p.tickets + c0 + first, 1u) == unsigned(n - 1);
-            __syncthreads();
-            if (s_last) {
-                __threadfence();
-                if (tid == 0) p.tickets[c0 + first] = 0;   // ready for the next call
-                join_parts<T, D>(p, out, c0, first, 1, n, groups == 1, reinterpret_cast<float*>(s_kv));
-                if (groups > 1) {
+            bool last = true;
+            if (joins.counts(first)) {
+                if (tid == 0) s_last = atomicAdd(p.tickets + c0 + first, 1u) == unsigned(n - 1);
+                __syncthreads();
+                last = s_last;
+                if (last) {
                     __threadfence();
-                    __syncthreads();
-                    if (tid == 0) s_last = atomicAdd(p.tickets + gridDim.x + c0, 1u) == unsigned(groups - 1);
-                    __syncthreads();
-                    if (s_last) {
-                        __threadfence();
-                        if (tid == 0) p.tickets[gridDim.x + c0] = 0;
-                        join_parts<T, D>(p, out, c0, 0, per, groups, true, reinterpret_cast<float*>(s_kv));
-                    }
+                    if (tid == 0) p.tickets[c0 + first] = 0;   // ready for the next call
+                    join_parts<T, D>(p, out, c0, first, 1, n, joins.groups == 1, reinterpret_cast<float*>(s_kv));
+                    __threadfence();
+                }
+            }
+            if (last && joins.groups > 1) {
+                __syncthreads();
+                if (tid == 0) s_last = atomicAdd(p.tickets + gridDim.x + c0, 1u) == unsigned(joins.groups - 1);
+                __syncthreads();
+                if (s_last) {
+                    __threadfence();
+                    if (tid == 0) p.tickets[gridDim.x + c0] = 0;
+                    join_parts<T, D>(p, out, c0, 0, joins.per, joins.groups, true, reinterpret_cast<float*>(s_kv));
                 }
             }
         }

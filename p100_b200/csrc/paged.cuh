@@ -132,18 +132,18 @@ struct Lengths {                     // in shared memory, the arrays sized by n_
 };
 
 template <int ROWS>
-__device__ __forceinline__ int row_tiles(const Desc& d, int n) {
+__host__ __device__ __forceinline__ int row_tiles(const Desc& d, int n) {
     return int(((long long)n * d.group + ROWS - 1) / ROWS);
 }
 // Keys [0, key_end) are seen by some row of the tile.
 template <int ROWS>
-__device__ __forceinline__ int key_end(const Desc& d, int n, int kv, int tile) {
+__host__ __device__ __forceinline__ int key_end(const Desc& d, int n, int kv, int tile) {
     const int last = min((tile + 1) * ROWS, n * d.group) - 1;
     const int end = d.causal ? kv - n + last / d.group + 1 : kv;
     return max(0, min(end, kv));
 }
 template <int ROWS, int KEYS>
-__device__ __forceinline__ int tile_units(const Desc& d, int n, int kv, int tile) {
+__host__ __device__ __forceinline__ int tile_units(const Desc& d, int n, int kv, int tile) {
     return max(1, (key_end<ROWS>(d, n, kv, tile) + KEYS - 1) / KEYS);
 }
 
@@ -254,9 +254,14 @@ struct Item {
     long long tile_first;    // its first unit (cut)
 };
 
+// The first unit of share c of `parts`.
+__host__ __device__ __forceinline__ long long share_begin(long long total, int c, int parts) {
+    if (total < (1LL << 31) / parts) return unsigned(total) * unsigned(c) / unsigned(parts);   // a short division
+    return total * c / parts;
+}
 // The CTA whose share of `parts` holds unit u: the largest c with
-// total * c / parts <= u.
-__device__ __forceinline__ int share_of(long long u, long long total, int parts) {
+// share_begin(c) <= u.
+__host__ __device__ __forceinline__ int share_of(long long u, long long total, int parts) {
     if (total < (1LL << 31) / parts) return int((unsigned(u + 1) * unsigned(parts) - 1) / unsigned(total));
     return int(((u + 1) * parts - 1) / total);
 }
@@ -290,13 +295,8 @@ struct Share {
         round = 0;
         if (s.head->whole) return;
         const long long total = s.head->total;
-        if (total < (1LL << 31) / parts) {   // short divisions
-            at = unsigned(total) * unsigned(cta) / unsigned(parts);
-            end = unsigned(total) * unsigned(cta + 1) / unsigned(parts);
-        } else {
-            at = total * cta / parts;
-            end = total * (cta + 1) / parts;
-        }
+        at = share_begin(total, cta, parts);
+        end = share_begin(total, cta + 1, parts);
         if (at >= end) return;
         enter_seq(d, s, seq_of(d, s, at));
         const unsigned long long in_seq = (unsigned long long)at - s.first[seq];
