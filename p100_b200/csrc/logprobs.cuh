@@ -138,13 +138,15 @@ struct Vec16 {
         for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<const T2*>(&v[i]);
     }
     // Each pair's comparison is 0xffff in the half that holds; added up as one
-    // word, lo and hi of them make 65535 lo - 65536 hi modulo 2^32.
+    // word, lo and hi of them make 65535 lo - 65536 hi modulo 2^32.  counted()
+    // needs lo, hi < 2^16: a span has an eighth of that at most (a thread's whole
+    // row, 2^16 of each at kMaxLogits, would be too many).
     using Bound = T2;
     __device__ __forceinline__ void count(Bound ge, unsigned& n) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) n += __hge2_mask(h[i], ge);
     }
-    __device__ static __forceinline__ int counted(unsigned n) {   // lo, hi < 2^16: kMaxLogits
+    __device__ static __forceinline__ int counted(unsigned n) {
         const unsigned lo = -n & 0xffffu;
         return int(lo + ((lo - ((n + lo) >> 16)) & 0xffffu));
     }
@@ -347,11 +349,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) logprobs_kernel(const Params 
     __shared__ float s_bound;
     __shared__ float s_span[kSpans][kThreads];
     uint64_t(*s_save)[kThreads] = reinterpret_cast<uint64_t(*)[kThreads]>(s_key);   // a thread's state before a span
-    unsigned(*s_back)[kThreads] = reinterpret_cast<unsigned(*)[kThreads]>(s_key + 2 * kThreads);
+    float* s_back = reinterpret_cast<float*>(s_key + 2 * kThreads);
     __shared__ int s_above[W];
     __shared__ int s_count, s_hits, s_last;
     int* s_hit = reinterpret_cast<int*>(s_key + kCand / 2);   // spans to read again: kSpans x kThreads
     static_assert(kGroups == 64 && W == 4 && kMaxTop <= 32 && kMaxParts <= 32, "a lane for each alternative and part, 16 groups a warp");
+    static_assert(kMaxLogits / kThreads / kSpans / 2 < 1 << 16, "counts of a span");
     static_assert(kSpans * kThreads * sizeof(int) <= kCand / 2 * sizeof(unsigned long long), "spans beside half of the keys");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -379,7 +382,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) logprobs_kernel(const Params 
     }
 
     Running r;
-    unsigned reached = 0;
+    unsigned reached = 0;   // of the span
+    int above = 0;
     const typename Vec<T>::Bound bge = Vec<T>::bound(ge), bgt = Vec<T>::bound(gt);
     const uint4* v = reinterpret_cast<const uint4*>(x + vlo);
     auto take = [&](const uint4& q4, int i) {
@@ -457,26 +461,26 @@ __global__ void __launch_bounds__(kThreads, kCtas) logprobs_kernel(const Params 
             if (!masked) {
                 s_save[0][tid] = r.s2;
                 s_save[1][tid] = r.u2;
-                s_back[0][tid] = __float_as_uint(r.m);
-                s_back[1][tid] = reached;
+                s_back[tid] = r.m;
                 run(begin, end, std::false_type(), begin == 0);
             }
             if (masked || isnan(r.weighted())) {
                 if (!masked) {
                     r.s2 = s_save[0][tid];
                     r.u2 = s_save[1][tid];
-                    r.m = __uint_as_float(s_back[0][tid]);
+                    r.m = s_back[tid];
                     r.top = -3.402823466e38f;
-                    reached = s_back[1][tid];
+                    reached = 0;
                 }
                 run(begin, end, std::true_type(), false);
             }
         }
         s_span[span][tid] = r.top;
         best = fmaxf(best, r.top);
+        above += Vec<T>::counted(reached);
+        reached = 0;
     }
     r.top = best;
-    int above = Vec<T>::counted(reached);
     if (tid < nsingle) {
         const float f = paged::to_float<T>(x[single]);
         above += f >= (single < tok ? ge : gt);
