@@ -231,8 +231,9 @@ struct Cap {
         float c = scale * kLog2e;
 #pragma unroll
         for (int i = 0; i < 5; ++i, c = c * near * near) k[i] = fap::kTanh[i] * c;
-        // elsewhere the powers would leave FP32's range
-        most = near < 1e3f && k[4] > 1e-37f && k[4] < 1e30f ? 0.5f / near : -1.f;
+        // elsewhere the powers would leave FP32's range, or hidden()'s value, about
+        // -5e22 softcap, would not be far below every score
+        most = near < 1e3f && softcap > 1e-15f && k[4] > 1e-37f && k[4] < 1e30f ? 0.5f / near : -1.f;
     }
     // A hidden score: x p(x^2) is far below every other's, and finite where p is 1.
     __device__ __forceinline__ float hidden(bool far) const { return far ? -1e18f : -1000.f * most; }
