@@ -283,10 +283,11 @@ __device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tm
         if (p.box == 0) continue;   // the gathering warps load
         const int* table = d.block_table + (long long)it.seq * d.max_pages;
         auto find = [&](int t, int& page, int& off) {
-            const int key = (it.key_tile + t) * kKeys + i * p.box;
             page = -1;
             off = 0;
-            if (mine && t < it.count && key < end) {
+            if (!mine || t >= it.count) return;
+            const int key = (it.key_tile + t) * kKeys + i * p.box;
+            if (key < end) {
                 const int n = key / d.page_size;
                 off = key - n * d.page_size;
                 page = table[n];
@@ -516,8 +517,8 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
         loaded = false;
         const int limit = Row(d, job, w, row).limit;
         float m = -INFINITY, l = 0.f;
-        int key0 = job.key_tile * kKeys;
-        for (int t = 0; t < count; ++t, key0 += kKeys) {
+        for (int t = 0; t < count; ++t) {
+            const int key0 = (job.key_tile + t) * kKeys;   // key0 + kKeys may pass 2^31
             if (!warp_wait(&bars.s_full[w], done++ & 1, &bars.abort)) return;
             fence_after();
             float s[128];
@@ -532,8 +533,8 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
                     loaded = true;
                 }
             }
-            const bool masked = __any_sync(0xffffffffu, limit < key0 + kKeys);
             const int lim = limit - key0;
+            const bool masked = __any_sync(0xffffffffu, lim < kKeys);
             float hidden = -INFINITY, k[5];
             if (CAP) {
                 if (masked) {   // whatever stands there must not look large
@@ -593,10 +594,10 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
                     }
                 }
             }
-            if (w == 0 && key0 + kKeys > job.end) {   // rows of V that no key of the item's rows reaches
+            if (w == 0 && job.end - key0 < kKeys) {   // rows of V that no key of the item's rows reaches
                 const unsigned u = 2 * (used + t) + 1;
                 if (!warp_wait(&bars.full[u % NS], (u / NS) & 1, &bars.abort)) return;
-                if (key0 + row >= job.end) {
+                if (row >= job.end - key0) {
                     uint8_t* v = ring + (u % NS) * tile_bytes<D>() + row * 128;
 #pragma unroll
                     for (int i = 0; i < D / 8; ++i)

@@ -144,7 +144,7 @@ __host__ __device__ __forceinline__ int key_end(const Desc& d, int n, int kv, in
 }
 template <int ROWS, int KEYS>
 __host__ __device__ __forceinline__ int tile_units(const Desc& d, int n, int kv, int tile) {
-    return max(1, (key_end<ROWS>(d, n, kv, tile) + KEYS - 1) / KEYS);
+    return max(0, key_end<ROWS>(d, n, kv, tile) - 1) / KEYS + 1;   // of up to 2^31 - 1 keys
 }
 
 // Units of one kv head of a lane's sequence, every lane of the warp its own:

@@ -62,3 +62,11 @@ def test_no_word_or_place_is_shared(follow, ctas):
     if ctas >= 264:   # the sweep reaches what it is there for
         assert sum(r["grouped"] > 0 for r in rows) > 100 and sum(r["ones"] > 0 for r in rows) > 20
         assert sum(r["followed"] > 0 for r in rows) > 0
+
+
+def test_lengths_near_the_largest(follow):
+    """A length next to 2^31 is cut over every CTA like any other."""
+    rows = follow([(ctas, kernel, True, 1, 4, [(n, 2 ** 31 - back)]) for back in (1, 19, 64, 127, 128, 1000)
+                   for kernel, ctas, n in ((0, 296, 1), (1, 148, 5))])
+    for r, ctas in zip(rows, [296, 148] * 6):
+        assert (r["cut"], r["most"], r["shared"], r["empty"]) == (1, ctas, 0, 0)
