@@ -446,6 +446,16 @@ def _pages_of(k_pages, v_pages, dev, desc):
     need = (n - 1) * page + (heads - 1) * head + (size - 1) * token + d if n > 0 else 0
     for t, what in ((k_pages, "k_pages"), (v_pages, "v_pages")):
         _need(t, what, dev, dtype, dense=False)
+        # a tensor whose sizes name its axes must have the descriptor's strides in their order
+        shape, strides = t.shape, t.stride()
+        if shape == (n, heads, size, d) and strides == (page, head, token, 1):
+            continue
+        orders = [steps for order, steps in (((heads, size, d), (page, head, token, 1)),
+                                             ((size, heads, d), (page, token, head, 1)),
+                                             ((size, d) if heads == 1 else None, (page, token, 1))) if order == shape[1:]]
+        if orders and not any(all(a == b or m == 1 for m, a, b in zip(shape, strides, steps)) for steps in orders):
+            raise InvalidArgument(ERR_INVALID, f"{what} {list(shape)} has strides {strides}, the descriptor {page} "
+                                               f"between pages, {head} between heads, {token} between tokens")
         if t.numel() >= need and t.is_contiguous():
             continue
         have = t.untyped_storage().nbytes() // 2 - t.storage_offset()
@@ -467,7 +477,9 @@ def paged_append(desc, qkv, block_table, q_start, kv_len, k_pages, v_pages, rope
                  eps=1e-5, rope_half=False, q=None, stream=None):
     """New tokens into a paged cache (p100_paged_append): per-head norms and rotation of the fused rows qkv
     [n_tokens, (n_head_q + 2 n_head_kv) head_dim] (float32, float16 or bfloat16), k and v to their pages, the
-    queries returned as q [n_tokens, n_head_q, head_dim] of the cache's type."""
+    queries returned as q [n_tokens, n_head_q, head_dim] of the cache's type.  Pages [n_pages, n_head_kv, page_size,
+    head_dim] or [n_pages, page_size, n_head_kv, head_dim] must have the descriptor's strides in that order; of a tensor
+    of other sizes the descriptor's alone count."""
     torch = _torch()
     dev = torch.cuda.current_device()
     width = (desc.n_head_q + 2 * desc.n_head_kv) * desc.head_dim
