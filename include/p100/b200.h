@@ -372,12 +372,14 @@ p100_status p100_fa_paged_workspace_init(void* ws, size_t ws_bytes, p100_stream_
 /* Attention of the new tokens over their sequences' cached tokens, their own
  * (appended before) among them: query head h reads kv head h / (n_head_q /
  * n_head_kv); with causal, new token i of n sees keys [0, kv_len - n + i],
- * without it all kv_len.  Scores, softmax statistics and sums are FP32; the
- * probabilities are rounded once to dtype for the product with V.  A row that
- * sees no key gives o = 0 and lse = -inf.  Within [0, kv_len), values that
- * are not finite reach the rows whose tile holds them even where causal hides
- * them.  lse [n_tokens][n_head_q] (natural log) may be NULL; o must not overlap
- * q.  Sequences may share pages.
+ * without it all kv_len.  Scores, softmax statistics and sums are FP32.  For
+ * the product with V a call of at most 16 rows a sequence (max_q x n_head_q /
+ * n_head_kv) carries each probability in two parts of dtype, 2^-16 (bfloat16)
+ * or 2^-22 off; others round it once to dtype.  A row that sees no key gives o =
+ * 0 and lse = -inf.  Within [0, kv_len), values that are not finite reach the
+ * rows whose tile holds them even where causal hides them.  lse
+ * [n_tokens][n_head_q] (natural log) may be NULL; o must not overlap q.
+ * Sequences may share pages.
  * Results do not depend on the order in which blocks run. */
 p100_status p100_fa_paged(const p100_paged_desc* desc, const void* q, const void* k_pages, const void* v_pages,
                           const int* block_table, const int* q_start, const int* kv_len, void* o, float* lse, void* ws,

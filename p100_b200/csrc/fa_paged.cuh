@@ -11,8 +11,16 @@
 // copies (any page size; a row's page is looked up two tiles ahead), swizzled
 // so that ldmatrix reads without bank conflicts; rows behind kv_len are filled
 // with zeros, so what a page holds there never reaches a product.  Statistics
-// and accumulators are FP32; the probabilities are rounded once to the cache's
-// 16-bit type, as the tensor cores take them.
+// and accumulators are FP32.
+//
+// The tensor cores take 16-bit probabilities.  Each goes in two parts, rounded
+// to nearest: the probability and what that rounding left of it, so a product
+// loses 2^-16 (bfloat16) or 2^-22 of it and an FP32 output has the digits of
+// FP32 probabilities.  Where a kv head has 8 rows or fewer (SPARE) the second
+// parts are the upper 8 rows of the same products and are added to the lower
+// ones at the end, at no cost (64 sequences up to 8192 tokens: 0.997 of the time
+// with one part); else they take products of their own (1.03 of it with 16
+// rows).  In FP16 the largest probability is 2^15, see kLift.
 //
 // HBM bytes bound it: K and V are read once per row tile.  A row tile cut by
 // the shares leaves its partials {m, l, unnormalised o} in the workspace and
@@ -23,6 +31,8 @@
 // bandwidth (293 us with one CTA an SM); one of 4096 tokens (32 / 8 heads) 14.4
 // us, of which the copies take 2.
 #pragma once
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace p100b {
@@ -40,6 +50,13 @@ constexpr int kOffs = 5;   // tiles whose row offsets are held
 constexpr int kDirect = 48;   // parts that one CTA joins (two levels cost 2.4 us more than one of 37 parts)
 constexpr int kMaxJoin = 48;  // at most so many in one join
 constexpr int kMinUnits = 2;  // of a share, where there is less work than CTAs (one of 4096: 18.4 us, with 4 or 8 20.5)
+
+// log2 of the largest probability before the normalisation: FP16 holds nothing
+// below 2^-25, and the many keys that a long context has there can weigh more
+// than a rounding of the output.  The statistics m are that much below the
+// maximum.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 15.f : 0.f;
 
 struct Params {
     Desc d;
@@ -224,7 +241,7 @@ __device__ __forceinline__ void join_parts(const Params& p, const Out& out, int 
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool SPARE>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_kernel(const Params p) {
     extern __shared__ __align__(128) uint8_t smem[];
     constexpr int kRowBytes = D * 2;
@@ -344,40 +361,56 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_kernel(const Params p) {
                 }
             }
             const int key0 = (it.key_tile + t) * kKeys + warp * 16 + cq;   // this lane's first column
+            // Row g + 8 h: its probabilities, rounded (high, of both blocks of 8
+            // keys) and what the rounding left (rest); the factor of its sums so far.
+            auto softmax = [&](int h, uint32_t (&high)[2], uint32_t (&rest)[2]) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x = p.softcap != 0.f ? cap_score(s[j][e], cap_in, p.softcap * kLog2e) : s[j][e] * to_log2;
-                    s[j][e] = key0 + j * 8 + (e & 1) < limit[e >> 1] ? x : -INFINITY;
-                }
-            uint32_t pf[4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
+                    for (int e = 2 * h; e < 2 * h + 2; ++e) {
+                        float x = p.softcap != 0.f ? cap_score(s[j][e], cap_in, p.softcap * kLog2e) : s[j][e] * to_log2;
+                        s[j][e] = key0 + j * 8 + (e & 1) < limit[h] ? x : -INFINITY;
+                    }
                 float mx = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float mn = fmaxf(m[h], mx);
+                const float mn = fmaxf(m[h], mx - kLift<T>);
                 const float base = mn == -INFINITY ? 0.f : mn;
                 const float a = paged::exp2_approx(m[h] - base);
                 m[h] = mn;
                 float sum = 0.f;
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        s[j][2 * h + e] = paged::exp2_approx(s[j][2 * h + e] - base);
-                        sum += s[j][2 * h + e];
-                    }
-                l[h] = l[h] * a + sum;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    acc[i][2 * h] *= a;
-                    acc[i][2 * h + 1] *= a;
+                for (int j = 0; j < 2; ++j) {
+                    const float p0 = paged::exp2_approx(s[j][2 * h] - base), p1 = paged::exp2_approx(s[j][2 * h + 1] - base);
+                    sum += p0;
+                    sum += p1;
+                    float h0, h1;
+                    high[j] = paged::pack2<T>(p0, p1);
+                    paged::unpack2<T>(high[j], h0, h1);
+                    rest[j] = paged::pack2<T>(p0 - h0, p1 - h1);
                 }
-                pf[h] = paged::pack2<T>(s[0][2 * h], s[0][2 * h + 1]);
-                pf[2 + h] = paged::pack2<T>(s[1][2 * h], s[1][2 * h + 1]);
+                l[h] = l[h] * a + sum;
+                return a;
+            };
+            uint32_t pf[4], pr[4];   // probabilities of rows g and g + 8, what their rounding left
+            float a[2];
+            {
+                uint32_t high[2], rest[2];
+                a[0] = a[1] = softmax(0, high, rest);
+                pf[0] = high[0], pf[2] = high[1];
+                if (SPARE) {
+                    pf[1] = rest[0], pf[3] = rest[1];
+                } else {
+                    pr[0] = rest[0], pr[2] = rest[1];
+                    a[1] = softmax(1, high, rest);
+                    pf[1] = high[0], pf[3] = high[1];
+                    pr[1] = rest[0], pr[3] = rest[1];
+                }
             }
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][e] *= a[e >> 1];
             {
                 // matrices 0/1: dims 0-7 of keys 0-7 and 8-15; 2/3: dims 8-15
                 const int key = warp * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
@@ -388,11 +421,19 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_kernel(const Params p) {
                     ldsm4_t(row + (((2 * i + (lane >> 4)) ^ (key & 7)) << 4), b);
                     mma16<T>(acc[2 * i], pf, b[0], b[1]);
                     mma16<T>(acc[2 * i + 1], pf, b[2], b[3]);
+                    if (!SPARE) {
+                        mma16<T>(acc[2 * i], pr, b[0], b[1]);
+                        mma16<T>(acc[2 * i + 1], pr, b[2], b[3]);
+                    }
                 }
             }
             if (tid < kKeys) s_off[(ahead % kOffs) * kKeys + tid] = next_off;
         }
 
+        if (SPARE) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) acc[i][0] += acc[i][2], acc[i][1] += acc[i][3];
+        }
         // Join the warps: statistics, then the accumulators added in warp order.
         cp_wait<0>();
         __syncthreads();

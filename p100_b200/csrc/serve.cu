@@ -168,16 +168,25 @@ p100_status launch_fa_paged_tc_d(const fatc::Params& prm, int head_dim, const CU
                : launch_fa_paged_tc<T, 128, false>(prm, tmk, tmv, sms, s);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool SPARE>
 p100_status launch_fa_paged_mma(const fap::Params& prm, int sms, cudaStream_t stream) {
     static thread_local int configured[64] = {};
-    auto kern = fap::fa_paged_kernel<T, D>;
+    auto kern = fap::fa_paged_kernel<T, D, SPARE>;
     constexpr size_t fixed = fap::smem_bytes<D>();
     if (p100_status st = allow_smem(kern, fixed + paged::Lengths::bytes(paged::kMaxSeq), configured,
                                     "cudaFuncSetAttribute(fa_paged)"))
         return st;
     kern<<<sms * kMmaCtas, fap::kThreads, fixed + paged::Lengths::bytes(prm.d.n_seq), stream>>>(prm);
     return cuda_status(cudaGetLastError(), "fa_paged_kernel launch");
+}
+
+template <typename T>
+p100_status launch_fa_paged_mma_d(const fap::Params& prm, int head_dim, int sms, cudaStream_t s) {
+    // 8 rows a kv head or fewer: the second parts of their probabilities take the other 8
+    const bool spare = (long long)prm.d.max_q * prm.d.group <= fap::kRows / 2;
+    if (head_dim == 64)
+        return spare ? launch_fa_paged_mma<T, 64, true>(prm, sms, s) : launch_fa_paged_mma<T, 64, false>(prm, sms, s);
+    return spare ? launch_fa_paged_mma<T, 128, true>(prm, sms, s) : launch_fa_paged_mma<T, 128, false>(prm, sms, s);
 }
 
 template <typename S, typename T>
@@ -382,11 +391,8 @@ p100_status p100_fa_paged(const p100_paged_desc* desc, const void* q, const void
         return desc->dtype == P100_F16 ? launch_fa_paged_tc_d<__half>(t, desc->head_dim, tmk, tmv, sms, stream)
                                        : launch_fa_paged_tc_d<__nv_bfloat16>(t, desc->head_dim, tmk, tmv, sms, stream);
     }
-    if (desc->dtype == P100_F16)
-        return desc->head_dim == 64 ? launch_fa_paged_mma<__half, 64>(prm, sms, stream)
-                                    : launch_fa_paged_mma<__half, 128>(prm, sms, stream);
-    return desc->head_dim == 64 ? launch_fa_paged_mma<__nv_bfloat16, 64>(prm, sms, stream)
-                                : launch_fa_paged_mma<__nv_bfloat16, 128>(prm, sms, stream);
+    return desc->dtype == P100_F16 ? launch_fa_paged_mma_d<__half>(prm, desc->head_dim, sms, stream)
+                                   : launch_fa_paged_mma_d<__nv_bfloat16>(prm, desc->head_dim, sms, stream);
 }
 
 size_t p100_logprobs_workspace_size(int rows, int n, int dtype, int top_k) {
