@@ -11,8 +11,10 @@
 //                   lane): the query rows into shared memory; per key tile the
 //                   128 scores of the row from tensor memory into registers,
 //                   running maximum and sum in FP32, the probabilities rounded
-//                   to the cache's 16-bit type into tensor memory, in the
-//                   scores' place; at the end the accumulator, normalised
+//                   once to the cache's 16-bit type (a second part, as in
+//                   fa_paged.cuh, would be half as many products again, which
+//                   bound this kernel) into tensor memory, in the scores'
+//                   place; at the end the accumulator, normalised
 //   warp 8          issues every tcgen05.mma: S = Q K^T (both from shared
 //                   memory, K-major, 128-byte swizzle) and O += P V (P from
 //                   tensor memory, V as it lies, N-major), M = 128 rows
@@ -24,7 +26,7 @@
 //
 // The accumulator is rescaled only when a row's maximum has risen by more
 // than 2^8 since the reference it uses (the probabilities then stay below 2^8,
-// exact in scale in either 16-bit type); the row's thread does it in place,
+// in FP16, whose reference is taken lower, below 2^15); the row's thread does it in place,
 // between the product that the scores' arrival proves finished and the next.
 // Rows of V behind the last visible key are zeroed in shared memory before
 // their product, so what a page holds there reaches nothing.
@@ -66,6 +68,11 @@ constexpr int kSoftmaxRegs = 192, kIssueRegs = 120;
 static_assert(256 * kSoftmaxRegs + 128 * kIssueRegs <= kThreads * 168, "register split");
 constexpr int kSub = 128 * 128;           // bytes of 128 rows x 64 values
 constexpr float kRise = 8.0f;             // log2 of the rise that forces a rescale
+// The reference lies that far below the maximum it was taken from, so that FP16
+// probabilities stay below 2^15 and what it cannot hold of them, 2^-25, is below
+// 2^-32 of the row's largest: many keys of a long context may lie there.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 15.f - kRise : 0.f;
 
 template <int D>
 __host__ __device__ constexpr int slots() { return D == 128 ? 4 : 8; }
@@ -575,6 +582,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
             } else {
                 mx *= c;
             }
+            mx -= kLift<T>;
             if (t == 0) {
                 m = mx;
             } else {

@@ -4,7 +4,8 @@ Bound of o: (rel + 2 e + 2^-18) sum p |v| + tail sum |v| + 2^-24 with e, 2^-18 a
 what is lost of a probability relative to it, `tail` what a small one loses of the row's largest.
 
 Single tokens carry a probability in two 16-bit parts, each rounded to nearest: rel = u^2 (2^-16 in bfloat16, 2^-22 in
-float16).  In float16 the largest is 2^15 and nothing below 2^-25 is held, so tail = 2^-40; bfloat16 has FP32's range."""
+float16).  In float16 the largest is 2^15 and nothing below 2^-25 is held, so tail = 2^-40; bfloat16 has FP32's range.
+Chunks round a probability once, rel = u; in float16 the largest is 2^7 or more, so tail = 2^-32."""
 import math
 
 import pytest
@@ -72,3 +73,11 @@ def test_far_tails_of_single_tokens(cuda, dtype, group):
     o, _ = attend(b, q, o_fp32=True)
     assert 1e-3 < float(o.min()) and float(o.max()) < 2e-3
     check64(cuda, b, q, o, *kept(cuda, b))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_far_tails_of_chunks(cuda, dtype):
+    b, q = far_tail(cuda, [40, 9], 65536, dtype)
+    o, _ = attend(b, q, o_fp32=True)
+    assert 1e-3 < float(o.min()) and float(o.max()) < 2e-3
+    check64(cuda, b, q, o, cuda.finfo(b.t).eps / 2, 2.0 ** -32 if dtype == "f16" else 0.0)
