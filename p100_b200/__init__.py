@@ -75,7 +75,8 @@ class AttnDesc(C.Structure):
 
 
 class PagedDesc(C.Structure):
-    """p100_paged_desc: new tokens of a batch of sequences and their paged K/V cache."""
+    """p100_paged_desc: new tokens of a batch of sequences and their paged K/V cache.  max_q = 0 stands for n_tokens; a
+    batch that decodes one token each should say 1 (by default it takes 1.6 to 1.9 times the time)."""
     _fields_ = [("n_seq", C.c_int), ("n_tokens", C.c_int), ("max_q", C.c_int), ("n_head_q", C.c_int),
                 ("n_head_kv", C.c_int), ("head_dim", C.c_int), ("dtype", C.c_int), ("page_size", C.c_int),
                 ("n_pages", C.c_int), ("max_pages", C.c_int), ("scale", C.c_float), ("softcap", C.c_float),

@@ -27,9 +27,9 @@
 // its last CTA (an atomic ticket, no waiting) joins them in share order; more
 // than kDirect parts are joined in groups first, each by its last CTA, so that
 // no CTA reads more than about the square root of their number.  Measured: 64
-// sequences up to 8192 tokens (64 / 8 heads of 128) 190 us, 0.98 of measured
-// bandwidth (293 us with one CTA an SM); one of 4096 tokens (32 / 8 heads) 14.4
-// us, of which the copies take 2.
+// sequences up to 8192 tokens (64 / 8 heads of 128) 190 us in graph replays, 0.98
+// of measured bandwidth (293 us with one CTA an SM); one of 4096 tokens (32 / 8
+// heads) 14 us, of which the copies take 2.
 #pragma once
 #include <type_traits>
 

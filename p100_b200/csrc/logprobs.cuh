@@ -21,8 +21,8 @@
 // small: 16-bit logits are masked, compared and counted two at a time before
 // their conversion, the sums run on pairs of FP32.  Few rows are split over
 // several CTAs; the last one of a row (an atomic ticket, no waiting) joins the
-// parts.  Measured: 2048 rows of 128256 bf16 with 8 alternatives 120 us (4.4
-// TB/s), the loads alone 88; one fp32 row with 20 alternatives 12 us; 333 rows
+// parts.  Measured: 2048 rows of 128256 bf16 with 8 alternatives 116 to 126 us
+// (4.2 to 4.5 TB/s), the loads alone 88; one fp32 row with 20 alternatives 12 us; 333 rows
 // of 32003 fp32 with 32 alternatives 22.6 us.  128 threads and 8 CTAs an SM: 118
 // us against 131 of 256 threads and 4.
 #pragma once

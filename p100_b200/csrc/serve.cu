@@ -93,6 +93,8 @@ static_assert(paged::kMaxSeq == P100_PAGED_MAX_SEQ, "lengths in shared memory");
 
 // The tensor-core kernel takes calls in which a sequence may have more rows
 // (new tokens x query heads per kv head) than the mma.sync kernel's row tile.
+// One token each of 64 sequences of 8192 (64 / 8 heads): 245 us on the mma.sync
+// kernel, 396 on the other; of 16 sequences (12 / 4 heads of 64) 31 and 59.
 bool fa_paged_on_tc(const paged::Desc& d) { return (long long)d.max_q * d.group > fap::kRows && d.n_pages > 0; }
 
 // Units of a sequence's kv head are counted in 32 bits.
@@ -213,7 +215,11 @@ const char* logprobs_reason(int rows, int n, int dtype, int top_k) {
     return nullptr;
 }
 // Parts of a row: as many CTAs as the device holds at once, each with two
-// vectors or more for every thread.
+// vectors or more for every thread.  The quotient is rounded down, so a row count
+// just above a divisor of the device's places leaves some of them empty, and one
+// just above all of them starts a second wave.  128256 bf16 logits with 8
+// alternatives: 394 rows (3 parts) 34.6 us, 395 (2) 36.9; 592 (2) 45.9, 593 (1)
+// 48.5; 1184 68.3, 1185 (second wave) 84.6.
 int logprobs_parts(int rows, int n, int dtype, int sms) {
     const long long vec = 16 / (long long)dtype_bytes(dtype);
     const long long most = std::min<long long>(lp::kMaxParts, n / (2 * vec * lp::kThreads));
