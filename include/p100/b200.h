@@ -358,9 +358,9 @@ typedef struct p100_paged_desc {
  * rope_cs[position] (p100_rope_table's layout; NULL: no rotation; rope_half
  * == 0 pairs values 2i and 2i + 1, != 0 values i and i + head_dim / 2), the v
  * heads as they are; q to q, k and v to their row in the pages.  FP32
- * arithmetic, one rounding (nearest even) to dtype.  A token whose position
- * lies outside [0, max_pos) of the table or outside the block table is left
- * out and raises P100_ERR_INVALID in p100_device_error(). */
+ * arithmetic, one rounding (nearest even) to dtype.  Neither q nor the pages
+ * may overlap qkv.  A token whose position lies outside [0, max_pos) of the table
+ * or outside the block table is left out and raises P100_ERR_INVALID in p100_device_error(). */
 p100_status p100_paged_append(const p100_paged_desc* desc, const void* qkv, int qkv_type, long long qkv_stride,
                               const float* q_norm, const float* k_norm, float eps, const float* rope_cs, int max_pos,
                               int rope_half, const int* block_table, const int* q_start, const int* kv_len, void* q,
