@@ -86,3 +86,34 @@ def test_parts_of_chunks(cuda):
     first = serve(cuda, b, q, want, ws)
     again = serve(cuda, b, q, want, ws)
     assert all(cuda.equal(x, y) for x, y in zip(first, again))
+
+
+def test_replayed_with_other_lengths_beside_another_call(cuda):
+    """A captured call of several levels whose lengths change between replays, while another stream runs the same
+    sequences with a workspace of its own."""
+    torch = cuda
+    heads, lens = FOLLOWED[0]
+    b, q = batch(torch, lens, heads, 8, "f16", 128, 64, 3)
+    ws, other = workspace(b), workspace(b)
+    o = torch.empty((b.n_tokens, b.hq, b.dim), dtype=b.t, device="cuda")
+    lse = torch.empty((b.n_tokens, b.hq), device="cuda")
+    o2, lse2 = torch.empty_like(o), torch.empty_like(lse)
+    args = (b.desc(), q, b.k, b.v, b.table, b.q_start, b.kv_len)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        P.fa_paged(*args, o=o, lse=lse, ws=ws)
+    side = torch.cuda.Stream()
+    for kv in (lens, [lens[0] - 64, 200], [9000, 1], lens):
+        b.kv_lens = kv
+        b.kv_len.copy_(torch.tensor(kv, dtype=torch.int32))
+        want = attend64(b, q)
+        for x in (o, lse, o2, lse2):
+            x.fill_(math.nan)
+        torch.cuda.synchronize()
+        for _ in range(10):
+            graph.replay()
+            P.fa_paged(*args, o=o2, lse=lse2, ws=other, stream=side)
+        torch.cuda.synchronize()
+        P.check(P.device_error())
+        check(torch, b, o, lse, want)
+        assert torch.equal(o, o2) and torch.equal(lse, lse2)
