@@ -410,6 +410,122 @@ p100_status p100_logprobs(const void* logits, int dtype, int n, int rows, long l
                           int top_k, float* logprob, float* entropy, int* rank, int* top_index, float* top_logprob,
                           void* ws, size_t ws_bytes, p100_stream_t stream);
 
+/* ------------------------------------------- paged cache: steps and drafted trees */
+/* A step of decoding with drafted tokens, without the host knowing a length:
+ * p100_paged_plan gives the new tokens their pages, starts, slots and positions,
+ * p100_tree_mask turns the drafts' parents into masks and positions, then in
+ * every layer p100_paged_append_rope and p100_fa_tree; when the caller has
+ * chosen the tokens to keep, p100_paged_keep moves their rows in every layer,
+ * and the next plan starts from the lengths it returns.  No reference
+ * counterpart.  Everything about a request is int32 in device memory and read
+ * when the kernels run, so one captured graph serves all steps. */
+
+/* The plan of a step.  Request s has length[s] tokens that stay and n_new[s]
+ * to come (a draft, a chunk, 0): kv_len[s] = length[s] + n_new[s], q_start [n_seq
+ * + 1] the running sum of n_new from 0.  The request's first held[s] table
+ * entries are its pages; entries that kv_len does not need go back to the pool
+ * (set to -1) and missing ones are taken from it, so length 0 with n_new 0 ends a
+ * request, and a call repeated with the same lengths changes nothing.  Pages
+ * given back are on top: a call undone by the next one's lengths leaves pool
+ * and table as they were.
+ * Of new token t: position[t] = length + its index, slot[t] = page x page_size +
+ * row, the cache row that p100_paged_append gives it; rows from q_start[n_seq] to
+ * n_tokens get -1.  slot (int64) and position may each be NULL.
+ * pool: 2 + n_pages ints: the number of free pages, how many were missing, and
+ * the free pages themselves, the next one last.  Too few free pages: pool[1] says
+ * how many are missing, no page moves, q_start is all 0 (the step's kernels do
+ * nothing), kv_len = length.  The same with pool[1] = -1 and P100_ERR_INVALID in
+ * p100_device_error() for negative lengths, more than max_pages pages a request,
+ * more than n_tokens new tokens, or counts that do not fit the pool.
+ * Of desc it uses n_seq, n_tokens, page_size, n_pages and max_pages.  Calls on
+ * one pool are ordered by the caller; no two arrays may overlap. */
+p100_status p100_paged_plan(const p100_paged_desc* desc, const int* length, const int* n_new, int* pool, int* held,
+                            int* block_table, int* q_start, int* kv_len, long long* slot, int* position,
+                            p100_stream_t stream);
+/* A pool with every page free and requests that hold none (table entries -1). */
+p100_status p100_paged_pool_init(const p100_paged_desc* desc, int* pool, int* held, int* block_table,
+                                 p100_stream_t stream);
+
+#define P100_TREE_MAX_WORDS 32   /* a tree has at most 1024 tokens */
+/* The masks and positions of drafted trees.  New token i of a sequence hangs
+ * on its new token parent (parent[q_start + i], below i) or, with -1, on the last
+ * token before the new ones; it sees its ancestors and itself: bit j % 32 of
+ * mask[token * mask_words + j / 32] says that it sees new token j.  position =
+ * kv_len - n + its depth (may be NULL).  A sequence with more than 32
+ * mask_words new tokens, fewer tokens in all than new ones or tokens behind
+ * n_tokens is left out, a parent out of order counts as -1; both raise
+ * P100_ERR_INVALID in p100_device_error(). */
+p100_status p100_tree_mask(const int* parent, const int* q_start, const int* kv_len, int n_seq, int n_tokens,
+                           int mask_words, unsigned* mask, int* position, p100_stream_t stream);
+
+/* Rotary frequencies: pair i of rope_dim / 2 turns by theta^(-2i / rope_dim)
+ * radians a token, scaled for contexts longer than the model was trained on. */
+typedef enum p100_rope_kind {
+    P100_ROPE_NONE = 0,
+    P100_ROPE_LINEAR = 1,    /* divided by factor */
+    P100_ROPE_NTK = 2,       /* theta times factor^(rope_dim / (rope_dim - 2)) */
+    P100_ROPE_BANDS = 3,     /* by the turns t = original f / 2 pi: f / factor below low turns, f above high,
+                                between them w f + (1 - w) f / factor, w = (t - low) / (high - low) */
+    P100_ROPE_YARN = 4,      /* f / factor r + f (1 - r): r rises from 0 at pair floor(d(high)) to 1 at ceil(d(low)),
+                                both kept in [0, rope_dim - 1], d(b) = rope_dim ln(original / (2 pi b)) / (2 ln
+                                theta); mscale 0 means 0.1 ln(factor) + 1 (1 for factors up to 1) */
+    P100_ROPE_DIVISORS = 5   /* f / divisors[i] */
+} p100_rope_kind;
+typedef struct p100_rope_scaling {
+    int kind;                /* p100_rope_kind */
+    int original;            /* tokens of the trained context (BANDS, YARN) */
+    double factor;           /* LINEAR, NTK, BANDS, YARN */
+    double low, high;        /* BANDS: turns; YARN: slow and fast turns (commonly 1 and 32) */
+    double mscale;             /* factor of the rotated values; 0 means 1 (YARN: see above) */
+    const double* divisors;  /* DIVISORS: rope_dim / 2 of them, host memory */
+} p100_rope_scaling;
+/* What p100_rope_init makes of them; a plain value that calls copy. */
+typedef struct p100_rope {
+    int rope_dim;            /* the first values of a head that turn: even, at most head_dim */
+    int half;                /* 0: pairs of values 2i, 2i + 1; else i, i + rope_dim / 2 */
+    float mscale;
+    int reserved;            /* 0 */
+    unsigned long long turns[64];   /* of a token, in units of 2^-64 turn */
+} p100_rope;
+/* Host: fills *rope.  scaling NULL: unscaled. */
+p100_status p100_rope_init(p100_rope* rope, int rope_dim, int half, double theta, const p100_rope_scaling* scaling);
+/* p100_paged_append with the first rope_dim values of each q and k head rotated
+ * by rope's frequencies at position[token] (NULL: the token's own position in its
+ * sequence, where its row in the cache is in any case): angles to 2^-24 of a
+ * half turn at every position up to 2^31 - 1, without a table.  The other values
+ * of a head are kept.  mscale multiplies the rotated values.  A token with a
+ * negative position or without a place in the block table is left out and raises
+ * P100_ERR_INVALID in p100_device_error(). */
+p100_status p100_paged_append_rope(const p100_paged_desc* desc, const void* qkv, int qkv_type, long long qkv_stride,
+                                   const float* q_norm, const float* k_norm, float eps, const p100_rope* rope,
+                                   const int* position, const int* block_table, const int* q_start, const int* kv_len,
+                                   void* q, void* k_pages, void* v_pages, p100_stream_t stream);
+
+/* p100_fa_paged for drafted trees: a new token sees every token before its
+ * sequence's new ones, and of those the ones its row of mask names (rows of
+ * mask_words words, p100_tree_mask's layout; any bits are allowed, its own may be
+ * clear, those at and behind the number of new tokens count for nothing).
+ * causal is not read.  A sequence with more than 32 mask_words new tokens makes
+ * the call do nothing and raises P100_ERR_INVALID in p100_device_error().
+ * Workspace, outputs, refusals and values that are not finite as
+ * p100_fa_paged's.  Each probability goes to the product with V in two parts of
+ * dtype, 2^-16 (bfloat16) or 2^-22 off. */
+p100_status p100_fa_tree(const p100_paged_desc* desc, const void* q, const void* k_pages, const void* v_pages,
+                         const unsigned* mask, int mask_words, const int* block_table, const int* q_start,
+                         const int* kv_len, void* o, float* lse, void* ws, size_t ws_bytes, p100_stream_t stream);
+
+/* Keeps chosen new tokens: for i < keep_len[s], the K and V rows of new token
+ * keep[q_start[s] + i] of sequence s become those of new token i (keep rises:
+ * the path of an accepted draft), in the pages' place; rows behind them stay as
+ * they are.  length[s] = kv_len - n + keep_len[s], the next plan's length
+ * (may be NULL).  A keep_len outside [0, n] leaves its sequence out, an index
+ * out of order or range its row; both, and pages out of range, raise
+ * P100_ERR_INVALID in p100_device_error().  Sequences may not share the pages
+ * that hold new tokens. */
+p100_status p100_paged_keep(const p100_paged_desc* desc, void* k_pages, void* v_pages, const int* keep,
+                            const int* keep_len, const int* block_table, const int* q_start, const int* kv_len,
+                            int* length, p100_stream_t stream);
+
 /* --------------------------------------------------- batch-1 decoder */
 /* A Llama-3-shaped model with synthetic weights, decoded one token per
  * p100_decoder_step.  No reference counterpart (see above).  Every linear

@@ -39,6 +39,9 @@ QMV_MMA = 4  # P100_QMV_MMA: batch 2..16 never on the tcgen05 kernel
 F32, F16, BF16 = 0, 1, 2
 PAGED_MAX_SEQ = 1024   # P100_PAGED_MAX_SEQ
 LOGPROBS_MAX_TOP = 32
+TREE_MAX_WORDS = 32    # P100_TREE_MAX_WORDS
+# kinds of scaled rotary frequencies (p100_rope_kind)
+ROPE_NONE, ROPE_LINEAR, ROPE_NTK, ROPE_BANDS, ROPE_YARN, ROPE_DIVISORS = range(6)
 TP_PEER_MAX = 65536   # P100_TP_PEER_MAX: all-reduces up to this count may run over peer memory
 
 STATUS = {0: "P100_OK", 1: "P100_ERR_INVALID", 2: "P100_ERR_CUDA", 3: "P100_ERR_NCCL",
@@ -90,6 +93,46 @@ class PagedDesc(C.Structure):
         super().__init__(n_seq, n_tokens, max_q, n_head_q, n_head_kv, head_dim, dtype, page_size, n_pages, max_pages,
                          scale, softcap, int(bool(causal)), int(bool(o_fp32)), page_stride, head_stride, token_stride,
                          q_stride, o_stride)
+
+
+class RopeScaling(C.Structure):
+    """p100_rope_scaling."""
+    _fields_ = [("kind", C.c_int), ("original", C.c_int), ("factor", C.c_double), ("low", C.c_double),
+                ("high", C.c_double), ("mscale", C.c_double), ("divisors", C.POINTER(C.c_double))]
+
+
+class Rope(C.Structure):
+    """p100_rope: the rotation of the first rope_dim values of a head, pairs of adjacent values or (half) of value i
+    and i + rope_dim / 2, with the frequencies theta^(-2i / rope_dim) scaled as p100_rope_kind says: factor (LINEAR,
+    NTK, BANDS, YARN), low, high and original (BANDS, YARN), divisors (DIVISORS); mscale multiplies the rotated
+    values, 0 stands for the kind's own."""
+    _fields_ = [("rope_dim", C.c_int), ("half", C.c_int), ("mscale", C.c_float), ("reserved", C.c_int),
+                ("turns", C.c_ulonglong * 64)]
+
+    def __init__(self, rope_dim, theta, half=False, scaling=ROPE_NONE, factor=0.0, low=0.0, high=0.0, original=0,
+                 mscale=0.0, divisors=None):
+        super().__init__()
+        values = None
+        if divisors is not None:
+            if len(divisors) != rope_dim // 2:
+                raise InvalidArgument(ERR_INVALID, f"divisors needs {rope_dim // 2} values, has {len(divisors)}")
+            values = (C.c_double * len(divisors))(*divisors)
+        s = RopeScaling(scaling, original, factor, low, high, mscale, values)
+        check(lib().p100_rope_init(C.byref(self), rope_dim, int(bool(half)), theta, C.byref(s)))
+
+
+class PagedPlan(typing.NamedTuple):
+    """p100_paged_plan's outputs."""
+    q_start: object    # int32 [n_seq + 1]
+    kv_len: object     # int32 [n_seq]
+    slot: object       # int64 [n_tokens], -1 behind the last new token
+    position: object   # int32 [n_tokens], -1 behind the last new token
+
+
+class TreeMask(typing.NamedTuple):
+    """p100_tree_mask's outputs."""
+    mask: object       # int32 [n_tokens, mask_words], the words' bits
+    position: object   # int32 [n_tokens]
 
 
 class LogProbs(typing.NamedTuple):
@@ -168,6 +211,13 @@ def _bind(lib):
         "p100_logprobs_workspace_size": (sz, [ip, ip, ip, ip]),
         "p100_logprobs_workspace_init": (ip, [vp, sz, st]),
         "p100_logprobs": (ip, [vp, ip, ip, ip, C.c_longlong, vp, ip, vp, vp, vp, vp, vp, vp, sz, st]),
+        "p100_paged_plan": (ip, [vp] * 10 + [st]),
+        "p100_paged_pool_init": (ip, [vp] * 4 + [st]),
+        "p100_tree_mask": (ip, [vp, vp, vp, ip, ip, ip, vp, vp, st]),
+        "p100_rope_init": (ip, [vp, ip, ip, C.c_double, vp]),
+        "p100_paged_append_rope": (ip, [vp, vp, ip, C.c_longlong, vp, vp, C.c_float] + [vp] * 8 + [st]),
+        "p100_fa_tree": (ip, [vp] * 5 + [ip] + [vp] * 6 + [sz, st]),
+        "p100_paged_keep": (ip, [vp] * 9 + [st]),
         "p100_decoder_create": (ip, [vp, vp, C.POINTER(vp)]),
         "p100_decoder_init_random": (ip, [vp, C.c_ulonglong]),
         "p100_decoder_fill_kv": (ip, [vp, ip, C.c_ulonglong, C.c_float]),
@@ -474,15 +524,8 @@ def _lengths_of(dev, desc, block_table, q_start, kv_len):
     _need(kv_len, "kv_len", dev, int32, n)
 
 
-def paged_append(desc, qkv, block_table, q_start, kv_len, k_pages, v_pages, rope_cs=None, q_norm=None, k_norm=None,
-                 eps=1e-5, rope_half=False, q=None, stream=None):
-    """New tokens into a paged cache (p100_paged_append): per-head norms and rotation of the fused rows qkv
-    [n_tokens, (n_head_q + 2 n_head_kv) head_dim] (float32, float16 or bfloat16), k and v to their pages, the
-    queries returned as q [n_tokens, n_head_q, head_dim] of the cache's type.  Pages [n_pages, n_head_kv, page_size,
-    head_dim] or [n_pages, page_size, n_head_kv, head_dim] must have the descriptor's strides in that order; of a tensor
-    of other sizes the descriptor's alone count."""
-    torch = _torch()
-    dev = torch.cuda.current_device()
+def _fused_rows(dev, desc, qkv, block_table, q_start, kv_len, k_pages, v_pages, q_norm, k_norm):
+    """The type of an append's fused rows, when its inputs are as they should be."""
     width = (desc.n_head_q + 2 * desc.n_head_kv) * desc.head_dim
     qkv_type = _dtype_of(qkv, "qkv")
     _need(qkv, "qkv", dev, dense=False)
@@ -494,17 +537,34 @@ def paged_append(desc, qkv, block_table, q_start, kv_len, k_pages, v_pages, rope
     _pages_of(k_pages, v_pages, dev, desc)
     for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
         if w is not None:
-            _need(w, what, dev, torch.float32, desc.head_dim)
+            _need(w, what, dev, _torch().float32, desc.head_dim)
+    return qkv_type
+
+
+def _queries(dev, desc, qkv, q, stream):
+    if q is None:
+        return _alloc(stream, lambda: _new_rows(qkv, desc, _paged_type(desc), desc.q_stride))
+    _rows_of(q, "q", dev, desc, _paged_type(desc), desc.q_stride)
+    return q
+
+
+def paged_append(desc, qkv, block_table, q_start, kv_len, k_pages, v_pages, rope_cs=None, q_norm=None, k_norm=None,
+                 eps=1e-5, rope_half=False, q=None, stream=None):
+    """New tokens into a paged cache (p100_paged_append): per-head norms and rotation of the fused rows qkv
+    [n_tokens, (n_head_q + 2 n_head_kv) head_dim] (float32, float16 or bfloat16), k and v to their pages, the
+    queries returned as q [n_tokens, n_head_q, head_dim] of the cache's type.  Pages [n_pages, n_head_kv, page_size,
+    head_dim] or [n_pages, page_size, n_head_kv, head_dim] must have the descriptor's strides in that order; of a tensor
+    of other sizes the descriptor's alone count."""
+    torch = _torch()
+    dev = torch.cuda.current_device()
+    qkv_type = _fused_rows(dev, desc, qkv, block_table, q_start, kv_len, k_pages, v_pages, q_norm, k_norm)
     max_pos = 0
     if rope_cs is not None:
         _need(rope_cs, "rope_cs", dev, torch.float32)
         if rope_cs.dim() != 3 or rope_cs.shape[1] != desc.head_dim // 2 or rope_cs.shape[2] != 2:
             raise InvalidArgument(ERR_INVALID, f"rope_cs must be [max_pos, {desc.head_dim // 2}, 2]")
         max_pos = rope_cs.shape[0]
-    if q is None:
-        q = _alloc(stream, lambda: _new_rows(qkv, desc, _paged_type(desc), desc.q_stride))
-    else:
-        _rows_of(q, "q", dev, desc, _paged_type(desc), desc.q_stride)
+    q = _queries(dev, desc, qkv, q, stream)
     check(lib().p100_paged_append(C.byref(desc), qkv.data_ptr(), qkv_type, qkv.stride(0) if qkv.shape[0] > 1 else 0,
                                   _addr(q_norm), _addr(k_norm), eps, _addr(rope_cs), max_pos, int(bool(rope_half)),
                                   block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), q.data_ptr(),
@@ -534,8 +594,17 @@ def fa_paged_workspace(desc, stream=None):
 def fa_paged(desc, q, k_pages, v_pages, block_table, q_start, kv_len, o=None, lse=None, ws=None, stream=None):
     """Attention of the new tokens over a paged cache (p100_fa_paged): q [n_tokens, n_head_q, head_dim] of the
     cache's type -> o of the same shape (float32 with desc.o_fp32), lse fp32 [n_tokens, n_head_q]."""
+    dev = _torch().cuda.current_device()
+    o, lse, ws = _attention(dev, desc, q, k_pages, v_pages, block_table, q_start, kv_len, o, lse, ws, stream)
+    check(lib().p100_fa_paged(C.byref(desc), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                              block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), o.data_ptr(),
+                              lse.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream(stream, dev)))
+    return o, lse
+
+
+def _attention(dev, desc, q, k_pages, v_pages, block_table, q_start, kv_len, o, lse, ws, stream):
+    """The outputs and the workspace of an attention call, when its inputs are as they should be."""
     torch = _torch()
-    dev = torch.cuda.current_device()
     o_type = torch.float32 if desc.o_fp32 else _paged_type(desc)
     _rows_of(q, "q", dev, desc, _paged_type(desc), desc.q_stride)
     _lengths_of(dev, desc, block_table, q_start, kv_len)
@@ -552,12 +621,142 @@ def fa_paged(desc, q, k_pages, v_pages, block_table, q_start, kv_len, o=None, ls
         ws = fa_paged_workspace(desc, stream)
     else:
         _need(ws, "ws", dev, torch.uint8)
-    check(lib().p100_fa_paged(C.byref(desc), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                              block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), o.data_ptr(),
-                              lse.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream(stream, dev)))
+    return o, lse, ws
+
+
+# ---------------------------------------------------------------- steps and drafted trees
+def _plan_state(dev, desc, pool, held, block_table):
+    int32 = _torch().int32
+    _need(pool, "pool", dev, int32, 2 + desc.n_pages)
+    _need(held, "held", dev, int32, desc.n_seq)
+    _need(block_table, "block_table", dev, int32, desc.n_seq * desc.max_pages)
+    if block_table.dim() != 2 or block_table.shape[1] != desc.max_pages:
+        raise InvalidArgument(ERR_INVALID, f"block_table must be [n_seq, {desc.max_pages}]")
+
+
+def paged_pool(desc, stream=None):
+    """(pool, held, block_table) with every page of desc free (p100_paged_pool_init), int32 on the current device."""
+    torch = _torch()
+
+    def make():
+        new, i = torch.empty, torch.int32
+        return (new(2 + desc.n_pages, dtype=i, device="cuda"), new(desc.n_seq, dtype=i, device="cuda"),
+                new((desc.n_seq, desc.max_pages), dtype=i, device="cuda"))
+
+    pool, held, table = _alloc(stream, make)
+    check(lib().p100_paged_pool_init(C.byref(desc), _addr(pool), _addr(held), _addr(table), _stream(stream)))
+    return pool, held, table
+
+
+def paged_plan(desc, length, n_new, pool, held, block_table, out=None, stream=None):
+    """The plan of a step (p100_paged_plan): pages for n_new tokens behind length of each request (int32 [n_seq]),
+    pool, held and block_table updated in place.  Returns PagedPlan; out: one of an earlier call to write into, of
+    which slot and position may be None."""
+    torch = _torch()
+    dev = torch.cuda.current_device()
+    i = torch.int32
+    _need(length, "length", dev, i, desc.n_seq)
+    _need(n_new, "n_new", dev, i, desc.n_seq)
+    _plan_state(dev, desc, pool, held, block_table)
+    if out is None:
+        new = length.new_empty
+        out = _alloc(stream, lambda: PagedPlan(new(desc.n_seq + 1), new(desc.n_seq),
+                                               new(desc.n_tokens, dtype=torch.int64), new(desc.n_tokens)))
+    else:
+        _need(out.q_start, "q_start", dev, i, desc.n_seq + 1)
+        _need(out.kv_len, "kv_len", dev, i, desc.n_seq)
+        if out.slot is not None:
+            _need(out.slot, "slot", dev, torch.int64, desc.n_tokens)
+        if out.position is not None:
+            _need(out.position, "position", dev, i, desc.n_tokens)
+    check(lib().p100_paged_plan(C.byref(desc), length.data_ptr(), n_new.data_ptr(), pool.data_ptr(), held.data_ptr(),
+                                block_table.data_ptr(), out.q_start.data_ptr(), out.kv_len.data_ptr(),
+                                _addr(out.slot), _addr(out.position), _raw_stream(stream, dev)))
+    return out
+
+
+def tree_mask(parent, q_start, kv_len, mask_words, mask=None, position=None, stream=None):
+    """Masks and positions of drafted trees (p100_tree_mask): parent int32 [n_tokens], the parent's index in the token's
+    own tree or -1.  Returns TreeMask."""
+    torch = _torch()
+    dev = torch.cuda.current_device()
+    i, n_tokens, n_seq = torch.int32, parent.numel(), kv_len.numel()
+    _need(parent, "parent", dev, i)
+    _need(kv_len, "kv_len", dev, i)
+    _need(q_start, "q_start", dev, i, n_seq + 1)
+    if not 1 <= mask_words <= TREE_MAX_WORDS:
+        raise InvalidArgument(ERR_INVALID, "mask_words must be between 1 and 32")
+    if mask is None:
+        mask = _alloc(stream, lambda: parent.new_empty((n_tokens, mask_words)))
+    else:
+        _mask_of(mask, dev, n_tokens)
+        if mask.shape[1] != mask_words:
+            raise InvalidArgument(ERR_INVALID, f"mask must have {mask_words} words a token")
+    if position is None:
+        position = _alloc(stream, lambda: parent.new_empty(n_tokens))
+    else:
+        _need(position, "position", dev, i, n_tokens)
+    check(lib().p100_tree_mask(parent.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), n_seq, n_tokens, mask_words,
+                               mask.data_ptr(), position.data_ptr(), _raw_stream(stream, dev)))
+    return TreeMask(mask, position)
+
+
+def _mask_of(mask, dev, n_tokens):
+    _need(mask, "mask", dev, _torch().int32)
+    if mask.dim() != 2 or mask.shape[0] < n_tokens:
+        raise InvalidArgument(ERR_INVALID, f"mask must be [{n_tokens}, mask_words]")
+
+
+def paged_append_rope(desc, qkv, rope, block_table, q_start, kv_len, k_pages, v_pages, position=None, q_norm=None,
+                      k_norm=None, eps=1e-5, q=None, stream=None):
+    """paged_append with the rotation of a Rope instead of a table, at int32 position [n_tokens] (None: each token's own
+    position in its sequence) (p100_paged_append_rope).  Returns q."""
+    torch = _torch()
+    dev = torch.cuda.current_device()
+    qkv_type = _fused_rows(dev, desc, qkv, block_table, q_start, kv_len, k_pages, v_pages, q_norm, k_norm)
+    if position is not None:
+        _need(position, "position", dev, torch.int32, desc.n_tokens)
+    q = _queries(dev, desc, qkv, q, stream)
+    check(lib().p100_paged_append_rope(C.byref(desc), qkv.data_ptr(), qkv_type,
+                                       qkv.stride(0) if qkv.shape[0] > 1 else 0, _addr(q_norm), _addr(k_norm), eps,
+                                       C.byref(rope), _addr(position), block_table.data_ptr(), q_start.data_ptr(),
+                                       kv_len.data_ptr(), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                                       _raw_stream(stream, dev)))
+    return q
+
+
+def fa_tree(desc, q, k_pages, v_pages, mask, block_table, q_start, kv_len, o=None, lse=None, ws=None, stream=None):
+    """Attention of drafted trees over a paged cache (p100_fa_tree): fa_paged with the int32 words mask [n_tokens,
+    mask_words] over each sequence's new tokens; ws from fa_paged_workspace."""
+    dev = _torch().cuda.current_device()
+    _mask_of(mask, dev, desc.n_tokens)
+    o, lse, ws = _attention(dev, desc, q, k_pages, v_pages, block_table, q_start, kv_len, o, lse, ws, stream)
+    check(lib().p100_fa_tree(C.byref(desc), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), mask.data_ptr(),
+                             mask.shape[1], block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(),
+                             o.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream(stream, dev)))
     return o, lse
 
 
+def paged_keep(desc, k_pages, v_pages, keep, keep_len, block_table, q_start, kv_len, length=None, stream=None):
+    """Moves the rows of kept new tokens in the pages (p100_paged_keep): keep int32 [n_tokens], keep_len int32 [n_seq].
+    Returns length, the tokens of each sequence that stay."""
+    torch = _torch()
+    dev = torch.cuda.current_device()
+    _lengths_of(dev, desc, block_table, q_start, kv_len)
+    _pages_of(k_pages, v_pages, dev, desc)
+    _need(keep, "keep", dev, torch.int32, desc.n_tokens)
+    _need(keep_len, "keep_len", dev, torch.int32, desc.n_seq)
+    if length is None:
+        length = _alloc(stream, lambda: keep_len.new_empty(desc.n_seq))
+    else:
+        _need(length, "length", dev, torch.int32, desc.n_seq)
+    check(lib().p100_paged_keep(C.byref(desc), k_pages.data_ptr(), v_pages.data_ptr(), keep.data_ptr(),
+                                keep_len.data_ptr(), block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(),
+                                length.data_ptr(), _raw_stream(stream, dev)))
+    return length
+
+
+# ---------------------------------------------------------------- scoring
 def logprobs_workspace(rows, n, top_k=0, dtype=F32, stream=None):
     """A workspace for logprobs of that many rows, or None where none is needed.  The size for F32 rows serves the
     16-bit types too."""

@@ -68,6 +68,8 @@ struct Params {
     float* ws_ml;      // [CTAs][2][kRows][2], m in units of log2
     unsigned* tickets; // [2][CTAs]
     float scale, softcap;
+    const unsigned* mask;   // of a tree: [n_tokens][words]
+    int words;
 };
 
 // Shares of a call's units on so many CTAs.  Every share has a unit, so every
@@ -241,7 +243,14 @@ __device__ __forceinline__ void join_parts(const Params& p, const Out& out, int 
     }
 }
 
-template <typename T, int D, bool SPARE>
+// Whether a token of a drafted tree sees new token `node` of its sequence; row:
+// its words of the mask.
+__device__ __forceinline__ bool sees(const unsigned* row, int node) { return row[node >> 5] >> (node & 31) & 1u; }
+
+// With TREE, keys before the sequence's new tokens are seen by all, of the new
+// tokens those of the mask's bits (the host clears causal and bounds max_q by
+// the mask's width).
+template <typename T, int D, bool SPARE, bool TREE = false>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_kernel(const Params p) {
     extern __shared__ __align__(128) uint8_t smem[];
     constexpr int kRowBytes = D * 2;
@@ -331,6 +340,12 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_kernel(const Params p) {
             const int r = g + 8 * h;
             limit[h] = r >= rows ? 0 : d.causal ? min(kv, kv - n + (row0 + r) / d.group + 1) : kv;
         }
+        const unsigned* bits[2] = {nullptr, nullptr};
+        if (TREE) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (g + 8 * h < rows) bits[h] = p.mask + (long long)(q0 + (row0 + g + 8 * h) / d.group) * p.words;
+        }
         float acc[D / 8][4];
 #pragma unroll
         for (int i = 0; i < D / 8; ++i)
@@ -369,7 +384,10 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_kernel(const Params p) {
 #pragma unroll
                     for (int e = 2 * h; e < 2 * h + 2; ++e) {
                         float x = p.softcap != 0.f ? cap_score(s[j][e], cap_in, p.softcap * kLog2e) : s[j][e] * to_log2;
-                        s[j][e] = key0 + j * 8 + (e & 1) < limit[h] ? x : -INFINITY;
+                        const int key = key0 + j * 8 + (e & 1);
+                        bool seen = key < limit[h];
+                        if (TREE && seen && key >= kv - n) seen = sees(bits[h], key - (kv - n));
+                        s[j][e] = seen ? x : -INFINITY;
                     }
                 float mx = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));

@@ -3,18 +3,10 @@
 // and the scoring of logits.  A translation unit of its own, with its own
 // g_device_error word, which p100_device_error reads through
 // serve_device_error.
-#include <climits>
-#include <cmath>
 #include <cstring>
-#include <algorithm>
 
-#include <cudaTypedefs.h>
-
-#include "common.cuh"
-#include "fa_paged.cuh"
-#include "fa_paged_tc.cuh"
 #include "logprobs.cuh"
-#include "paged_append.cuh"
+#include "paged_host.cuh"
 
 namespace p100b {
 
@@ -30,122 +22,12 @@ p100_status serve_device_error(int clear, int* value) {
 
 namespace {
 
-size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
-bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-
-// Dynamic shared memory beyond 48 KB, once per kernel and device.
-template <typename K>
-p100_status allow_smem(K kern, size_t bytes, int (&configured)[64], const char* what) {
-    int dev = 0;
-    if (cudaError_t e = cudaGetDevice(&dev)) return cuda_status(e, what);
-    if (configured[dev]) return P100_OK;
-    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)))
-        return cuda_status(e, what);
-    configured[dev] = 1;
-    return P100_OK;
-}
-
 // ------------------------------------------------------------ paged cache
-// The descriptor with its defaults filled in, or the reason it is refused.
-const char* paged_reason(const p100_paged_desc& in, paged::Desc& d) {
-    if (in.n_seq < 0 || in.n_tokens < 0 || in.max_q < 0 || in.n_pages < 0 || in.max_pages < 0)
-        return "counts must not be negative";
-    if (in.n_seq > P100_PAGED_MAX_SEQ) return "n_seq exceeds P100_PAGED_MAX_SEQ";
-    if (in.n_head_q <= 0 || in.n_head_kv <= 0 || in.page_size <= 0) return "all dimensions must be positive";
-    if (in.n_head_q % in.n_head_kv) return "n_head_q must be divisible by n_head_kv";
-    if (in.head_dim != 64 && in.head_dim != 128) return "head_dim must be 64 or 128";
-    if (in.dtype != P100_F16 && in.dtype != P100_BF16) return "dtype must be P100_F16 or P100_BF16";
-    if (!std::isfinite(in.scale)) return "scale must be finite";
-    if (!std::isfinite(in.softcap) || in.softcap < 0.0f) return "softcap must be finite and non-negative";
-    if (in.softcap > 1e15f) return "softcap must be at most 1e15";   // hidden scores are set to -1e18
-    if ((long long)in.n_tokens * in.n_head_q > INT_MAX) return "n_tokens * n_head_q exceeds 2^31 - 1";
-    if ((long long)in.max_pages * in.page_size > INT_MAX) return "max_pages * page_size exceeds 2^31 - 1";
-    const long long D = in.head_dim;
-    d.n_seq = in.n_seq;
-    d.n_tokens = in.n_tokens;
-    d.max_q = in.max_q ? std::min(in.max_q, in.n_tokens) : in.n_tokens;
-    d.n_head_q = in.n_head_q;
-    d.n_head_kv = in.n_head_kv;
-    d.group = in.n_head_q / in.n_head_kv;
-    d.page_size = in.page_size;
-    d.n_pages = in.n_pages;
-    d.max_pages = in.max_pages;
-    d.causal = in.causal != 0;
-    d.token_stride = in.token_stride ? in.token_stride : D;
-    d.head_stride = in.head_stride ? in.head_stride : in.page_size * D;
-    d.page_stride = in.page_stride ? in.page_stride : (long long)in.n_head_kv * in.page_size * D;
-    d.q_stride = in.q_stride ? in.q_stride : in.n_head_q * D;
-    d.o_stride = in.o_stride ? in.o_stride : in.n_head_q * D;
-    for (long long s : {d.token_stride, d.head_stride, d.page_stride}) {
-        if (s < D) return "page strides must be at least head_dim";
-        if (s % 8) return "strides must be multiples of 8 elements";
-    }
-    for (long long s : {d.q_stride, d.o_stride}) {
-        if (s < in.n_head_q * D) return "q and o strides must be at least n_head_q * head_dim";
-        if (s % 8) return "strides must be multiples of 8 elements";
-    }
-    return nullptr;
-}
-
-// CTAs of the mma.sync kernel: two on every SM.
-constexpr int kMmaCtas = 2;
-static_assert(paged::kMaxSeq == P100_PAGED_MAX_SEQ, "lengths in shared memory");
-
 // The tensor-core kernel takes calls in which a sequence may have more rows
 // (new tokens x query heads per kv head) than the mma.sync kernel's row tile.
 // One token each of 64 sequences of 8192 (64 / 8 heads): 245 us on the mma.sync
 // kernel, 396 on the other; of 16 sequences (12 / 4 heads of 64) 31 and 59.
 bool fa_paged_on_tc(const paged::Desc& d) { return (long long)d.max_q * d.group > fap::kRows && d.n_pages > 0; }
-
-// Units of a sequence's kv head are counted in 32 bits.
-bool fa_paged_too_long(const paged::Desc& d, int rows, int keys, int over) {
-    const double tiles = std::ceil(double(d.max_q) * d.group / rows);
-    return tiles * (double(d.max_pages) * d.page_size / keys + 1 + over) >= 4294967295.0;
-}
-
-// Partials of both kernels share one place: their calls follow one another.
-struct FaPagedWs {
-    size_t tickets, o, ml, total;
-};
-size_t fa_paged_ticket_bytes(int sms) { return round256(size_t(sms) * kMmaCtas * 2 * sizeof(unsigned)); }
-FaPagedWs fa_paged_ws(const p100_paged_desc& in, int sms) {
-    const size_t rows = size_t(sms) * 2 * std::max(kMmaCtas * fap::kRows, fatc::kRows);
-    FaPagedWs w;
-    w.tickets = fa_paged_ticket_bytes(sms);   // first, so that init clears little
-    w.o = round256(rows * in.head_dim * sizeof(float));
-    w.ml = round256(rows * 2 * sizeof(float));
-    w.total = w.tickets + w.o + w.ml;
-    return w;
-}
-
-// The pages as a 4-d tensor (head_dim, token of the page, kv head, page) in
-// boxes of 64 values x `box` tokens with the 128-byte swizzle.
-p100_status page_map(CUtensorMap* map, const void* base, const p100_paged_desc& in, const paged::Desc& d, int box) {
-    static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess) {
-            (void)cudaGetLastError();
-            f = nullptr;
-        }
-        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-    }();
-    if (!encode) return set_error(P100_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-    const cuuint64_t dims[4] = {cuuint64_t(in.head_dim), cuuint64_t(d.page_size), cuuint64_t(d.n_head_kv),
-                                cuuint64_t(d.n_pages)};
-    const cuuint64_t strides[3] = {cuuint64_t(d.token_stride) * 2, cuuint64_t(d.head_stride) * 2,
-                                   cuuint64_t(d.page_stride) * 2};
-    const cuuint32_t boxes[4] = {64, cuuint32_t(box), 1, 1};
-    const cuuint32_t elem[4] = {1, 1, 1, 1};
-    const CUresult r =
-        encode(map, in.dtype == P100_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-               const_cast<void*>(base), dims, strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS)
-        return set_error(P100_ERR_INVALID, "page tensor map rejected (error %d): strides or extents", int(r));
-    return P100_OK;
-}
 
 template <typename T, int D, bool CAP>
 p100_status launch_fa_paged_tc(const fatc::Params& prm, const CUtensorMap& tmk, const CUtensorMap& tmv, int sms,
@@ -189,20 +71,6 @@ p100_status launch_fa_paged_mma_d(const fap::Params& prm, int head_dim, int sms,
     if (head_dim == 64)
         return spare ? launch_fa_paged_mma<T, 64, true>(prm, sms, s) : launch_fa_paged_mma<T, 64, false>(prm, sms, s);
     return spare ? launch_fa_paged_mma<T, 128, true>(prm, sms, s) : launch_fa_paged_mma<T, 128, false>(prm, sms, s);
-}
-
-template <typename S, typename T>
-p100_status launch_append(const paged::AppendParams& prm, int head_dim, unsigned blocks, cudaStream_t stream) {
-    if (head_dim == 64)
-        paged::paged_append_kernel<S, T, 64><<<blocks, paged::kAppendThreads, 0, stream>>>(prm);
-    else
-        paged::paged_append_kernel<S, T, 128><<<blocks, paged::kAppendThreads, 0, stream>>>(prm);
-    return cuda_status(cudaGetLastError(), "paged_append_kernel launch");
-}
-template <typename S>
-p100_status launch_append_to(const paged::AppendParams& prm, int dtype, int head_dim, unsigned blocks, cudaStream_t s) {
-    return dtype == P100_F16 ? launch_append<S, __half>(prm, head_dim, blocks, s)
-                             : launch_append<S, __nv_bfloat16>(prm, head_dim, blocks, s);
 }
 
 // ------------------------------------------------------------ logits
@@ -254,56 +122,19 @@ p100_status p100_paged_append(const p100_paged_desc* desc, const void* qkv, int 
                               int rope_half, const int* block_table, const int* q_start, const int* kv_len, void* q,
                               void* k_pages, void* v_pages, p100_stream_t stream) {
     clear_error();
-    if (!desc) return set_error(P100_ERR_INVALID, "null descriptor");
     paged::AppendParams prm = {};
-    if (const char* why = paged_reason(*desc, prm.d)) return set_error(P100_ERR_INVALID, "%s", why);
-    if (qkv_type != P100_F32 && qkv_type != P100_F16 && qkv_type != P100_BF16)
-        return set_error(P100_ERR_INVALID, "unknown qkv type %d", qkv_type);
-    const long long heads = (long long)desc->n_head_q + 2LL * desc->n_head_kv, width = heads * desc->head_dim;
-    if (qkv_stride == 0) qkv_stride = width;
-    if (qkv_stride < width) return set_error(P100_ERR_INVALID, "qkv_stride must be at least a fused row");
-    if (qkv_stride * (qkv_type == P100_F32 ? 4 : 2) % 16)
-        return set_error(P100_ERR_INVALID, "qkv rows must be 16-byte aligned");
-    if ((q_norm || k_norm) && !(std::isfinite(eps) && eps >= 0.0f))
-        return set_error(P100_ERR_INVALID, "eps must be finite and non-negative");
-    if (rope_cs && max_pos <= 0) return set_error(P100_ERR_INVALID, "max_pos must be positive");
-    int sms = 0;
-    if (p100_status st = require_sm100(nullptr, &sms)) return st;
-    if (desc->n_tokens == 0 || desc->n_seq == 0) return P100_OK;
-    if (!qkv || !block_table || !q_start || !kv_len || !q || !k_pages || !v_pages)
-        return set_error(P100_ERR_INVALID, "null buffer");
-    if (!aligned(qkv, 16) || !aligned(q, 16) || !aligned(k_pages, 16) || !aligned(v_pages, 16))
-        return set_error(P100_ERR_INVALID, "qkv, q and the pages must be 16-byte aligned");
+    unsigned blocks = 0;
+    if (p100_status st = append_params(desc, qkv, qkv_type, qkv_stride, q_norm, k_norm, eps,
+                                       rope_cs && max_pos <= 0 ? "max_pos must be positive" : nullptr, block_table,
+                                       q_start, kv_len, q, k_pages, v_pages, prm, blocks))
+        return st;
+    if (!blocks) return P100_OK;
     if (!aligned(rope_cs, 8)) return set_error(P100_ERR_INVALID, "rope_cs must be 8-byte aligned");
-    prm.d.block_table = block_table;
-    prm.d.q_start = q_start;
-    prm.d.kv_len = kv_len;
-    prm.qkv = qkv;
-    prm.qkv_stride = qkv_stride;
-    prm.q_norm = q_norm;
-    prm.k_norm = k_norm;
-    prm.eps = eps;
     prm.rope = reinterpret_cast<const float2*>(rope_cs);
     prm.max_pos = max_pos;
     prm.half = rope_half != 0;
-    prm.q = q;
-    prm.k = k_pages;
-    prm.v = v_pages;
-    // as many warps a token as give every SM kAppendWarps of them, and no warp
-    // more than kAppendMost steps
-    const int at_once = qkv_type == P100_F32 ? 32 * paged::append_values<float>() / desc->head_dim
-                                             : 32 * paged::append_values<__half>() / desc->head_dim;
-    const int together = qkv_type == P100_F32 ? paged::append_steps<float>() : paged::append_steps<__half>();
-    const long long steps = paged::Steps(desc->n_head_q, desc->n_head_kv, at_once).all();
-    const long long fill = std::min((steps + together - 1) / together, (long long)sms * paged::kAppendWarps / desc->n_tokens);
-    prm.warps = int(std::max({1LL, fill, (steps + paged::kAppendMost - 1) / paged::kAppendMost}));
-    const long long blocks = ((long long)desc->n_tokens * prm.warps + paged::kAppendThreads / 32 - 1) / (paged::kAppendThreads / 32);
-    if (blocks > INT_MAX) return set_error(P100_ERR_INVALID, "too many heads and tokens for one call");
-    switch (qkv_type) {
-        case P100_F32: return launch_append_to<float>(prm, desc->dtype, desc->head_dim, unsigned(blocks), stream);
-        case P100_F16: return launch_append_to<__half>(prm, desc->dtype, desc->head_dim, unsigned(blocks), stream);
-        default: return launch_append_to<__nv_bfloat16>(prm, desc->dtype, desc->head_dim, unsigned(blocks), stream);
-    }
+    return launch_append_from<paged::ByTable>(prm, paged::NoParams{}, qkv_type, desc->dtype, desc->head_dim, blocks,
+                                              stream);
 }
 
 size_t p100_fa_paged_workspace_size(const p100_paged_desc* desc) {
