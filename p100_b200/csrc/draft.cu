@@ -3,6 +3,7 @@
 // the append with computed rotations, the attention of trees and the move of
 // accepted rows.  A translation unit of its own, with its own g_device_error
 // word, which p100_device_error reads through draft_device_error.
+#include "fa_tree.cuh"
 #include "paged_host.cuh"
 #include "paged_plan.cuh"
 #include "rope.cuh"
@@ -59,6 +60,10 @@ const char* words_reason(int mask_words) {
     return mask_words < 1 || mask_words > P100_TREE_MAX_WORDS ? "mask_words must be between 1 and 32" : nullptr;
 }
 
+bool fa_tree_on_tc(const paged::Desc& d) {
+    return (long long)d.max_q * d.group > fap::kRows && d.n_pages > 0;
+}
+
 template <typename T, int D, bool SPARE>
 p100_status launch_fa_tree_mma(const fap::Params& prm, int sms, cudaStream_t stream) {
     static thread_local int configured[64] = {};
@@ -76,6 +81,29 @@ p100_status launch_fa_tree_mma_d(const fap::Params& prm, int head_dim, int sms, 
     if (head_dim == 64)
         return spare ? launch_fa_tree_mma<T, 64, true>(prm, sms, s) : launch_fa_tree_mma<T, 64, false>(prm, sms, s);
     return spare ? launch_fa_tree_mma<T, 128, true>(prm, sms, s) : launch_fa_tree_mma<T, 128, false>(prm, sms, s);
+}
+
+template <typename T, int D, bool CAP>
+p100_status launch_fa_tree_tc(const fatr::Params& prm, const CUtensorMap& tmk, const CUtensorMap& tmv, int sms,
+                              cudaStream_t stream) {
+    static thread_local int configured[64] = {};
+    auto kern = fatr::fa_tree_kernel<T, D, CAP>;
+    constexpr size_t fixed = fatr::smem_bytes<D>();
+    if (p100_status st = allow_smem(kern, fixed + paged::Lengths::bytes(paged::kMaxSeq), configured,
+                                    "cudaFuncSetAttribute(fa_tree)"))
+        return st;
+    kern<<<sms, fatr::kThreads, fixed + paged::Lengths::bytes(prm.d.n_seq), stream>>>(prm, tmk, tmv);
+    return cuda_status(cudaGetLastError(), "fa_tree_kernel launch");
+}
+template <typename T>
+p100_status launch_fa_tree_tc_d(const fatr::Params& prm, int head_dim, const CUtensorMap& tmk, const CUtensorMap& tmv,
+                                int sms, cudaStream_t s) {
+    const bool cap = prm.softcap != 0.0f;
+    if (head_dim == 64)
+        return cap ? launch_fa_tree_tc<T, 64, true>(prm, tmk, tmv, sms, s)
+                   : launch_fa_tree_tc<T, 64, false>(prm, tmk, tmv, sms, s);
+    return cap ? launch_fa_tree_tc<T, 128, true>(prm, tmk, tmv, sms, s)
+               : launch_fa_tree_tc<T, 128, false>(prm, tmk, tmv, sms, s);
 }
 
 }  // namespace
@@ -222,7 +250,9 @@ p100_status p100_fa_tree(const p100_paged_desc* desc, const void* q, const void*
         return set_error(P100_ERR_INVALID, "q, o and the pages must be 16-byte aligned");
     prm.d.causal = 0;
     prm.d.max_q = std::min(prm.d.max_q, 32 * mask_words);
-    if (fa_paged_too_long(prm.d, fap::kRows, fap::kKeys, fap::kOver))
+    const bool on_tc = fa_tree_on_tc(prm.d);
+    if (on_tc ? fa_paged_too_long(prm.d, fatr::kRows, fatr::kKeys, fatr::kOver)
+              : fa_paged_too_long(prm.d, fap::kRows, fap::kKeys, fap::kOver))
         return set_error(P100_ERR_INVALID, "max_q x max_pages x page_size is too long for one call");
     const FaPagedWs w = fa_paged_ws(*desc, sms);
     if (ws_bytes < w.total || !ws)
@@ -245,6 +275,34 @@ p100_status p100_fa_tree(const p100_paged_desc* desc, const void* q, const void*
     prm.ws_ml = reinterpret_cast<float*>(at + w.tickets + w.o);
     prm.scale = desc->scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(desc->head_dim)) : desc->scale;
     prm.softcap = desc->softcap;
+    if (on_tc) {
+        fatr::Params t = {};
+        t.d = prm.d;
+        t.q = prm.q;
+        t.o = prm.o;
+        t.o_f32 = prm.o_f32;
+        t.lse = prm.lse;
+        t.ws_o = prm.ws_o;
+        t.ws_ml = prm.ws_ml;
+        t.tickets = prm.tickets;
+        t.scale = prm.scale;
+        t.softcap = prm.softcap;
+        t.k = k_pages;
+        t.v = v_pages;
+        t.mask = mask;
+        t.words = mask_words;
+        // boxes of whole rows where 16 or more divide a page, else gathered rows (as p100_fa_paged)
+        t.box = std::min(fatr::kKeys, prm.d.page_size & -prm.d.page_size);
+        CUtensorMap tmk = {}, tmv = {};
+        if (t.box < 16) {
+            t.box = 0;
+        } else {
+            if (p100_status st = page_map(&tmk, k_pages, *desc, prm.d, t.box)) return st;
+            if (p100_status st = page_map(&tmv, v_pages, *desc, prm.d, t.box)) return st;
+        }
+        return desc->dtype == P100_F16 ? launch_fa_tree_tc_d<__half>(t, desc->head_dim, tmk, tmv, sms, stream)
+                                       : launch_fa_tree_tc_d<__nv_bfloat16>(t, desc->head_dim, tmk, tmv, sms, stream);
+    }
     return desc->dtype == P100_F16 ? launch_fa_tree_mma_d<__half>(prm, desc->head_dim, sms, stream)
                                    : launch_fa_tree_mma_d<__nv_bfloat16>(prm, desc->head_dim, sms, stream);
 }
