@@ -83,6 +83,7 @@ p100_status launch_fa_tree_mma_d(const fap::Params& prm, int head_dim, int sms, 
     return spare ? launch_fa_tree_mma<T, 128, true>(prm, sms, s) : launch_fa_tree_mma<T, 128, false>(prm, sms, s);
 }
 
+static_assert(sizeof(fatr::Cut) <= kCutBytes && fatr::kRows <= fatc::kRows, "workspace");
 template <typename T, int D, bool CAP>
 p100_status launch_fa_tree_tc(const fatr::Params& prm, const CUtensorMap& tmk, const CUtensorMap& tmv, int sms,
                               cudaStream_t stream) {
@@ -92,8 +93,19 @@ p100_status launch_fa_tree_tc(const fatr::Params& prm, const CUtensorMap& tmk, c
     if (p100_status st = allow_smem(kern, fixed + paged::Lengths::bytes(paged::kMaxSeq), configured,
                                     "cudaFuncSetAttribute(fa_tree)"))
         return st;
-    kern<<<sms, fatr::kThreads, fixed + paged::Lengths::bytes(prm.d.n_seq), stream>>>(prm, tmk, tmv);
-    return cuda_status(cudaGetLastError(), "fa_tree_kernel launch");
+    const size_t lengths = paged::Lengths::bytes(prm.d.n_seq);
+    kern<<<sms, fatr::kThreads, fixed + lengths, stream>>>(prm, tmk, tmv);
+    if (p100_status st = cuda_status(cudaGetLastError(), "fa_tree_kernel launch")) return st;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute dependent = {};
+    dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    dependent.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(sms);
+    cfg.blockDim = dim3(fatr::kJoinThreads);
+    cfg.stream = stream;
+    cfg.attrs = &dependent;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, fatr::fa_tree_join_kernel<T, D>, prm, sms), "fa_tree_join_kernel launch");
 }
 template <typename T>
 p100_status launch_fa_tree_tc_d(const fatr::Params& prm, int head_dim, const CUtensorMap& tmk, const CUtensorMap& tmv,
@@ -251,6 +263,7 @@ p100_status p100_fa_tree(const p100_paged_desc* desc, const void* q, const void*
     prm.d.causal = 0;
     prm.d.max_q = std::min(prm.d.max_q, 32 * mask_words);
     const bool on_tc = fa_tree_on_tc(prm.d);
+    if (sms > fatr::kJoinThreads) return set_error(P100_ERR_UNSUPPORTED, "more SMs than the joining kernel expects");
     if (on_tc ? fa_paged_too_long(prm.d, fatr::kRows, fatr::kKeys, fatr::kOver)
               : fa_paged_too_long(prm.d, fap::kRows, fap::kKeys, fap::kOver))
         return set_error(P100_ERR_INVALID, "max_q x max_pages x page_size is too long for one call");
@@ -284,7 +297,7 @@ p100_status p100_fa_tree(const p100_paged_desc* desc, const void* q, const void*
         t.lse = prm.lse;
         t.ws_o = prm.ws_o;
         t.ws_ml = prm.ws_ml;
-        t.tickets = prm.tickets;
+        t.cuts = reinterpret_cast<fatr::Cut*>(at + w.tickets + w.o + w.ml);
         t.scale = prm.scale;
         t.softcap = prm.softcap;
         t.k = k_pages;

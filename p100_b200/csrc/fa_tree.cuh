@@ -19,11 +19,14 @@
 //                   no multiple of 16 tokens
 //
 // At the end of an item the warpgroups exchange their statistics and each joins
-// one half of the accumulators' columns; parts of a row tile cut by the shares
-// are joined through the workspace as fa_paged_tc.cuh's are.
+// one half of the accumulators' columns.  Parts of a row tile cut by the shares
+// are left in the workspace, and a second kernel joins them.
 //
-// The probabilities go to the tensor cores in two 16-bit parts (the rounding and
-// what it left), both in the scores' place in tensor memory.
+// The probabilities are rounded once to the cache's 16-bit type, as fa_paged_tc.cuh
+// does and for its reason: a second part (what the rounding left) would be half as
+// many products again, and both the products and the energy they take count here
+// (48 trees of 8 over 8192 tokens: 147 us, with two parts 180, at the 1000 W cap
+// that streaming the cache alone comes near).
 #pragma once
 #include "fa_paged_tc.cuh"
 
@@ -54,6 +57,13 @@ constexpr int kMmaWarp = fatc::kMmaWarp, kLoadWarp = fatc::kLoadWarp, kGatherWar
 template <int D>
 __host__ __device__ constexpr int slots() { return D == 128 ? 5 : 8; }
 
+// The row tile that a CTA begins and others end, as the joining kernel gets it.
+struct Cut {
+    int last;                    // CTA of the last part; the CTA itself: none
+    int q0, row0, rows, head;    // the sequence's first token; first row, rows of the tile; kv head
+    int pad[3];
+};
+
 struct Params {
     Desc d;
     const void* q;
@@ -62,7 +72,7 @@ struct Params {
     float* lse;
     float* ws_o;        // [CTAs][2][D / 4][128] float4
     float* ws_ml;       // [CTAs][2][128] float2
-    unsigned* tickets;  // [CTAs]
+    Cut* cuts;          // [CTAs]
     float scale, softcap;
     int box;            // rows of a TMA box, 0: gathered rows
     const void *k, *v;
@@ -71,10 +81,9 @@ struct Params {
 };
 
 struct Barriers {
-    uint64_t full[8], empty[8], q_full, s_full[2], p_full[2][2], stats, o_free, joined, job_full[kJobs], job_empty[kJobs], drain;
+    uint64_t full[8], empty[8], q_full, s_full[2], p_full[2][2], stats, o_free, job_full[kJobs], job_empty[kJobs], drain;
     uint32_t tmem;
     int abort;
-    int last;
     Job jobs[kJobs];
     float2 ml[2][kRows];   // the warpgroups' maxima and sums
 };
@@ -287,14 +296,11 @@ __device__ __forceinline__ bool mma_role(const Desc& d, float scale, Barriers& b
         fatc::mma_commit(&bars.s_full[w]);
         fatc::mma_commit(&bars.empty[slot]);
     };
-    auto pv = [&](int w, int half, unsigned slot, bool add) {   // O_w += P_w V over half of the keys, both parts of P
+    auto pv = [&](int w, int half, unsigned slot, bool add) {   // O_w += P_w V over half of the keys
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
-#pragma unroll
-            for (int k = half * (kKeys / 32); k < (half + 1) * (kKeys / 32); ++k)
-                fatc::mma_ts(tmem + 256 + w * D, tmem + w * 128 + part * 64 + k * 8,
-                             fatc::sw128_desc(ring + slot * tile_bytes<D>() + uint32_t(k) * 2048, kSub, 1024), kIdescO,
-                             add || part > 0 || k > 0);
+        for (int k = half * (kKeys / 32); k < (half + 1) * (kKeys / 32); ++k)
+            fatc::mma_ts(tmem + 256 + w * D, tmem + w * 128 + k * 8,
+                         fatc::sw128_desc(ring + slot * tile_bytes<D>() + uint32_t(k) * 2048, kSub, 1024), kIdescO, add || k > 0);
     };
     for (unsigned j = 0;; ++j) {
         if (!warp_wait(&bars.job_full[j % kJobs], (j / kJobs) & 1, &bars.abort)) return false;
@@ -375,6 +381,30 @@ __device__ __forceinline__ uint32_t seen32(const unsigned* row, int words, int k
         bits = __funnelshift_r(lo, hi, node & 31);
     }
     return left < 32 ? bits & ((1u << left) - 1) : bits;
+}
+
+// Values of a row over their sum, to o.
+template <typename T, int N>
+__device__ __forceinline__ void write_row(const Params& p, const float (&o)[N], long long at, float sum) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (p.o_f32) {
+        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.o) + at);
+#pragma unroll
+        for (int e = 0; e < N; e += 4) dst[e / 4] = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+    } else if constexpr (N == 4) {
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + at) =
+            make_uint2(paged::pack2<T>(o[0] * inv, o[1] * inv), paged::pack2<T>(o[2] * inv, o[3] * inv));
+    } else {
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.o) + at);
+#pragma unroll
+        for (int e = 0; e < N; e += 8)
+            dst[e / 8] = make_uint4(paged::pack2<T>(o[e] * inv, o[e + 1] * inv), paged::pack2<T>(o[e + 2] * inv, o[e + 3] * inv),
+                                    paged::pack2<T>(o[e + 4] * inv, o[e + 5] * inv), paged::pack2<T>(o[e + 6] * inv, o[e + 7] * inv));
+    }
+}
+__device__ __forceinline__ void write_lse(const Params& p, int token, int head, float top, float sum) {
+    if (p.lse)
+        p.lse[(long long)token * p.d.n_head_q + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) / 1.4426950408889634f;
 }
 
 template <typename T, int D, bool CAP>
@@ -504,7 +534,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
             for (int half = 0; half < 2; ++half) {   // the products with the first half start while the second is computed
 #pragma unroll
                 for (int i = 4 * half; i < 4 * half + 4; ++i) {
-                    uint32_t pk[8], rest[8];
+                    uint32_t pk[8];
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
                         const uint64_t x = pair(s[i * 16 + e], s[i * 16 + e + 1]);
@@ -515,17 +545,15 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
 #pragma unroll
                             for (int n = 3; n >= 0; --n) f = fma2(z, f, pair(k[n], k[n]));
                         }
-                        float a, b, ha, hb;
+                        float a, b;
                         unpair(fma2(x, f, b2), a, b);
                         a = paged::exp2_approx(a);
                         b = paged::exp2_approx(b);
                         sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair(a, b));
                         pk[e >> 1] = paged::pack2<T>(a, b);
-                        paged::unpack2<T>(pk[e >> 1], ha, hb);
-                        rest[e >> 1] = paged::pack2<T>(a - ha, b - hb);
                     }
                     fatc::st8(t_s + i * 8, pk);
-                    fatc::st8(t_s + 64 + i * 8, rest);
+                    
                 }
                 fatc::wait_st();
                 fatc::fence_before();
@@ -571,80 +599,22 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
         fatc::fence_before();
         mbar_arrive(&bars.o_free);
         const long long o_at = r.at(d, job, d.o_stride, D) + w * kCols;
-        auto write = [&](float inv) {
-            if (!r.live) return;
-#pragma unroll
-            for (int e = 0; e < kCols; ++e) o[e] *= inv;
-            if (p.o_f32) {
-                float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.o) + o_at);
-#pragma unroll
-                for (int e = 0; e < kCols / 4; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-            } else {
-                uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.o) + o_at);
-#pragma unroll
-                for (int e = 0; e < kCols / 8; ++e)
-                    dst[e] = make_uint4(paged::pack2<T>(o[8 * e], o[8 * e + 1]), paged::pack2<T>(o[8 * e + 2], o[8 * e + 3]),
-                                        paged::pack2<T>(o[8 * e + 4], o[8 * e + 5]), paged::pack2<T>(o[8 * e + 6], o[8 * e + 7]));
-            }
-        };
-        auto write_lse = [&](float most, float all) {
-            if (w == 0 && r.live && p.lse)
-                p.lse[(long long)(job.q0 + r.tok) * d.n_head_q + job.head * d.group + r.g] =
-                    all == 0.f ? -INFINITY : (most + log2f(all)) / kLog2e;
-        };
         if (job.whole) {
-            write(total == 0.f ? 0.f : 1.f / total);
-            write_lse(top, total);
-        } else {
-            // the CTAs that have a part
-            const int c0 = paged::share_of(job.first, total_units, parts), c1 = paged::share_of(job.first + job.units - 1, total_units, parts);
-            const long long slot = blockIdx.x * 2 + (job.key_tile == 0);
-            float4* dst = reinterpret_cast<float4*>(p.ws_o) + (slot * (D / 4) + w * (kCols / 4)) * 128 + row;
             if (r.live) {
-#pragma unroll
-                for (int e = 0; e < kCols / 4; ++e)
-                    __stcg(dst + e * 128, make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
-                if (w == 0) __stcg(reinterpret_cast<float2*>(p.ws_ml) + slot * 128 + row, make_float2(top, total));
+                write_row<T>(p, o, o_at, total);
+                if (w == 0) write_lse(p, job.q0 + r.tok, job.head * d.group + r.g, top, total);
             }
-            // one thread takes the ticket when all have written
-            __threadfence();
-            mbar_arrive(&bars.joined);
-            if (!warp_wait(&bars.joined, 0, &bars.abort)) return;
-            if (threadIdx.x == 0) bars.last = atomicAdd(p.tickets + c0, 1u) == unsigned(c1 - c0);
-            mbar_arrive(&bars.joined);
-            if (!warp_wait(&bars.joined, 1, &bars.abort)) return;
-            if (bars.last) {   // join the parts in share order
-                __threadfence();
-                if (threadIdx.x == 0) p.tickets[c0] = 0;   // ready for the next call
-                if (r.live) {
-                    const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + row;
-                    const float4* po = reinterpret_cast<const float4*>(p.ws_o) + w * (kCols / 4) * 128 + row;
-                    auto part = [&](int q) { return (long long)q * 2 + (q == c0); };
-                    float most = -INFINITY, all = 0.f;
-#pragma unroll 4
-                    for (int q = c0; q <= c1; ++q) most = fmaxf(most, __ldcg(ml + part(q) * 128).x);
-                    const float ground = most == -INFINITY ? 0.f : most;
+        } else if (r.live) {   // a part for fa_tree_join_kernel
+            const long long slot = blockIdx.x * 2 + (job.key_tile == 0);
+            float4* dst = reinterpret_cast<float4*>(p.ws_o) + (slot * (D / 4) + w * (kCols / 4)) * kRows + row;
 #pragma unroll
-                    for (int e = 0; e < kCols; ++e) o[e] = 0.f;
-#pragma unroll 1
-                    for (int q = c0; q <= c1; ++q) {
-                        const float2 v = __ldcg(ml + part(q) * 128);
-                        const float f = paged::exp2_approx(v.x - ground);
-                        all = fmaf(f, v.y, all);
-#pragma unroll
-                        for (int e = 0; e < kCols / 4; ++e) {
-                            const float4 x = __ldcg(po + (part(q) * (D / 4) + e) * 128);
-                            o[4 * e] = fmaf(f, x.x, o[4 * e]);
-                            o[4 * e + 1] = fmaf(f, x.y, o[4 * e + 1]);
-                            o[4 * e + 2] = fmaf(f, x.z, o[4 * e + 2]);
-                            o[4 * e + 3] = fmaf(f, x.w, o[4 * e + 3]);
-                        }
-                    }
-                    write(all == 0.f ? 0.f : 1.f / all);
-                    write_lse(most, all);
-                }
-            }
+            for (int e = 0; e < kCols / 4; ++e)
+                __stcg(dst + e * kRows, make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
+            if (w == 0) __stcg(reinterpret_cast<float2*>(p.ws_ml) + slot * kRows + row, make_float2(top, total));
         }
+        if (threadIdx.x == 0 && !job.whole && job.key_tile == 0)
+            p.cuts[blockIdx.x] = {paged::share_of(job.first + job.units - 1, total_units, parts), job.q0, job.row0,
+                                  min(kRows, job.n * d.group - job.row0), job.head, {}};
         __syncwarp();
         if ((row & 31) == 0) mbar_arrive(&bars.job_empty[j % kJobs]);
     }
@@ -661,6 +631,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Lengths len(reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(&bars + 1) + 15) & ~uintptr_t(15)), p.d.n_seq);
     const int warp = threadIdx.x >> 5;
 
+    pdl_allow_dependents();   // the joining kernel, which waits for this one's end
+    if (threadIdx.x == 0) p.cuts[blockIdx.x].last = blockIdx.x;
     if (threadIdx.x == kLoadWarp * 32 && p.box) {
         prefetch_tensormap(&tmk);
         prefetch_tensormap(&tmv);
@@ -686,7 +658,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&bars.q_full, 256);
         mbar_init(&bars.stats, 256);
         mbar_init(&bars.o_free, 256);
-        mbar_init(&bars.joined, 256);
     } else if (threadIdx.x == 31) {
         mbar_init(&bars.drain, 1);
         bars.abort = 0;
@@ -729,6 +700,104 @@ __global__ void __launch_bounds__(kThreads, 1)
     fatc::fence_after();
     if (warp == kMmaWarp)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// ------------------------------------------------------------ join
+// Row tiles cut by the shares: 32 rows x 4 COLS columns of the parts are a warp's
+// item, joined in share order, and the items of all cuts are dealt out over the
+// warps of all CTAs.  (The last CTA of a row tile to finish would read its parts
+// at one SM's rate: those of one tree over 4096 keys, 19 of 32 KB, in 10 us.)
+// What it costs is a few round trips to the L2: the cuts, then PARTS parts in
+// each; a cut of few parts has wider items instead.
+constexpr int kJoinThreads = 512, kFewParts = 3;
+template <typename T, int D, int COLS, int PARTS>
+__device__ __forceinline__ void join_item(const Params& p, const Cut& cut, int c0, int row, int col) {
+    const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + row;
+    const float4* po = reinterpret_cast<const float4*>(p.ws_o) + col * kRows + row;
+    const bool live = row < cut.rows;
+    float top = -INFINITY, sum = 0.f, o[COLS][4] = {};
+    for (int q0 = c0; q0 <= cut.last; q0 += PARTS) {
+        float2 st[PARTS];
+        float4 x[PARTS][COLS];
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) {
+            const long long part = (long long)(q0 + k) * 2 + (q0 + k == c0);
+            const bool in = live && q0 + k <= cut.last;
+            st[k] = in ? __ldcg(ml + part * kRows) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int i = 0; i < COLS; ++i)
+                x[k][i] = in ? __ldcg(po + (part * (D / 4) + i) * kRows) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        const float before = top;
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) top = fmaxf(top, st[k].x);
+        const float safe = top == -INFINITY ? 0.f : top, a = paged::exp2_approx(before - safe);
+        sum *= a;
+#pragma unroll
+        for (int i = 0; i < COLS; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] *= a;
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) {
+            const float f = paged::exp2_approx(st[k].x - safe);
+            sum = fmaf(f, st[k].y, sum);
+#pragma unroll
+            for (int i = 0; i < COLS; ++i) {
+                o[i][0] = fmaf(f, x[k][i].x, o[i][0]);
+                o[i][1] = fmaf(f, x[k][i].y, o[i][1]);
+                o[i][2] = fmaf(f, x[k][i].z, o[i][2]);
+                o[i][3] = fmaf(f, x[k][i].w, o[i][3]);
+            }
+        }
+    }
+    if (!live) return;
+    const Desc& d = p.d;
+    const int r = cut.row0 + row, tok = r / d.group, head = cut.head * d.group + (r - tok * d.group), token = cut.q0 + tok;
+#pragma unroll
+    for (int i = 0; i < COLS; ++i)
+        write_row<T>(p, o[i], (long long)token * d.o_stride + (long long)head * D + (col + i) * 4, sum);
+    if (col == 0) write_lse(p, token, head, top, sum);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) fa_tree_join_kernel(const Params p, int ctas) {
+    __shared__ int s_first[kJoinThreads];   // items before a CTA's cut
+    __shared__ int s_warp[kJoinThreads / 32];
+    constexpr int kWide = 4;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_wait_prior_grid();
+    int own = 0;
+    if (tid < ctas && p.cuts[tid].last != tid)
+        own = (p.cuts[tid].rows + 31) / 32 * (D / 4) / (p.cuts[tid].last - tid < kFewParts ? kWide : 1);
+    int v = own;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, off);
+        if (lane >= off) v += u;
+    }
+    if (lane == 31) s_warp[warp] = v;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int i = 0; i < kJoinThreads / 32; ++i) {
+        if (i < warp) v += s_warp[i];
+        total += s_warp[i];
+    }
+    s_first[tid] = v - own;
+    __syncthreads();
+    for (int item = warp * gridDim.x + blockIdx.x; item < total; item += gridDim.x * (kJoinThreads / 32)) {
+        int c0 = 0, hi = ctas - 1;   // the last CTA whose first item is at or before this one
+        while (c0 < hi) {
+            const int mid = (c0 + hi + 1) >> 1;
+            if (s_first[mid] <= item) c0 = mid; else hi = mid - 1;
+        }
+        const Cut cut = p.cuts[c0];
+        const int at = item - s_first[c0];
+        if (cut.last - c0 < kFewParts)
+            join_item<T, D, kWide, kFewParts>(p, cut, c0, at / (D / 4 / kWide) * 32 + lane, at % (D / 4 / kWide) * kWide);
+        else
+            join_item<T, D, 1, 10>(p, cut, c0, at / (D / 4) * 32 + lane, at % (D / 4));
+    }
 }
 
 }  // namespace fatr

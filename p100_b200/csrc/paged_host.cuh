@@ -81,10 +81,11 @@ bool fa_paged_too_long(const paged::Desc& d, int rows, int keys, int over) {
     return tiles * (double(d.max_pages) * d.page_size / keys + 1 + over) >= 4294967295.0;
 }
 
-// Partials of both kernels share one place: their calls follow one another.
+// Partials of all kernels share one place: their calls follow one another.
 struct FaPagedWs {
-    size_t tickets, o, ml, total;
+    size_t tickets, o, ml, cuts, total;
 };
+constexpr size_t kCutBytes = 32;   // of the tree kernel's note on a cut row tile
 size_t fa_paged_ticket_bytes(int sms) { return round256(size_t(sms) * kMmaCtas * 2 * sizeof(unsigned)); }
 FaPagedWs fa_paged_ws(const p100_paged_desc& in, int sms) {
     const size_t rows = size_t(sms) * 2 * std::max(kMmaCtas * fap::kRows, fatc::kRows);
@@ -92,7 +93,8 @@ FaPagedWs fa_paged_ws(const p100_paged_desc& in, int sms) {
     w.tickets = fa_paged_ticket_bytes(sms);   // first, so that init clears little
     w.o = round256(rows * in.head_dim * sizeof(float));
     w.ml = round256(rows * 2 * sizeof(float));
-    w.total = w.tickets + w.o + w.ml;
+    w.cuts = round256(size_t(sms) * kCutBytes);
+    w.total = w.tickets + w.o + w.ml + w.cuts;
     return w;
 }
 
