@@ -60,8 +60,15 @@ const char* words_reason(int mask_words) {
     return mask_words < 1 || mask_words > P100_TREE_MAX_WORDS ? "mask_words must be between 1 and 32" : nullptr;
 }
 
-bool fa_tree_on_tc(const paged::Desc& d) {
-    return (long long)d.max_q * d.group > fap::kRows && d.n_pages > 0;
+// The tensor-core kernel takes all but the smallest trees.  Two tokens of 48
+// sequences of 8192 (64 / 8 heads: 16 rows a kv head) 163 us, on the mma.sync
+// kernel 179; of one sequence of 4096 (32 / 8 heads) with four tokens 16.6 and 23.2;
+// up to 8 rows that kernel's half-empty products are the cheaper ones (one token
+// of the 48: 181 and 176; 64 sequences of 512 with 32 heads and 8 tokens 111 and
+// 82), and with heads of 64, whose tiles are half as long, up to 16 (13 trees of 5
+// over 3001: 25 and 22).
+bool fa_tree_on_tc(const paged::Desc& d, int head_dim) {
+    return (long long)d.max_q * d.group > (head_dim == 64 ? fap::kRows : fap::kRows / 2);
 }
 
 template <typename T, int D, bool SPARE>
@@ -77,10 +84,10 @@ p100_status launch_fa_tree_mma(const fap::Params& prm, int sms, cudaStream_t str
 }
 template <typename T>
 p100_status launch_fa_tree_mma_d(const fap::Params& prm, int head_dim, int sms, cudaStream_t s) {
-    const bool spare = (long long)prm.d.max_q * prm.d.group <= fap::kRows / 2;
-    if (head_dim == 64)
-        return spare ? launch_fa_tree_mma<T, 64, true>(prm, sms, s) : launch_fa_tree_mma<T, 64, false>(prm, sms, s);
-    return spare ? launch_fa_tree_mma<T, 128, true>(prm, sms, s) : launch_fa_tree_mma<T, 128, false>(prm, sms, s);
+    if (head_dim == 128) return launch_fa_tree_mma<T, 128, true>(prm, sms, s);
+    // 8 rows a kv head or fewer: the second parts of their probabilities take the other 8
+    return (long long)prm.d.max_q * prm.d.group <= fap::kRows / 2 ? launch_fa_tree_mma<T, 64, true>(prm, sms, s)
+                                                                  : launch_fa_tree_mma<T, 64, false>(prm, sms, s);
 }
 
 static_assert(sizeof(fatr::Cut) <= kCutBytes && fatr::kRows <= fatc::kRows, "workspace");
@@ -262,7 +269,7 @@ p100_status p100_fa_tree(const p100_paged_desc* desc, const void* q, const void*
         return set_error(P100_ERR_INVALID, "q, o and the pages must be 16-byte aligned");
     prm.d.causal = 0;
     prm.d.max_q = std::min(prm.d.max_q, 32 * mask_words);
-    const bool on_tc = fa_tree_on_tc(prm.d);
+    const bool on_tc = fa_tree_on_tc(prm.d, desc->head_dim);
     if (sms > fatr::kJoinThreads) return set_error(P100_ERR_UNSUPPORTED, "more SMs than the joining kernel expects");
     if (on_tc ? fa_paged_too_long(prm.d, fatr::kRows, fatr::kKeys, fatr::kOver)
               : fa_paged_too_long(prm.d, fap::kRows, fap::kKeys, fap::kOver))
@@ -307,7 +314,7 @@ p100_status p100_fa_tree(const p100_paged_desc* desc, const void* q, const void*
         // boxes of whole rows where 16 or more divide a page, else gathered rows (as p100_fa_paged)
         t.box = std::min(fatr::kKeys, prm.d.page_size & -prm.d.page_size);
         CUtensorMap tmk = {}, tmv = {};
-        if (t.box < 16) {
+        if (t.box < 16 || desc->n_pages == 0) {
             t.box = 0;
         } else {
             if (p100_status st = page_map(&tmk, k_pages, *desc, prm.d, t.box)) return st;

@@ -250,7 +250,7 @@ __device__ __forceinline__ void gather_role(const Params& p, Barriers& bars, uin
                 fap::cp_async16(slot + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), from + (o < 0 ? 0 : o), o >= 0);
             }
             fap::cp_commit();
-            if (used > item0) {
+            if (used > item0) {   // (three slots' copies in flight were no faster)
                 fap::cp_wait<1>();
                 announce(used - 1);
             }
@@ -436,22 +436,26 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
         const unsigned* bits = p.mask + (long long)(job.q0 + (r.live ? r.tok : 0)) * p.words;
         const bool any_row = (row & ~31) < job.n * d.group - job.row0;   // of the warp
         float m = -INFINITY, l = 0.f;
+        // Zeroes the rows of V behind the last key, before the products of tile t.
+        auto clear_v = [&](int t, int key0) {
+            if (job.end - key0 >= kKeys) return true;
+            const unsigned u = used + v_at(t, count);
+            if (!warp_wait(&bars.full[u % NS], (u / NS) & 1, &bars.abort)) return false;
+            if (row >= job.end - key0) {
+                uint8_t* v = ring + (u % NS) * tile_bytes<D>() + row * 128;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i)
+                    *reinterpret_cast<uint4*>(v + (i >> 3) * kSub + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fatc::fence_async();
+            return true;
+        };
         for (int t = w; t < count; t += 2) {
             const int key0 = (job.key_tile + t) * kKeys;   // key0 + kKeys may pass 2^31
             if (!warp_wait(&bars.s_full[w], done++ & 1, &bars.abort)) return;
             fatc::fence_after();
-            if (job.end - key0 < kKeys) {   // rows of V behind the last key
-                const unsigned u = used + v_at(t, count);
-                if (!warp_wait(&bars.full[u % NS], (u / NS) & 1, &bars.abort)) return;
-                if (row >= job.end - key0) {
-                    uint8_t* v = ring + (u % NS) * tile_bytes<D>() + row * 128;
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i)
-                        *reinterpret_cast<uint4*>(v + (i >> 3) * kSub + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-                }
-                fatc::fence_async();
-            }
             if (!any_row) {   // the products of these rows go nowhere
+                if (!clear_v(t, key0)) return;
                 mbar_arrive(&bars.p_full[w][0]);
                 mbar_arrive(&bars.p_full[w][1]);
                 continue;
@@ -556,6 +560,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
                     
                 }
                 fatc::wait_st();
+                if (half == 0 && !clear_v(t, key0)) return;
                 fatc::fence_before();
                 mbar_arrive(&bars.p_full[w][half]);
             }

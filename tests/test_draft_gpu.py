@@ -522,6 +522,21 @@ def test_chain_is_causal_attention(cuda, q_lens, kv_lens):
     assert bool(((o - o1).abs() <= 5 * 2.0 ** -10).all()) and bool(((lse - lse1).abs() <= 2.0 ** -16 * (1 + lse.abs())).all())
 
 
+@pytest.mark.parametrize("dim,group", [(64, 4), (128, 2), (128, 8)])
+def test_tree_without_pages(cuda, dim, group):
+    """A cache without a page: trees whose masks are empty in sequences of no length give 0 and -inf."""
+    torch = cuda
+    d = P.PagedDesc(n_seq=2, n_tokens=7, max_q=4, n_head_q=2 * group, n_head_kv=2, page_size=16, n_pages=0, max_pages=1,
+                    head_dim=dim)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    k = torch.zeros(8, dtype=torch.float16, device="cuda")
+    q = torch.ones(7, 2 * group, dim, dtype=torch.float16, device="cuda")
+    o, lse = P.fa_tree(d, q, k, k, torch.full((7, 1), -1, **i32), torch.full((2, 1), -1, **i32), torch.tensor([0, 3, 7], **i32),
+                       torch.zeros(2, **i32))
+    P.check(P.device_error())
+    assert bool((o == 0).all()) and bool(torch.isneginf(lse).all())
+
+
 def test_tree_reports_too_many_tokens(cuda):
     b = Batch(cuda, [33, 2], [50, 60], 4, 1, 64, "f16", 16)
     b.fill()
