@@ -55,6 +55,18 @@ const char* rope_reason(const p100_rope* rope, const p100_paged_desc* desc) {
     return nullptr;
 }
 
+struct AppendRopeLaunch {
+    const paged::AppendParams& prm;
+    const paged::TurnParams turns;
+    unsigned blocks;
+    cudaStream_t stream;
+    template <typename S, typename T, int D>
+    p100_status operator()() const {
+        paged::append_rope_kernel<S, T, D><<<blocks, paged::kAppendThreads, 0, stream>>>(prm, turns);
+        return cuda_status(cudaGetLastError(), "append_rope_kernel launch");
+    }
+};
+
 // ------------------------------------------------------------ trees
 const char* words_reason(int mask_words) {
     return mask_words < 1 || mask_words > P100_TREE_MAX_WORDS ? "mask_words must be between 1 and 32" : nullptr;
@@ -247,8 +259,8 @@ p100_status p100_paged_append_rope(const p100_paged_desc* desc, const void* qkv,
                                        block_table, q_start, kv_len, q, k_pages, v_pages, prm, blocks))
         return st;
     if (!blocks) return P100_OK;
-    return launch_append_from<paged::ByTurns>(prm, paged::TurnParams{*rope, position}, qkv_type, desc->dtype,
-                                              desc->head_dim, blocks, stream);
+    return append_typed(qkv_type, desc->dtype, desc->head_dim,
+                        AppendRopeLaunch{prm, paged::TurnParams{*rope, position}, blocks, stream});
 }
 
 p100_status p100_fa_tree(const p100_paged_desc* desc, const void* q, const void* k_pages, const void* v_pages,

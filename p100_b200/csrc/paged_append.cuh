@@ -4,8 +4,7 @@
 //
 // Per head x of a token at position p: x' = x w / sqrt(mean(x^2) + eps) (with
 // norm weights), then for each pair (a, b): (a cos - b sin, a sin + b cos)
-// with the angle of p, from a table (ByTable) or computed from the pair's
-// frequency (ByTurns, rope.cuh); pairs are adjacent values, or value i with
+// with the table's angle of p; pairs are adjacent values, or value i with
 // value i + D/2.  All in FP32; the one rounding is the store to 16 bits.
 //
 // Bytes bound it: every value is read once and written once.  A lane takes the
@@ -41,7 +40,7 @@ struct AppendParams {
     const float* q_norm;    // [D] or null
     const float* k_norm;
     float eps;
-    const float2* rope;     // [max_pos][D/2] or null (ByTable)
+    const float2* rope;     // [max_pos][D/2] or null
     int max_pos, half;
     int warps;              // that share a token
     void *q, *k, *v;
@@ -89,54 +88,8 @@ __device__ __forceinline__ int find_seq(const Desc& d, int t, int& q0, int& q1, 
     return q0 <= t && t < q1 ? lo + k : -1;
 }
 
-struct NoParams {};
-// The rotation by the table of AppendParams, as a lane holds it: the cosines
-// and sines of its values' pairs, adjacent ones (cs[0 .. E / 2)) or with the
-// partner lane's.
-template <int E, int D>
-struct ByTable {
-    using Params = NoParams;
-    static constexpr int kLanes = D / E;
-    float2 cs[E];
-    bool second;
-
-    __device__ __forceinline__ bool begin(const AppendParams& p, const Params&, int, int pos, int in_head) {
-        if (p.rope && pos >= p.max_pos) return false;
-        second = in_head >= kLanes / 2;
-        if (p.rope) {
-            const float2* c = p.rope + (long long)pos * (D / 2);
-            if (p.half) {
-#pragma unroll
-                for (int i = 0; i < E; ++i) cs[i] = c[in_head % (kLanes / 2) * E + i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < E / 2; ++i) cs[i] = c[in_head * (E / 2) + i];
-            }
-        }
-        return true;
-    }
-    __device__ __forceinline__ bool turns(const AppendParams& p, const Params&) const { return p.rope; }
-    __device__ __forceinline__ void turn(const AppendParams& p, const Params&, float (&y)[E]) const {
-        if (p.half) {
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const float o = __shfl_xor_sync(0xffffffffu, y[i], kLanes / 2);
-                y[i] = second ? o * cs[i].y + y[i] * cs[i].x : y[i] * cs[i].x - o * cs[i].y;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < E / 2; ++i) {
-                const float a = y[2 * i], b = y[2 * i + 1];
-                y[2 * i] = a * cs[i].x - b * cs[i].y;
-                y[2 * i + 1] = a * cs[i].y + b * cs[i].x;
-            }
-        }
-    }
-};
-
-template <typename S, typename T, int D, template <int, int> class ROT>
-__global__ void __launch_bounds__(kAppendThreads)
-    paged_append_kernel(const AppendParams p, const __grid_constant__ typename ROT<append_values<S>(), D>::Params r) {
+template <typename S, typename T, int D>
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendParams p) {
     constexpr int E = append_values<S>();
     constexpr int kLanes = D / E;              // of a head
     constexpr int kHeads = 32 / kLanes;        // of a step
@@ -172,10 +125,22 @@ __global__ void __launch_bounds__(kAppendThreads)
     if (seq < 0) return;   // a padding token
     const int pos = kv - (q1 - q0) + (t - q0);
     const int page_at = pos / p.d.page_size;
-    ROT<E, D> rot;
-    if (pos < 0 || page_at >= p.d.max_pages || !rot.begin(p, r, t, pos, in_head)) {
+    if (pos < 0 || page_at >= p.d.max_pages || (p.rope && pos >= p.max_pos)) {
         if (lane == 0) flag_input();
         return;
+    }
+    // pairs of the lane's values: adjacent ones (cs[0 .. E / 2)), or with the partner lane's
+    const bool second = in_head >= kLanes / 2;
+    float2 cs[E];
+    if (p.rope) {
+        const float2* c = p.rope + (long long)pos * (D / 2);
+        if (p.half) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) cs[i] = c[in_head % (kLanes / 2) * E + i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < E / 2; ++i) cs[i] = c[in_head * (E / 2) + i];
+        }
     }
     long long dst = 0;
     bool has_page = true;
@@ -189,7 +154,7 @@ __global__ void __launch_bounds__(kAppendThreads)
         const int base = first_of(kind), stop = min(end, first_of(kind + 1)) - base, from = at - base;
         const int heads = kind == 0 ? p.d.n_head_q : p.d.n_head_kv;
         const float* norm = kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr;
-        const bool turn = rot.turns(p, r) && kind < 2;
+        const bool turn = p.rope && kind < 2;
         const S* src = source(kind);
         if (at != begin) load(src, from, stop, heads);
         T* to = kind == 0 ? static_cast<T*>(p.q) + t * p.d.q_stride : static_cast<T*>(kind == 2 ? p.v : p.k) + dst;
@@ -221,7 +186,22 @@ __global__ void __launch_bounds__(kAppendThreads)
 #pragma unroll
                     for (int i = 0; i < E; ++i) y[i] = y[i] * r * w[i];
                 }
-                if (turn) rot.turn(p, r, y);
+                if (turn) {
+                    if (p.half) {
+#pragma unroll
+                        for (int i = 0; i < E; ++i) {
+                            const float o = __shfl_xor_sync(0xffffffffu, y[i], kLanes / 2);
+                            y[i] = second ? o * cs[i].y + y[i] * cs[i].x : y[i] * cs[i].x - o * cs[i].y;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < E / 2; ++i) {
+                            const float a = y[2 * i], b = y[2 * i + 1];
+                            y[2 * i] = a * cs[i].x - b * cs[i].y;
+                            y[2 * i + 1] = a * cs[i].y + b * cs[i].x;
+                        }
+                    }
+                }
                 if ((step + u) * kHeads + own < heads && (kind == 0 || has_page))
                     store_values<T, E>(to + (step + u) * kHeads * stride, y);
             }

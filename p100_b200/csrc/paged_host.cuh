@@ -179,28 +179,20 @@ p100_status append_params(const p100_paged_desc* desc, const void* qkv, int qkv_
     return P100_OK;
 }
 
-template <template <int, int> class ROT, typename S, typename T, int D, typename R>
-p100_status launch_append(const paged::AppendParams& prm, const R& rot, unsigned blocks, cudaStream_t stream) {
-    paged::paged_append_kernel<S, T, D, ROT><<<blocks, paged::kAppendThreads, 0, stream>>>(prm, rot);
-    return cuda_status(cudaGetLastError(), "paged_append_kernel launch");
-}
-template <template <int, int> class ROT, typename S, typename R>
-p100_status launch_append_to(const paged::AppendParams& prm, const R& rot, int dtype, int head_dim, unsigned blocks,
-                             cudaStream_t s) {
-    if (dtype == P100_F16)
-        return head_dim == 64 ? launch_append<ROT, S, __half, 64>(prm, rot, blocks, s)
-                              : launch_append<ROT, S, __half, 128>(prm, rot, blocks, s);
-    return head_dim == 64 ? launch_append<ROT, S, __nv_bfloat16, 64>(prm, rot, blocks, s)
-                          : launch_append<ROT, S, __nv_bfloat16, 128>(prm, rot, blocks, s);
-}
-// R: the rotation's parameters, the same for every type.
-template <template <int, int> class ROT, typename R>
-p100_status launch_append_from(const paged::AppendParams& prm, const R& rot, int qkv_type, int dtype, int head_dim,
-                               unsigned blocks, cudaStream_t s) {
+// An append kernel for the call's types: launch<S, T, D>() is given them.
+template <typename L>
+p100_status append_typed(int qkv_type, int dtype, int head_dim, const L& launch) {
+    auto to = [&](auto from) {
+        using S = decltype(from);
+        if (dtype == P100_F16)
+            return head_dim == 64 ? launch.template operator()<S, __half, 64>() : launch.template operator()<S, __half, 128>();
+        return head_dim == 64 ? launch.template operator()<S, __nv_bfloat16, 64>()
+                              : launch.template operator()<S, __nv_bfloat16, 128>();
+    };
     switch (qkv_type) {
-        case P100_F32: return launch_append_to<ROT, float>(prm, rot, dtype, head_dim, blocks, s);
-        case P100_F16: return launch_append_to<ROT, __half>(prm, rot, dtype, head_dim, blocks, s);
-        default: return launch_append_to<ROT, __nv_bfloat16>(prm, rot, dtype, head_dim, blocks, s);
+        case P100_F32: return to(float());
+        case P100_F16: return to(__half());
+        default: return to(__nv_bfloat16());
     }
 }
 

@@ -73,6 +73,17 @@ p100_status launch_fa_paged_mma_d(const fap::Params& prm, int head_dim, int sms,
     return spare ? launch_fa_paged_mma<T, 128, true>(prm, sms, s) : launch_fa_paged_mma<T, 128, false>(prm, sms, s);
 }
 
+struct AppendLaunch {
+    const paged::AppendParams& prm;
+    unsigned blocks;
+    cudaStream_t stream;
+    template <typename S, typename T, int D>
+    p100_status operator()() const {
+        paged::paged_append_kernel<S, T, D><<<blocks, paged::kAppendThreads, 0, stream>>>(prm);
+        return cuda_status(cudaGetLastError(), "paged_append_kernel launch");
+    }
+};
+
 // ------------------------------------------------------------ logits
 size_t dtype_bytes(int t) { return t == P100_F32 ? 4 : 2; }
 const char* logprobs_reason(int rows, int n, int dtype, int top_k) {
@@ -133,8 +144,7 @@ p100_status p100_paged_append(const p100_paged_desc* desc, const void* qkv, int 
     prm.rope = reinterpret_cast<const float2*>(rope_cs);
     prm.max_pos = max_pos;
     prm.half = rope_half != 0;
-    return launch_append_from<paged::ByTable>(prm, paged::NoParams{}, qkv_type, desc->dtype, desc->head_dim, blocks,
-                                              stream);
+    return append_typed(qkv_type, desc->dtype, desc->head_dim, AppendLaunch{prm, blocks, stream});
 }
 
 size_t p100_fa_paged_workspace_size(const p100_paged_desc* desc) {
