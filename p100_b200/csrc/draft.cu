@@ -62,7 +62,7 @@ struct AppendRopeLaunch {
     cudaStream_t stream;
     template <typename S, typename T, int D>
     p100_status operator()() const {
-        paged::append_rope_kernel<S, T, D><<<blocks, paged::kAppendThreads, 0, stream>>>(prm, turns);
+        paged::append_rope_kernel<S, T, D><<<blocks, paged::kRopeThreads, 0, stream>>>(prm, turns);
         return cuda_status(cudaGetLastError(), "append_rope_kernel launch");
     }
 };
@@ -256,7 +256,7 @@ p100_status p100_paged_append_rope(const p100_paged_desc* desc, const void* qkv,
     paged::AppendParams prm = {};
     unsigned blocks = 0;
     if (p100_status st = append_params(desc, qkv, qkv_type, qkv_stride, q_norm, k_norm, eps, rope_reason(rope, desc),
-                                       block_table, q_start, kv_len, q, k_pages, v_pages, prm, blocks))
+                                       block_table, q_start, kv_len, q, k_pages, v_pages, paged::kRopeThreads, prm, blocks))
         return st;
     if (!blocks) return P100_OK;
     return append_typed(qkv_type, desc->dtype, desc->head_dim,

@@ -132,7 +132,7 @@ p100_status page_map(CUtensorMap* map, const void* base, const p100_paged_desc& 
 // stays 0 where there is nothing to do.
 p100_status append_params(const p100_paged_desc* desc, const void* qkv, int qkv_type, long long qkv_stride,
                           const float* q_norm, const float* k_norm, float eps, const char* why, const int* block_table,
-                          const int* q_start, const int* kv_len, void* q, void* k_pages, void* v_pages,
+                          const int* q_start, const int* kv_len, void* q, void* k_pages, void* v_pages, int threads,
                           paged::AppendParams& prm, unsigned& blocks) {
     blocks = 0;
     if (!desc) return set_error(P100_ERR_INVALID, "null descriptor");
@@ -173,7 +173,7 @@ p100_status append_params(const p100_paged_desc* desc, const void* qkv, int qkv_
     const long long steps = paged::Steps(desc->n_head_q, desc->n_head_kv, at_once).all();
     const long long fill = std::min((steps + together - 1) / together, (long long)sms * paged::kAppendWarps / desc->n_tokens);
     prm.warps = int(std::max({1LL, fill, (steps + paged::kAppendMost - 1) / paged::kAppendMost}));
-    const long long all = ((long long)desc->n_tokens * prm.warps + paged::kAppendThreads / 32 - 1) / (paged::kAppendThreads / 32);
+    const long long all = ((long long)desc->n_tokens * prm.warps + threads / 32 - 1) / (threads / 32);
     if (all > INT_MAX) return set_error(P100_ERR_INVALID, "too many heads and tokens for one call");
     blocks = unsigned(all);
     return P100_OK;

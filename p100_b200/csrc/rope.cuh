@@ -16,13 +16,16 @@
 // the first heads' loads are on their way.  All in FP32, two values an operation;
 // the one rounding is the store to 16 bits.
 //
-// Bytes bound it, then issue: partners that lie in another lane come as the 16-bit
-// values they were loaded as, values that do not turn and the v heads of the
-// cache's own type go through.  The cosines wait in shared memory for the
-// k heads: with 16 registers less, three CTAs share an SM instead of two.
-// Measured: 2,622 tokens of 64 / 8 heads of 128 from bf16 with norms, halves,
-// 30 us (36 with the branches on pairing and norm inside the loop of heads); 8,192 of
-// 64 / 8 heads from fp32 with norms 92 us, 0.84 of measured bandwidth.
+// Bytes bound it, then the latency of a warp's chain: partners that lie in another
+// lane come as the 16-bit values they were loaded as, values that do not turn and
+// the v heads of the cache's own type go through, and the loops are written out by
+// pairing and norm (with the branches inside 36 us below).  The cosines wait in
+// shared memory for the k heads.  Blocks of four warps, five an SM: with eight the
+// last ones leave SMs idle (30 us), with six of four the registers spill (27.5), with
+// four too few warps are there (35).
+// Measured: 2,622 tokens of 64 / 8 heads of 128 from bf16 with norms and halves
+// 24.4 us, 0.71 of measured bandwidth; 8,192 of them from fp32 with norms 92 us,
+// 0.83.
 #pragma once
 #include <type_traits>
 
@@ -30,6 +33,8 @@
 
 namespace p100b {
 namespace paged {
+
+constexpr int kRopeThreads = 128;
 
 struct TurnParams {
     p100_rope rope;
@@ -62,20 +67,20 @@ __device__ __forceinline__ void pairs(const uint4& x, uint64_t (&y)[N]) {
 }
 
 template <typename S, typename T, int D>
-__global__ void __launch_bounds__(kAppendThreads, 3)
+__global__ void __launch_bounds__(kRopeThreads, 5)
     append_rope_kernel(const AppendParams p, const __grid_constant__ TurnParams r) {
     constexpr int E = append_values<S>();
     constexpr int kLanes = D / E;              // of a head
     constexpr int kHeads = 32 / kLanes;        // of a step
     constexpr int U = append_steps<S>();
-    __shared__ float s_cs[E][kAppendThreads], s_sn[E][kAppendThreads];
-    __shared__ float s_heads[kAppendThreads * E];
+    __shared__ float s_cs[E][kRopeThreads], s_sn[E][kRopeThreads];
+    __shared__ float s_heads[kRopeThreads * E];
     __shared__ unsigned long long s_turns[64];   // a lane's own index into the parameters is one access for each lane
     if (threadIdx.x < 64) s_turns[threadIdx.x] = r.rope.turns[threadIdx.x];
     __syncthreads();
     const int lane = threadIdx.x & 31, in_head = lane % kLanes, v0 = in_head * E;
     const Steps steps(p.d.n_head_q, p.d.n_head_kv, kHeads);
-    const long long item = (long long)blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
+    const long long item = (long long)blockIdx.x * (kRopeThreads / 32) + (threadIdx.x >> 5);
     const int t = int(item / p.warps);
     if (t >= p.d.n_tokens) return;
     const int share = int(item - (long long)t * p.warps);

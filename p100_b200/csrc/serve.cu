@@ -137,7 +137,7 @@ p100_status p100_paged_append(const p100_paged_desc* desc, const void* qkv, int 
     unsigned blocks = 0;
     if (p100_status st = append_params(desc, qkv, qkv_type, qkv_stride, q_norm, k_norm, eps,
                                        rope_cs && max_pos <= 0 ? "max_pos must be positive" : nullptr, block_table,
-                                       q_start, kv_len, q, k_pages, v_pages, prm, blocks))
+                                       q_start, kv_len, q, k_pages, v_pages, paged::kAppendThreads, prm, blocks))
         return st;
     if (!blocks) return P100_OK;
     if (!aligned(rope_cs, 8)) return set_error(P100_ERR_INVALID, "rope_cs must be 8-byte aligned");
