@@ -180,6 +180,54 @@ inline void attention_paged(const PagedDesc& d, const void* q, const void* k_pag
     check(p100_fa_paged(&d, q, k_pages, v_pages, block_table, q_start, kv_len, o, lse, ws.data(), ws.size(), stream));
 }
 
+// Rotary frequencies (p100_rope_init).
+inline p100_rope rope(int rope_dim, double theta, bool half = false, const p100_rope_scaling* scaling = nullptr) {
+    p100_rope r;
+    check(p100_rope_init(&r, rope_dim, half ? 1 : 0, theta, scaling));
+    return r;
+}
+
+// A step over the paged cache: pages, starts, slots and positions of the new
+// tokens (p100_paged_plan); slot and position may be null.
+inline void paged_plan(const PagedDesc& d, const int* length, const int* n_new, int* pool, int* held, int* block_table,
+                       int* q_start, int* kv_len, long long* slot, int* position, cudaStream_t stream) {
+    check(p100_paged_plan(&d, length, n_new, pool, held, block_table, q_start, kv_len, slot, position, stream));
+}
+inline void paged_pool_init(const PagedDesc& d, int* pool, int* held, int* block_table, cudaStream_t stream) {
+    check(p100_paged_pool_init(&d, pool, held, block_table, stream));
+}
+
+// Masks and positions of drafted trees from the tokens' parents (p100_tree_mask).
+inline void tree_mask(const int* parent, const int* q_start, const int* kv_len, int n_seq, int n_tokens, int mask_words,
+                      unsigned* mask, int* position, cudaStream_t stream) {
+    check(p100_tree_mask(parent, q_start, kv_len, n_seq, n_tokens, mask_words, mask, position, stream));
+}
+
+// paged_append with computed rotations at given positions, or null for the
+// tokens' own (p100_paged_append_rope).
+inline void paged_append_rope(const PagedDesc& d, const void* qkv, p100_dtype qkv_type, long long qkv_stride,
+                              const float* q_norm, const float* k_norm, float eps, const p100_rope& rope,
+                              const int* position, const int* block_table, const int* q_start, const int* kv_len, void* q,
+                              void* k_pages, void* v_pages, cudaStream_t stream) {
+    check(p100_paged_append_rope(&d, qkv, qkv_type, qkv_stride, q_norm, k_norm, eps, &rope, position, block_table, q_start,
+                                 kv_len, q, k_pages, v_pages, stream));
+}
+
+// Attention of drafted trees over the pages (p100_fa_tree).
+inline void attention_tree(const PagedDesc& d, const void* q, const void* k_pages, const void* v_pages,
+                           const unsigned* mask, int mask_words, const int* block_table, const int* q_start,
+                           const int* kv_len, void* o, float* lse, const FaPagedWorkspace& ws, cudaStream_t stream) {
+    check(p100_fa_tree(&d, q, k_pages, v_pages, mask, mask_words, block_table, q_start, kv_len, o, lse, ws.data(),
+                       ws.size(), stream));
+}
+
+// The rows of kept new tokens to their final places (p100_paged_keep); length may
+// be null.
+inline void paged_keep(const PagedDesc& d, void* k_pages, void* v_pages, const int* keep, const int* keep_len,
+                       const int* block_table, const int* q_start, const int* kv_len, int* length, cudaStream_t stream) {
+    check(p100_paged_keep(&d, k_pages, v_pages, keep, keep_len, block_table, q_start, kv_len, length, stream));
+}
+
 // One rank of a row-split tensor-parallel group.
 class TensorParallel {
 public:
