@@ -48,7 +48,7 @@ using paged::pair;
 using paged::unpair;
 
 constexpr int kRows = 128, kKeys = 128;
-constexpr int kOver = 2;                  // what a row tile costs beyond its keys, in units
+constexpr int kOver = 4;                  // what a row tile costs beyond its keys, in units (48 trees of 8: 145 us, with 2 152)
 constexpr int kMinUnits = 2;              // of a share: a tile for each warpgroup
 constexpr int kWholeFrom = 4;             // row tiles per CTA from which they are dealt out whole
 constexpr int kThreads = fatc::kThreads;
@@ -118,7 +118,7 @@ __device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tm
     unsigned used = 0;                               // slots filled so far
     bool ok = true;
     struct Box {
-        int page, off;   // page -1: nothing to read
+        int page, off;   // off -1: nothing to read
     };
     for (unsigned j = 0; ok; ++j) {
         Item it;
@@ -147,24 +147,23 @@ __device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tm
         if (!more) break;
         if (p.box == 0) continue;   // the gathering warps load
         const int* table = d.block_table + (long long)it.seq * d.max_pages;
+        // Where a box lies; its table entry is looked at two tiles later, so that the loop does not wait for it.
         auto find = [&](int t) {
-            Box b = {-1, 0};
+            Box b = {0, -1};
             if (!mine || t >= it.count) return b;
             const int key = (it.key_tile + t) * kKeys + i * p.box;
             if (key < end) {
                 const int n = key / d.page_size;
                 b.off = key - n * d.page_size;
                 b.page = table[n];
-                if (b.page < 0 || b.page >= d.n_pages) {
-                    paged::flag_input();
-                    b.page = -1;
-                }
             }
             return b;
         };
         auto load = [&](const CUtensorMap* map, const Box& b) {
             const int slot = used % NS;
-            const uint32_t bytes = uint32_t(__popc(__ballot_sync(0xffffffffu, b.page >= 0))) * p.box * 128;
+            const bool known = b.page >= 0 && b.page < d.n_pages, there = b.off >= 0 && known;
+            if (b.off >= 0 && !known) paged::flag_input();
+            const uint32_t bytes = uint32_t(__popc(__ballot_sync(0xffffffffu, there))) * p.box * 128;
             if (used >= NS) ok = warp_wait(&bars.empty[slot], (used / NS - 1) & 1, &bars.abort);
             if (!ok) return;
             if (lane == 0) {
@@ -172,7 +171,7 @@ __device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tm
                 else mbar_arrive(&bars.full[slot]);
             }
             __syncwarp();
-            if (b.page >= 0)
+            if (there)
                 asm volatile(
                     "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
                     " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_addr(ring) + uint32_t(slot) * tile_bytes<D>() + at),
@@ -205,8 +204,8 @@ __device__ __forceinline__ void gather_role(const Params& p, Barriers& bars, uin
     const int chunk = lane % kChunks, sub = lane / kChunks;
     unsigned used = 0;
     bool ok = true;
-    struct Rows {
-        long long at[2];   // where the rows of keys `lane` and `lane + 32` begin, -1: not read
+    struct Rows {   // of keys `lane` and `lane + 32`
+        int page[2], off[2];   // off -1: not read
     };
     auto announce = [&](unsigned u) {
         fatc::fence_async();
@@ -221,16 +220,17 @@ __device__ __forceinline__ void gather_role(const Params& p, Barriers& bars, uin
         const long long head = job.head * d.head_stride + chunk * 8;
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.job_empty[j % kJobs]);
+        // (the table entries are looked at two tiles later, as in load_role)
         auto find = [&](int t) {
-            Rows r = {{-1, -1}};
+            Rows r = {{0, 0}, {-1, -1}};
             if (t >= count) return r;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int key = key0 + t * kKeys + h * 32;
                 if (key < end && key >= 0) {
-                    const int n = key / d.page_size, page = table[n];
-                    if (page < 0 || page >= d.n_pages) paged::flag_input();
-                    else r.at[h] = page * d.page_stride + (long long)(key - n * d.page_size) * d.token_stride;
+                    const int n = key / d.page_size;
+                    r.off[h] = key - n * d.page_size;
+                    r.page[h] = table[n];
                 }
             }
             return r;
@@ -241,13 +241,27 @@ __device__ __forceinline__ void gather_role(const Params& p, Barriers& bars, uin
                 ok = false;
                 return;
             }
+            long long at[2];   // where the rows begin, -1: not read
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const bool known = r.page[h] >= 0 && r.page[h] < d.n_pages;
+                if (r.off[h] >= 0 && !known) paged::flag_input();
+                at[h] = r.off[h] >= 0 && known ? r.page[h] * d.page_stride + r.off[h] * d.token_stride : -1;
+            }
             const T* from = static_cast<const T*>(pages) + head;
             const uint32_t slot = ring + (used % NS) * tile_bytes<D>() + (chunk >> 3) * kSub;
-#pragma unroll 8
-            for (int i = 0; i < 64; i += kStep) {
-                const long long o = __shfl_sync(0xffffffffu, i < 32 ? r.at[0] : r.at[1], (i & 31) + sub);
-                const int row = first + i + sub;
-                fap::cp_async16(slot + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), from + (o < 0 ? 0 : o), o >= 0);
+            // eight rows' places first, then their copies: one behind the other, each copy waited for its place's shuffle
+#pragma unroll 1
+            for (int i = 0; i < 64; i += 8 * kStep) {
+                long long o[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    o[u] = __shfl_sync(0xffffffffu, i + u * kStep < 32 ? at[0] : at[1], (i + u * kStep & 31) + sub);
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int row = first + i + u * kStep + sub;
+                    fap::cp_async16(slot + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), from + (o[u] < 0 ? 0 : o[u]), o[u] >= 0);
+                }
             }
             fap::cp_commit();
             if (used > item0) {   // (three slots' copies in flight were no faster)
