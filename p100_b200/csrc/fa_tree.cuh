@@ -193,8 +193,12 @@ __device__ __forceinline__ void load_role(const Params& p, const CUtensorMap* tm
         for (unsigned u = used > NS ? used - NS : 0; u < used; ++u) mbar_wait(&bars.full[u % NS], (u / NS) & 1);
 }
 
-// The tiles of pages of any size, as fa_paged_tc.cuh's gather_role but in this
-// kernel's order.
+// The tiles of pages of any size: each of two warps gathers 64 keys' rows, in the
+// order of load_role.  A slot's barrier takes the copies' own arrivals, and the
+// issuing warp puts the fence between them and its products (a gathering warp's
+// fence waits for the next slot's copies, too: 16 trees of 5 over 8192, pages of
+// 24, 91 us, with it 94).  What bounds it are the copies of 16 bytes: boxes take 63.
+// A third gathering warp, the one that hands out the items, made it 119.
 template <typename T, int D>
 __device__ __forceinline__ void gather_role(const Params& p, Barriers& bars, uint32_t ring) {
     constexpr int NS = slots<D>();
@@ -207,15 +211,11 @@ __device__ __forceinline__ void gather_role(const Params& p, Barriers& bars, uin
     struct Rows {   // of keys `lane` and `lane + 32`
         int page[2], off[2];   // off -1: not read
     };
-    auto announce = [&](unsigned u) {
-        fatc::fence_async();
-        mbar_arrive(&bars.full[u % NS]);
-    };
     for (unsigned j = 0;; ++j) {
-        if (!warp_wait(&bars.job_full[j % kJobs], (j / kJobs) & 1, &bars.abort)) return;
+        if (!warp_wait(&bars.job_full[j % kJobs], (j / kJobs) & 1, &bars.abort)) break;
         const Job& job = bars.jobs[j % kJobs];
         const int count = job.count, end = job.end, key0 = job.key_tile * kKeys + first + lane;
-        if (count == 0) return;
+        if (count == 0) break;
         const int* table = d.block_table + (long long)job.seq * d.max_pages;
         const long long head = job.head * d.head_stride + chunk * 8;
         __syncwarp();
@@ -235,7 +235,6 @@ __device__ __forceinline__ void gather_role(const Params& p, Barriers& bars, uin
             }
             return r;
         };
-        const unsigned item0 = used;
         auto load = [&](const void* pages, const Rows& r) {
             if (used >= NS && !warp_wait(&bars.empty[used % NS], (used / NS - 1) & 1, &bars.abort)) {
                 ok = false;
@@ -250,7 +249,7 @@ __device__ __forceinline__ void gather_role(const Params& p, Barriers& bars, uin
             }
             const T* from = static_cast<const T*>(pages) + head;
             const uint32_t slot = ring + (used % NS) * tile_bytes<D>() + (chunk >> 3) * kSub;
-            // eight rows' places first, then their copies: one behind the other, each copy waited for its place's shuffle
+            // eight rows' places first, then their copies
 #pragma unroll 1
             for (int i = 0; i < 64; i += 8 * kStep) {
                 long long o[8];
@@ -263,11 +262,7 @@ __device__ __forceinline__ void gather_role(const Params& p, Barriers& bars, uin
                     fap::cp_async16(slot + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), from + (o[u] < 0 ? 0 : o[u]), o[u] >= 0);
                 }
             }
-            fap::cp_commit();
-            if (used > item0) {   // (three slots' copies in flight were no faster)
-                fap::cp_wait<1>();
-                announce(used - 1);
-            }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_addr(&bars.full[used % NS])) : "memory");
             ++used;
         };
         Rows now = find(0), next = find(1);
@@ -279,19 +274,15 @@ __device__ __forceinline__ void gather_role(const Params& p, Barriers& bars, uin
             now = next;
             next = later;
         }
-        if (!ok) {
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            return;
-        }
-        fap::cp_wait<0>();
-        announce(used - 1);
+        if (!ok) break;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // Issues the products; false when a wait was given up.
 template <typename T, int D>
-__device__ __forceinline__ bool mma_role(const Desc& d, float scale, Barriers& bars, uint32_t q_smem, uint32_t ring,
-                                         uint32_t tmem) {
+__device__ __forceinline__ bool mma_role(const Desc& d, float scale, bool gathered, Barriers& bars, uint32_t q_smem,
+                                         uint32_t ring, uint32_t tmem) {
     constexpr int NS = slots<D>();
     // a negative scale turns the scores' sign here, so that the softmax has a positive one
     const uint32_t idesc_s = fatc::idesc_f16<T>(kKeys, false) | (scale < 0.f ? fatc::kNegateA : 0u);
@@ -299,7 +290,11 @@ __device__ __forceinline__ bool mma_role(const Desc& d, float scale, Barriers& b
     const int lane = threadIdx.x & 31;
     unsigned used = 0, items = 0, tiles[2] = {0, 0};
     auto slot_of = [&](unsigned at) { return (used + at) % NS; };
-    auto landed = [&](unsigned at) { return warp_wait(&bars.full[slot_of(at)], ((used + at) / NS) & 1, &bars.abort); };
+    auto landed = [&](unsigned at) {
+        const bool ok = warp_wait(&bars.full[slot_of(at)], ((used + at) / NS) & 1, &bars.abort);
+        if (gathered) fatc::fence_async();
+        return ok;
+    };
     auto qk = [&](int w, unsigned slot) {   // S_w = Q K^T
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
@@ -702,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp == kLoadWarp) {
             load_role<D>(p, &tmk, &tmv, len, bars, ring, share);
         } else if (warp == kMmaWarp) {
-            if (!mma_role<T, D>(p.d, p.scale, bars, fatc::uniform(smem_addr(q_smem)), fatc::uniform(smem_addr(ring)),
+            if (!mma_role<T, D>(p.d, p.scale, p.box == 0, bars, fatc::uniform(smem_addr(q_smem)), fatc::uniform(smem_addr(ring)),
                                 fatc::uniform(tmem))) {
                 // leave only when the products in flight are done
                 fatc::mma_commit(&bars.drain);
