@@ -495,11 +495,12 @@ def _pages_of(k_pages, v_pages, dev, desc):
     head = desc.head_stride or size * d
     page = desc.page_stride or heads * size * d
     need = (n - 1) * page + (heads - 1) * head + (size - 1) * token + d if n > 0 else 0
+    by_head, by_token = ((n, heads, size, d), (page, head, token, 1)), ((n, size, heads, d), (page, token, head, 1))
     for t, what in ((k_pages, "k_pages"), (v_pages, "v_pages")):
         _need(t, what, dev, dtype, dense=False)
         # a tensor whose sizes name its axes must have the descriptor's strides in their order
         shape, strides = t.shape, t.stride()
-        if shape == (n, heads, size, d) and strides == (page, head, token, 1):
+        if (shape, strides) == by_head or (shape, strides) == by_token:
             continue
         orders = [steps for order, steps in (((heads, size, d), (page, head, token, 1)),
                                              ((size, heads, d), (page, token, head, 1)),
