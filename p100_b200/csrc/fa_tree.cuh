@@ -25,8 +25,9 @@
 // The probabilities are rounded once to the cache's 16-bit type, as fa_paged_tc.cuh
 // does and for its reason: a second part (what the rounding left) would be half as
 // many products again, and both the products and the energy they take count here
-// (48 trees of 8 over 8192 tokens: 147 us, with two parts 180, at the 1000 W cap
-// that streaming the cache alone comes near).
+// (48 trees of 8 over 8192 tokens, 64 / 8 heads: 144 us, 0.86 of measured bandwidth,
+// at the 1000 W cap that streaming the cache alone comes near; two parts took a
+// fifth more).
 #pragma once
 #include "fa_paged_tc.cuh"
 
@@ -566,7 +567,6 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
                         pk[e >> 1] = paged::pack2<T>(a, b);
                     }
                     fatc::st8(t_s + i * 8, pk);
-                    
                 }
                 fatc::wait_st();
                 if (half == 0 && !clear_v(t, key0)) return;
