@@ -435,11 +435,16 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
         const Job& job = bars.jobs[j % kJobs];
         const int count = job.count;
         if (count == 0) return;
-        if (!loaded) load_queries<T, D>(p, job, q_smem);
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        fatc::fence_async();
-        fatc::fence_before();
-        mbar_arrive(&bars.q_full);
+        auto queries_ready = [&]() {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fatc::fence_async();
+            fatc::fence_before();
+            mbar_arrive(&bars.q_full);
+        };
+        if (!loaded) {
+            load_queries<T, D>(p, job, q_smem);
+            queries_ready();
+        }
         const Row r(d, job, row);
         // (a row that is none takes the first one's mask: its results go nowhere)
         const int ctx = job.kv - job.n, limit = job.kv;
@@ -612,6 +617,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
         }
         fatc::fence_before();
         mbar_arrive(&bars.o_free);
+        if (loaded) queries_ready();   // the next item's scores are computed while this one's results are written
         const long long o_at = r.at(d, job, d.o_stride, D) + w * kCols;
         if (job.whole) {
             if (r.live) {
