@@ -287,3 +287,78 @@ def test_other_streams(cuda):
     after = [b.rows(b.k, s, t - n) for s, (n, t) in enumerate(zip(b.q_lens, b.kv_lens))]
     assert torch.equal(after[0][:3], before[0][[1, 4, 5]]) and torch.equal(after[0][3:], before[0][3:])
     assert torch.equal(after[1][0], before[1][2]) and torch.equal(after[1][1:], before[1][1:])
+
+
+@pytest.mark.parametrize("softcap,scale", [(1e-22, 1e-22), (3e-30, -1e-30), (1e-16, 2e-16), (1e-14, 1e-14)])
+@pytest.mark.parametrize("q_lens,kv_lens", [([2, 1], [300, 70]), ([60, 3], [300, 70])])
+def test_tiny_caps_with_tiny_scales(cuda, q_lens, kv_lens, softcap, scale):
+    """Every score is next to zero, so a row's visible keys weigh the same; hidden ones must not weigh anything."""
+    b = Batch(cuda, q_lens, kv_lens, 6, 2, 64, "bf16", 16, seed=60)
+    b.fill()
+    mask, bits = masks(b, np.random.RandomState(0), "any", 2)
+    for size in (1.5, 0.01):
+        q = b.queries(size)
+        o, lse = attend_tree(b, q, mask, softcap=softcap, scale=scale, o_fp32=True)
+        check(cuda, b, o, lse, tree64(b, q, bits, scale, softcap))
+
+
+@pytest.mark.parametrize("softcap", [1e-6, 1e-3, 0.5, 5.0, 100.0, 2000.0, 1e6])
+@pytest.mark.parametrize("q_lens,kv_lens", [([2, 1, 1], [700, 5, 1]), ([60, 1, 40], [900, 3, 40])])
+def test_caps_of_any_size(cuda, q_lens, kv_lens, softcap):
+    """As test_paged_gpu's: caps below, among and far above the scores; the largest may differ from none by 1e-8."""
+    b = Batch(cuda, q_lens, kv_lens, 6, 2, 64, "bf16", 16)
+    b.fill()
+    mask, bits = masks(b, np.random.RandomState(0), "any", 2)
+    q = b.queries(2.0)
+    for scale in (0.0, -0.2):
+        o, lse = attend_tree(b, q, mask, softcap=softcap, scale=scale, o_fp32=True)
+        check(cuda, b, o, lse, tree64(b, q, bits, scale, softcap if softcap < 1e6 else 0.0))
+
+
+@pytest.mark.parametrize("rows", [3, 60])
+def test_large_scores_and_rising_maxima(cuda, rows):
+    """Scores whose maximum rises from tile to tile by far more than a rounding, and rows that one key decides."""
+    for dtype in ("f16", "bf16"):
+        b = Batch(cuda, [rows], [1000 + rows], 4, 1, 128, dtype, 16, seed=5)
+        b.fill()
+        page, off = b.slots(0)
+        grow = cuda.linspace(0.2, 6.0, 1000 + rows, device="cuda")[:, None, None]
+        k = b.k[page, :, off].float() * grow
+        b.k[page, :, off] = k.to(b.t)
+        q = b.queries(2.0)
+        mask, bits = masks(b, np.random.RandomState(0), "any", 2)
+        check(cuda, b, *attend_tree(b, q, mask), tree64(b, q, bits))
+
+
+@pytest.mark.parametrize("page,pages", [(8176, 262657), (114808, 18705)])   # 2^31 - 16 and 2^31 - 8 places
+@pytest.mark.parametrize("n", [1, 9])
+def test_as_many_keys_as_a_length_holds(cuda, n, page, pages):
+    """A sequence of almost 2^31 tokens whose table names one page over and over, as test_paged_limits_gpu's: its keys are
+    zero and weigh the same (V = 1); the newest token's own key (V = 3) decides its row, and no other row's bit names
+    it; what the page holds behind the last token would decide every row if it took part.
+
+    Bound: every term before the join is a whole number below 2^24 (of a power of two); the join adds at most 296 parts
+    with relative errors of 2^-24 each in o and in the sum, and the one division rounds: below 2^-14."""
+    torch = cuda
+    dim, group, kv = 64, 4, page * pages - 3
+    last = (kv - 1) % page
+    t = torch.float16
+    k = torch.zeros((2, 1, page, dim), dtype=t, device="cuda")
+    v = torch.ones((2, 1, page, dim), dtype=t, device="cuda")
+    k[1, 0, last], v[1, 0, last] = 5.0, 3.0
+    k[1, 0, last + 1:], v[1, 0, last + 1:] = 10.0, 100.0
+    table = torch.zeros((1, pages), dtype=torch.int32, device="cuda")
+    table[0, -1] = 1
+    q = torch.ones((n, group, dim), dtype=t, device="cuda")
+    d = P.PagedDesc(n_seq=1, n_tokens=n, n_head_q=group, n_head_kv=1, page_size=page, n_pages=2, max_pages=pages,
+                    head_dim=dim, o_fp32=True)
+    mask = torch.from_numpy(mask_of([np.arange(-1, n - 1)], 1)[0]).cuda()
+    o, lse = P.fa_tree(d, q, k, v, mask, table, torch.tensor([0, n], dtype=torch.int32, device="cuda"),
+                       torch.tensor([kv], dtype=torch.int32, device="cuda"))
+    P.check(P.device_error())
+    x = 5.0 * dim / math.sqrt(dim)   # the newest key's score; the others' weight is below 2^31 e^-40 < 2^-26 of its own
+    seen = math.log(kv - n + 1)
+    assert bool(((o[:-1] - 1.0).abs() <= 2.0 ** -14).all())
+    assert bool(((o[-1] - 3.0).abs() <= 3 * 2.0 ** -14).all())
+    assert bool(((lse[:-1] - seen).abs() <= 2.0 ** -14 + 2.0 ** -22 * seen).all())
+    assert bool(((lse[-1] - x).abs() <= 2.0 ** -14 + 2.0 ** -22 * x).all())
