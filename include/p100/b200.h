@@ -438,7 +438,8 @@ p100_status p100_logprobs(const void* logits, int dtype, int n, int rows, long l
  * p100_device_error() for negative lengths, more than max_pages pages a request,
  * more than n_tokens new tokens, or counts that do not fit the pool.
  * Of desc it uses n_seq, n_tokens, page_size, n_pages and max_pages.  Calls on
- * one pool are ordered by the caller; no two arrays may overlap. */
+ * one pool are ordered by the caller; no two arrays may overlap, but kv_len may
+ * be length itself (each call then goes on where the last one ended). */
 p100_status p100_paged_plan(const p100_paged_desc* desc, const int* length, const int* n_new, int* pool, int* held,
                             int* block_table, int* q_start, int* kv_len, long long* slot, int* position,
                             p100_stream_t stream);
@@ -519,7 +520,8 @@ p100_status p100_fa_tree(const p100_paged_desc* desc, const void* q, const void*
  * keep[q_start[s] + i] of sequence s become those of new token i (keep rises:
  * the path of an accepted draft), in the pages' place; rows behind them stay as
  * they are.  length[s] = kv_len - n + keep_len[s], the next plan's length
- * (may be NULL).  A keep_len outside [0, n] leaves its sequence out, an index
+ * (may be NULL; it must not overlap the other arrays, nor k_pages be v_pages:
+ * refused).  A keep_len outside [0, n] leaves its sequence out, an index
  * out of order or range its row; both, and pages out of range, raise
  * P100_ERR_INVALID in p100_device_error().  Sequences may not share the pages
  * that hold new tokens. */

@@ -652,7 +652,7 @@ def paged_pool(desc, stream=None):
 def paged_plan(desc, length, n_new, pool, held, block_table, out=None, stream=None):
     """The plan of a step (p100_paged_plan): pages for n_new tokens behind length of each request (int32 [n_seq]),
     pool, held and block_table updated in place.  Returns PagedPlan; out: one of an earlier call to write into, of
-    which slot and position may be None."""
+    which slot and position may be None; its kv_len may be length."""
     torch = _torch()
     dev = torch.cuda.current_device()
     i = torch.int32
@@ -740,7 +740,7 @@ def fa_tree(desc, q, k_pages, v_pages, mask, block_table, q_start, kv_len, o=Non
 
 def paged_keep(desc, k_pages, v_pages, keep, keep_len, block_table, q_start, kv_len, length=None, stream=None):
     """Moves the rows of kept new tokens in the pages (p100_paged_keep): keep int32 [n_tokens], keep_len int32 [n_seq].
-    Returns length, the tokens of each sequence that stay."""
+    Returns length, the tokens of each sequence that stay (a tensor of its own, not kv_len)."""
     torch = _torch()
     dev = torch.cuda.current_device()
     _lengths_of(dev, desc, block_table, q_start, kv_len)

@@ -67,6 +67,12 @@ struct AppendRopeLaunch {
     }
 };
 
+// Whether n ints at a and m at b share one.
+bool overlap(const int* a, size_t n, const int* b, size_t m) {
+    const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + m * sizeof(int) && y < x + n * sizeof(int);
+}
+
 // ------------------------------------------------------------ trees
 const char* words_reason(int mask_words) {
     return mask_words < 1 || mask_words > P100_TREE_MAX_WORDS ? "mask_words must be between 1 and 32" : nullptr;
@@ -352,6 +358,13 @@ p100_status p100_paged_keep(const p100_paged_desc* desc, void* k_pages, void* v_
         return set_error(P100_ERR_INVALID, "null buffer");
     if (!aligned(k_pages, 16) || !aligned(v_pages, 16))
         return set_error(P100_ERR_INVALID, "the pages must be 16-byte aligned");
+    if (k_pages == v_pages) return set_error(P100_ERR_INVALID, "v_pages must not be k_pages");
+    // a sequence's blocks read them while one of them writes its length
+    const size_t seqs = desc->n_seq;
+    if (length && (overlap(length, seqs, kv_len, seqs) || overlap(length, seqs, keep_len, seqs) ||
+                   overlap(length, seqs, q_start, seqs + 1) || overlap(length, seqs, keep, desc->n_tokens) ||
+                   overlap(length, seqs, block_table, seqs * desc->max_pages)))
+        return set_error(P100_ERR_INVALID, "length must not overlap the other arrays");
     p.d.block_table = block_table;
     p.d.q_start = q_start;
     p.d.kv_len = kv_len;

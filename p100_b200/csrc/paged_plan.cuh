@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
         s_give[tid] = int(v[1]);
         s_take[tid] = int(v[2]);
     }
-    cluster_meet();   // every CTA has read the pool's count, the lengths and `held`
+    cluster_meet();   // every CTA has read the pool's count, the lengths (kv_len may be their place) and `held`
     if (missing != 0) {   // refused: no pages move and no request has new tokens
         if (rank == 0) {
             if (tid < p.n_seq) p.kv_len[tid] = len;

@@ -201,3 +201,21 @@ def test_null_buffers(cuda, lib):
         z = [None if i == out else Z for i in range(7)]
         assert lib.p100_tree_mask(*z[:3], 1, 1, 1, z[6], None, None) == P.ERR_INVALID
         assert P.last_error() == "null buffer"
+
+
+@pytest.mark.gpu
+def test_keep_refuses_shared_arrays(cuda, lib):
+    """length may touch none of the arrays that the sequences' blocks read, at either end; refused before any launch."""
+    d = desc(head_dim=64)
+    at = {name: 4096 * (i + 1) for i, name in enumerate(("k", "v", "keep", "keep_len", "table", "q_start", "kv_len"))}
+    ints = {"keep": d.n_tokens, "keep_len": d.n_seq, "table": d.n_seq * d.max_pages, "q_start": d.n_seq + 1, "kv_len": d.n_seq}
+
+    def call(length, **other):
+        return lib.p100_paged_keep(C.byref(d), *[C.c_void_p(x) for x in {**at, **other}.values()], C.c_void_p(length), None)
+
+    for name, n in ints.items():
+        for length in (at[name], at[name] + 4 * (n - 1), at[name] - 4 * (d.n_seq - 1)):
+            assert call(length) == P.ERR_INVALID, name
+            assert P.last_error() == "length must not overlap the other arrays"
+    assert call(1 << 20, v=at["k"]) == P.ERR_INVALID
+    assert P.last_error() == "v_pages must not be k_pages"

@@ -362,3 +362,31 @@ def test_as_many_keys_as_a_length_holds(cuda, n, page, pages):
     assert bool(((o[-1] - 3.0).abs() <= 3 * 2.0 ** -14).all())
     assert bool(((lse[:-1] - seen).abs() <= 2.0 ** -14 + 2.0 ** -22 * seen).all())
     assert bool(((lse[-1] - x).abs() <= 2.0 ** -14 + 2.0 ** -22 * x).all())
+
+
+@pytest.mark.parametrize("n_seq,n_tokens", [(3, 16), (300, 900), (1000, 9000)])
+def test_plan_goes_on_from_its_own_lengths(cuda, n_seq, n_tokens):
+    """kv_len in length's place, as a captured step of single tokens has it: a CTA, a large CTA, a cluster."""
+    torch = cuda
+    d = P.PagedDesc(n_seq=n_seq, n_tokens=n_tokens, n_head_q=1, n_head_kv=1, page_size=4, n_pages=n_seq * 6, max_pages=6)
+    pool, held, table = P.paged_pool(d)
+    length = torch.arange(n_seq, dtype=torch.int32, device="cuda") % 5
+    n_new = (torch.arange(n_seq, dtype=torch.int32, device="cuda") % 7 != 0).int() * 2
+    apart = P.paged_plan(d, length, n_new, pool, held, table)
+    out = P.PagedPlan(*(torch.empty_like(x) for x in apart))
+    start, want = length.clone(), length.clone()
+    here = out._replace(kv_len=start)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        P.paged_plan(d, start, n_new, pool, held, table, out=here)
+    for _ in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        P.check(P.device_error())
+        first = (n_new.cumsum(0) - n_new).tolist()
+        place = here.position.tolist()
+        for s in range(0, n_seq, 37):
+            n, at = int(n_new[s]), first[s]
+            assert place[at:at + n] == [int(want[s]) + i for i in range(n)]
+        want += n_new
+        assert torch.equal(start, want) and held.tolist() == [-(-x // 4) for x in want.tolist()]
