@@ -509,9 +509,9 @@ p100_status p100_paged_append_rope(const p100_paged_desc* desc, const void* qkv,
  * causal is not read.  A sequence with more than 32 mask_words new tokens makes
  * the call do nothing and raises P100_ERR_INVALID in p100_device_error().
  * Workspace, outputs, refusals and values that are not finite as
- * p100_fa_paged's (a hidden new token's key may hold anything).  Calls of at
- * most 8 rows a sequence (max_q x n_head_q / n_head_kv; heads of 64: 16) carry
- * each probability in two parts of dtype, others round it once to dtype. */
+ * p100_fa_paged's (a hidden new token's key may hold anything).  Like there, calls
+ * of at most 16 rows a sequence (max_q x n_head_q / n_head_kv) carry each
+ * probability in two parts of dtype, others round it once to dtype. */
 p100_status p100_fa_tree(const p100_paged_desc* desc, const void* q, const void* k_pages, const void* v_pages,
                          const unsigned* mask, int mask_words, const int* block_table, const int* q_start,
                          const int* kv_len, void* o, float* lse, void* ws, size_t ws_bytes, p100_stream_t stream);

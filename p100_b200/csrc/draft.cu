@@ -78,15 +78,21 @@ const char* words_reason(int mask_words) {
     return mask_words < 1 || mask_words > P100_TREE_MAX_WORDS ? "mask_words must be between 1 and 32" : nullptr;
 }
 
-// The tensor-core kernel takes all but the smallest trees.  Two tokens of 48
-// sequences of 8192 (64 / 8 heads: 16 rows a kv head) 163 us, on the mma.sync
-// kernel 179; of one sequence of 4096 (32 / 8 heads) with four tokens 16.6 and 23.2;
-// up to 8 rows that kernel's half-empty products are the cheaper ones (one token
-// of the 48: 181 and 176; 64 sequences of 512 with 32 heads and 8 tokens 111 and
-// 82), and with heads of 64, whose tiles are half as long, up to 16 (13 trees of 5
-// over 3001: 25 and 22).
-bool fa_tree_on_tc(const paged::Desc& d, int head_dim) {
-    return (long long)d.max_q * d.group > (head_dim == 64 ? fap::kRows : fap::kRows / 2);
+// Which kernel takes a call of so many rows a kv head (max_q x group).  Up to 16 both
+// carry the probabilities in two parts, so the choice is one of time alone.
+//   over 16        tensor cores (tcgen05), probabilities rounded once
+//   9 to 16, D 128 tensor cores where the row tiles are fewer than the SMs (one
+//                  sequence of 4096, 32 / 8 heads, 4 tokens: 17.7 us, on mma.sync
+//                  23.7; 16 of them 44.4 and 45.2), else mma.sync (48 of 8192, 64 / 8
+//                  heads, 2 tokens: 176 us, on tensor cores 182; 64 of 512, 32 / 32
+//                  heads, 16 tokens: 116 and 130)
+//   else           mma.sync (one token of the 48: 170 us and 200; 64 of 512, 32 / 32
+//                  heads, 8 tokens: 83 and 123; heads of 64, 16 rows: 64 of 512 27
+//                  and 44, 13 trees of 5 over 3001 21 and 33, one of 4096 16.4 and 16.4)
+bool fa_tree_on_tc(const paged::Desc& d, int head_dim, int sms) {
+    const long long rows = (long long)d.max_q * d.group;
+    if (rows > fap::kRows) return true;
+    return head_dim == 128 && rows > fap::kRows / 2 && (long long)d.n_seq * d.n_head_kv < sms;
 }
 
 template <typename T, int D, bool SPARE>
@@ -102,18 +108,18 @@ p100_status launch_fa_tree_mma(const fap::Params& prm, int sms, cudaStream_t str
 }
 template <typename T>
 p100_status launch_fa_tree_mma_d(const fap::Params& prm, int head_dim, int sms, cudaStream_t s) {
-    if (head_dim == 128) return launch_fa_tree_mma<T, 128, true>(prm, sms, s);
     // 8 rows a kv head or fewer: the second parts of their probabilities take the other 8
-    return (long long)prm.d.max_q * prm.d.group <= fap::kRows / 2 ? launch_fa_tree_mma<T, 64, true>(prm, sms, s)
-                                                                  : launch_fa_tree_mma<T, 64, false>(prm, sms, s);
+    const bool spare = (long long)prm.d.max_q * prm.d.group <= fap::kRows / 2;
+    if (head_dim == 64) return spare ? launch_fa_tree_mma<T, 64, true>(prm, sms, s) : launch_fa_tree_mma<T, 64, false>(prm, sms, s);
+    return spare ? launch_fa_tree_mma<T, 128, true>(prm, sms, s) : launch_fa_tree_mma<T, 128, false>(prm, sms, s);
 }
 
 static_assert(sizeof(fatr::Cut) <= kCutBytes && fatr::kRows <= fatc::kRows, "workspace");
-template <typename T, int D, bool CAP>
+template <typename T, int D, bool CAP, bool TWO>
 p100_status launch_fa_tree_tc(const fatr::Params& prm, const CUtensorMap& tmk, const CUtensorMap& tmv, int sms,
                               cudaStream_t stream) {
     static thread_local int configured[64] = {};
-    auto kern = fatr::fa_tree_kernel<T, D, CAP>;
+    auto kern = fatr::fa_tree_kernel<T, D, CAP, TWO>;
     constexpr size_t fixed = fatr::smem_bytes<D>();
     if (p100_status st = allow_smem(kern, fixed + paged::Lengths::bytes(paged::kMaxSeq), configured,
                                     "cudaFuncSetAttribute(fa_tree)"))
@@ -137,10 +143,13 @@ p100_status launch_fa_tree_tc_d(const fatr::Params& prm, int head_dim, const CUt
                                 int sms, cudaStream_t s) {
     const bool cap = prm.softcap != 0.0f;
     if (head_dim == 64)
-        return cap ? launch_fa_tree_tc<T, 64, true>(prm, tmk, tmv, sms, s)
-                   : launch_fa_tree_tc<T, 64, false>(prm, tmk, tmv, sms, s);
-    return cap ? launch_fa_tree_tc<T, 128, true>(prm, tmk, tmv, sms, s)
-               : launch_fa_tree_tc<T, 128, false>(prm, tmk, tmv, sms, s);
+        return cap ? launch_fa_tree_tc<T, 64, true, false>(prm, tmk, tmv, sms, s)
+                   : launch_fa_tree_tc<T, 64, false, false>(prm, tmk, tmv, sms, s);
+    if ((long long)prm.d.max_q * prm.d.group <= fap::kRows)
+        return cap ? launch_fa_tree_tc<T, 128, true, true>(prm, tmk, tmv, sms, s)
+                   : launch_fa_tree_tc<T, 128, false, true>(prm, tmk, tmv, sms, s);
+    return cap ? launch_fa_tree_tc<T, 128, true, false>(prm, tmk, tmv, sms, s)
+               : launch_fa_tree_tc<T, 128, false, false>(prm, tmk, tmv, sms, s);
 }
 
 }  // namespace
@@ -287,7 +296,7 @@ p100_status p100_fa_tree(const p100_paged_desc* desc, const void* q, const void*
         return set_error(P100_ERR_INVALID, "q, o and the pages must be 16-byte aligned");
     prm.d.causal = 0;
     prm.d.max_q = std::min(prm.d.max_q, 32 * mask_words);
-    const bool on_tc = fa_tree_on_tc(prm.d, desc->head_dim);
+    const bool on_tc = fa_tree_on_tc(prm.d, desc->head_dim, sms);
     if (sms > fatr::kJoinThreads) return set_error(P100_ERR_UNSUPPORTED, "more SMs than the joining kernel expects");
     if (on_tc ? fa_paged_too_long(prm.d, fatr::kRows, fatr::kKeys, fatr::kOver)
               : fa_paged_too_long(prm.d, fap::kRows, fap::kKeys, fap::kOver))

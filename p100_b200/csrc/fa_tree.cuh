@@ -27,7 +27,10 @@
 // many products again, and both the products and the energy they take count here
 // (48 trees of 8 over 8192 tokens, 64 / 8 heads: 144 us, 0.86 of measured bandwidth,
 // at the 1000 W cap that streaming the cache alone comes near; two parts took a
-// fifth more).
+// fifth more).  Calls of at most 16 rows a kv head carry them in two (TWO), as
+// fa_paged.cuh does for as many rows: a short draft keeps the digits that its
+// tokens have one by one (one sequence of 4096, 32 / 8 heads, 4 tokens: 17.7 us, with
+// one part 16.4).  Both parts take the scores' place in tensor memory.
 #pragma once
 #include "fa_paged_tc.cuh"
 
@@ -281,7 +284,7 @@ __device__ __forceinline__ void gather_role(const Params& p, Barriers& bars, uin
 }
 
 // Issues the products; false when a wait was given up.
-template <typename T, int D>
+template <typename T, int D, bool TWO>
 __device__ __forceinline__ bool mma_role(const Desc& d, float scale, bool gathered, Barriers& bars, uint32_t q_smem,
                                          uint32_t ring, uint32_t tmem) {
     constexpr int NS = slots<D>();
@@ -308,9 +311,12 @@ __device__ __forceinline__ bool mma_role(const Desc& d, float scale, bool gather
     };
     auto pv = [&](int w, int half, unsigned slot, bool add) {   // O_w += P_w V over half of the keys
 #pragma unroll
-        for (int k = half * (kKeys / 32); k < (half + 1) * (kKeys / 32); ++k)
-            fatc::mma_ts(tmem + 256 + w * D, tmem + w * 128 + k * 8,
-                         fatc::sw128_desc(ring + slot * tile_bytes<D>() + uint32_t(k) * 2048, kSub, 1024), kIdescO, add || k > 0);
+        for (int part = 0; part < (TWO ? 2 : 1); ++part)
+#pragma unroll
+            for (int k = half * (kKeys / 32); k < (half + 1) * (kKeys / 32); ++k)
+                fatc::mma_ts(tmem + 256 + w * D, tmem + w * 128 + part * 64 + k * 8,
+                             fatc::sw128_desc(ring + slot * tile_bytes<D>() + uint32_t(k) * 2048, kSub, 1024), kIdescO,
+                             add || part > 0 || k > 0);
     };
     for (unsigned j = 0;; ++j) {
         if (!warp_wait(&bars.job_full[j % kJobs], (j / kJobs) & 1, &bars.abort)) return false;
@@ -417,7 +423,7 @@ __device__ __forceinline__ void write_lse(const Params& p, int token, int head, 
         p.lse[(long long)token * p.d.n_head_q + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) / 1.4426950408889634f;
 }
 
-template <typename T, int D, bool CAP>
+template <typename T, int D, bool CAP, bool TWO>
 __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, uint32_t q_smem, uint8_t* ring, uint32_t tmem,
                                              long long total_units, int parts) {
     constexpr int NS = slots<D>();
@@ -553,7 +559,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
             for (int half = 0; half < 2; ++half) {   // the products with the first half start while the second is computed
 #pragma unroll
                 for (int i = 4 * half; i < 4 * half + 4; ++i) {
-                    uint32_t pk[8];
+                    uint32_t pk[8], rest[8];
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
                         const uint64_t x = pair(s[i * 16 + e], s[i * 16 + e + 1]);
@@ -570,8 +576,14 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
                         b = paged::exp2_approx(b);
                         sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair(a, b));
                         pk[e >> 1] = paged::pack2<T>(a, b);
+                        if (TWO) {
+                            float high_a, high_b;
+                            paged::unpack2<T>(pk[e >> 1], high_a, high_b);
+                            rest[e >> 1] = paged::pack2<T>(a - high_a, b - high_b);
+                        }
                     }
                     fatc::st8(t_s + i * 8, pk);
+                    if (TWO) fatc::st8(t_s + 64 + i * 8, rest);
                 }
                 fatc::wait_st();
                 if (half == 0 && !clear_v(t, key0)) return;
@@ -640,7 +652,7 @@ __device__ __forceinline__ void softmax_role(const Params& p, Barriers& bars, ui
     }
 }
 
-template <typename T, int D, bool CAP>
+template <typename T, int D, bool CAP, bool TWO>
 __global__ void __launch_bounds__(kThreads, 1)
     fa_tree_kernel(const Params p, const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv) {
     extern __shared__ uint8_t smem_raw[];
@@ -697,14 +709,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem);
     if (warp < kMmaWarp) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(fatc::kSoftmaxRegs));
-        softmax_role<T, D, CAP>(p, bars, smem_addr(q_smem), ring, tmem, len.head->total, parts);
+        softmax_role<T, D, CAP, TWO>(p, bars, smem_addr(q_smem), ring, tmem, len.head->total, parts);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(fatc::kIssueRegs));
         if (warp == kLoadWarp) {
             load_role<D>(p, &tmk, &tmv, len, bars, ring, share);
         } else if (warp == kMmaWarp) {
-            if (!mma_role<T, D>(p.d, p.scale, p.box == 0, bars, fatc::uniform(smem_addr(q_smem)), fatc::uniform(smem_addr(ring)),
-                                fatc::uniform(tmem))) {
+            if (!mma_role<T, D, TWO>(p.d, p.scale, p.box == 0, bars, fatc::uniform(smem_addr(q_smem)),
+                                     fatc::uniform(smem_addr(ring)), fatc::uniform(tmem))) {
                 // leave only when the products in flight are done
                 fatc::mma_commit(&bars.drain);
                 __syncwarp();
