@@ -521,8 +521,11 @@ p100_status p100_fa_tree(const p100_paged_desc* desc, const void* q, const void*
  * the path of an accepted draft), in the pages' place; rows behind them stay as
  * they are.  length[s] = kv_len - n + keep_len[s], the next plan's length
  * (may be NULL; it must not overlap the other arrays, nor k_pages be v_pages:
- * refused).  A keep_len outside [0, n] leaves its sequence out, an index
- * out of order or range its row; both, and pages out of range, raise
+ * refused).  keep_len of a sequence without new tokens is not looked at: after a
+ * plan that lacked pages the call changes nothing and length = kv_len.  A keep_len
+ * outside [0, n] keeps nothing (length = kv_len - n), starts out of order or range
+ * or a kv_len that does not fit leave their sequence out (length = kv_len), an
+ * index out of order or range its row; all three, and pages out of range, raise
  * P100_ERR_INVALID in p100_device_error().  Sequences may not share the pages
  * that hold new tokens. */
 p100_status p100_paged_keep(const p100_paged_desc* desc, void* k_pages, void* v_pages, const int* keep,

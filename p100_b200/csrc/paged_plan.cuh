@@ -246,13 +246,14 @@ constexpr int kKeepThreads = 128, kKeepRows = 8;
 __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const KeepParams p, int chunks) {
     const Desc& d = p.d;
     const int s = blockIdx.y, lane = threadIdx.x & 31;
-    const int q0 = d.q_start[s], n = d.q_start[s + 1] - q0, kv = d.kv_len[s], kept = p.keep_len[s];
-    if (q0 < 0 || n < 0 || q0 > d.n_tokens - n || kv < n || kv > (long long)d.max_pages * d.page_size || kept < 0 ||
-        kept > n) {
-        if (threadIdx.x == 0) flag_input();
-        return;
-    }
-    if (p.length && blockIdx.x == 0 && threadIdx.x == 0) p.length[s] = kv - n + kept;
+    const int q0 = d.q_start[s], n = d.q_start[s + 1] - q0, kv = d.kv_len[s], asked = p.keep_len[s];
+    const bool usable = q0 >= 0 && n >= 0 && q0 <= d.n_tokens - n && kv >= n && kv <= (long long)d.max_pages * d.page_size;
+    const bool counted = asked >= 0 && asked <= n;
+    const int kept = usable && counted ? asked : 0;
+    // every sequence gets a length that the next plan can take; one without new
+    // tokens (a step that lacked pages has none) keeps its own, whatever was asked
+    if (p.length && blockIdx.x == 0 && threadIdx.x == 0) p.length[s] = usable ? kv - n + kept : kv;
+    if (threadIdx.x == 0 && (!usable || (!counted && n > 0))) flag_input();
     const int column = blockIdx.x * kKeepThreads + threadIdx.x, per = d.n_head_kv * chunks;
     const bool mine = column < 2 * per;
     const int c = column % per;
