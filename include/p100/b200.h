@@ -360,7 +360,9 @@ typedef struct p100_paged_desc {
  * heads as they are; q to q, k and v to their row in the pages.  FP32
  * arithmetic, one rounding (nearest even) to dtype.  Neither q nor the pages
  * may overlap qkv.  A token whose position lies outside [0, max_pos) of the table
- * or outside the block table is left out and raises P100_ERR_INVALID in p100_device_error(). */
+ * or behind the max_pages pages of its block table is left out; one whose entry
+ * there is no page has its query written, its key and value not.  Both raise
+ * P100_ERR_INVALID in p100_device_error(). */
 p100_status p100_paged_append(const p100_paged_desc* desc, const void* qkv, int qkv_type, long long qkv_stride,
                               const float* q_norm, const float* k_norm, float eps, const float* rope_cs, int max_pos,
                               int rope_half, const int* block_table, const int* q_start, const int* kv_len, void* q,
@@ -495,8 +497,9 @@ p100_status p100_rope_init(p100_rope* rope, int rope_dim, int half, double theta
  * sequence, where its row in the cache is in any case): angles to 2^-24 of a
  * half turn at every position up to 2^31 - 1, without a table.  The other values
  * of a head are kept.  mscale multiplies the rotated values.  A token with a
- * negative position or without a place in the block table is left out and raises
- * P100_ERR_INVALID in p100_device_error(). */
+ * negative position or behind the max_pages pages of its table is left out; one
+ * whose table entry is no page (-1, say) has its query written, its key and value
+ * not.  Both raise P100_ERR_INVALID in p100_device_error(). */
 p100_status p100_paged_append_rope(const p100_paged_desc* desc, const void* qkv, int qkv_type, long long qkv_stride,
                                    const float* q_norm, const float* k_norm, float eps, const p100_rope* rope,
                                    const int* position, const int* block_table, const int* q_start, const int* kv_len,
