@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
                 if (missing < 0) flag_input();
             }
         }
-        for (int t = me; t < p.n_tokens; t += all) {
+        for (unsigned t = me; t < unsigned(p.n_tokens); t += all) {
             if (p.slot) p.slot[t] = -1;
             if (p.position) p.position[t] = -1;
         }
@@ -134,18 +134,22 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
     }
     const int tokens = int(total[0]), give = int(total[1]), take = int(total[2]), top = count + give - 1;
     int* stack = p.pool + 2;
-    for (int r = me; r < give; r += all) {
+    // (the counters pass 2^31 - 1 behind the last of as many rows or pages)
+    for (unsigned i = me; i < unsigned(give); i += all) {
+        const int r = int(i);
         const int s = last_at(s_give, p.n_seq, r);
         int* entry = p.block_table + (long long)s * p.max_pages + s_need[s] + (r - s_give[s]);
         stack[top - r] = *entry;
         *entry = -1;
     }
     cluster_meet();
-    for (int k = me; k < take; k += all) {
+    for (unsigned i = me; i < unsigned(take); i += all) {
+        const int k = int(i);
         const int s = last_at(s_take, p.n_seq, k);
         p.block_table[(long long)s * p.max_pages + s_held[s] + (k - s_take[s])] = stack[top - k];
     }
-    for (int t = me; t < p.n_tokens; t += all) {
+    for (unsigned i = me; i < unsigned(p.n_tokens); i += all) {
+        const int t = int(i);
         int pos = -1;
         long long slot = -1;
         if (t < tokens) {
@@ -259,7 +263,8 @@ __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const KeepPara
     const int c = column % per;
     uint4* base = (column < per ? p.k : p.v) + (c / chunks) * (d.head_stride / 8) + c % chunks;
     const int* table = d.block_table + (long long)s * d.max_pages;
-    for (int i0 = 0; i0 < kept; i0 += 32) {
+    for (unsigned at0 = 0; at0 < unsigned(kept); at0 += 32) {   // (at0 may pass 2^31 - 1)
+        const int i0 = int(at0);
         long long from = -1, to = -1;   // of row i0 + lane, in 16 bytes; -1: stays
         if (i0 + lane < kept) {
             const int j = p.keep[q0 + i0 + lane], before = i0 + lane ? p.keep[q0 + i0 + lane - 1] : -1;
