@@ -2,10 +2,11 @@
 // quantised mat-vec and FlashAttention decode paths, plus library plumbing
 // (status text, device checks, the bounded-wait flag).
 //
-// One of two CUDA translation units (serve.cu holds the paged cache and the
-// scoring of logits): the headers of the decode path are all included here, so
-// its kernels share one g_device_error word per device; p100_device_error
-// reports serve.cu's and draft.cu's words too.
+// One of three CUDA translation units (serve.cu holds the paged cache and the
+// scoring of logits, draft.cu steps and drafted trees over the paged cache): the
+// headers of the decode path are all included here, so its kernels share one
+// g_device_error word per device; p100_device_error reports serve.cu's and
+// draft.cu's words too.
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>

@@ -45,7 +45,7 @@ p100_status cuda_status(cudaError_t err, const char* what);
 void clear_error();
 p100_status require_sm100(int* device_out, int* sm_count_out);
 bool fault_injected(const char* name);
-// In capi.cu (the CUDA translation unit).
+// In capi.cu.
 p100_status peer_allreduce(float* buf, size_t count, unsigned long long* const* slots, int world, int rank, int n_cap,
                            int* epoch, int* ticket, int* broken, unsigned long long wait_ns, cudaStream_t stream);
 float* tp_setup_scratch();
