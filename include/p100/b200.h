@@ -417,7 +417,8 @@ p100_status p100_logprobs(const void* logits, int dtype, int n, int rows, long l
  * p100_paged_plan gives the new tokens their pages, starts, slots and positions,
  * p100_tree_mask turns the drafts' parents into masks and positions, then in
  * every layer p100_paged_append_rope and p100_fa_tree; when the caller has
- * chosen the tokens to keep, p100_paged_keep moves their rows in every layer,
+ * chosen the tokens to keep (on the device: with a kernel of its own that
+ * compares the logits with the drafts), p100_paged_keep moves their rows in every layer,
  * and the next plan starts from the lengths it returns.  No reference
  * counterpart.  Everything about a request is int32 in device memory and read
  * when the kernels run, so one captured graph serves all steps. */

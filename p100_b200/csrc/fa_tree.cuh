@@ -25,7 +25,7 @@
 // The probabilities are rounded once to the cache's 16-bit type, as fa_paged_tc.cuh
 // does and for its reason: a second part (what the rounding left) would be half as
 // many products again, and both the products and the energy they take count here
-// (48 trees of 8 over 8192 tokens, 64 / 8 heads: 144 us, 0.86 of measured bandwidth,
+// (48 trees of 8 over 8192 tokens, 64 / 8 heads: 143 to 150 us, 0.83 to 0.87 of measured bandwidth,
 // at the 1000 W cap that streaming the cache alone comes near; two parts took a
 // fifth more).  Calls of at most 16 rows a kv head carry them in two (TWO), as
 // fa_paged.cuh does for as many rows: a short draft keeps the digits that its
@@ -54,7 +54,10 @@ using paged::unpair;
 constexpr int kRows = 128, kKeys = 128;
 constexpr int kOver = 4;                  // what a row tile costs beyond its keys, in units (48 trees of 8: 145 us, with 2 152)
 constexpr int kMinUnits = 2;              // of a share: a tile for each warpgroup
-constexpr int kWholeFrom = 4;             // row tiles per CTA from which they are dealt out whole
+// Row tiles per CTA from which they are dealt out whole.  64 / 8 heads, trees of 8:
+// 5.4 of up to 2048 tokens 106 us either way, of 512 55 (cut 66); 3.5 of 2048 82 (cut
+// 72), of 512 38 (cut 43).
+constexpr int kWholeFrom = 4;
 constexpr int kThreads = fatc::kThreads;
 constexpr int kMmaWarp = fatc::kMmaWarp, kLoadWarp = fatc::kLoadWarp, kGatherWarp = fatc::kGatherWarp;
 

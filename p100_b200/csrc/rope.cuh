@@ -23,7 +23,7 @@
 // shared memory for the k heads.  Blocks of four warps, five an SM: with eight the
 // last ones leave SMs idle (30 us), with six of four the registers spill (27.5), with
 // four too few warps are there (35).
-// Measured: 2,622 tokens of 64 / 8 heads of 128 from bf16 with norms and halves
+// Measured: 2,777 tokens of 64 / 8 heads of 128 from bf16 with norms and halves
 // 24.4 us, 0.71 of measured bandwidth; 8,192 of them from fp32 with norms 92 us,
 // 0.83.
 #pragma once
